@@ -1,0 +1,70 @@
+// Internal launch interface of chunk attention over a paged, possibly
+// quantised KV cache (not part of the public C ABI; see include/dllm_attn.h).
+#pragma once
+
+#include <cstdint>
+#include <cuda_runtime.h>
+#include <cuda_bf16.h>
+
+namespace dllm {
+
+struct ChunkArgs {
+  const __nv_bfloat16* q;  // [total_q, Hq, 128]
+  int64_t q_stride;        // elements between token rows
+  const __nv_bfloat16* k;  // fresh rows [total_k, Hkv, 128], or null
+  int64_t k_stride;
+  const __nv_bfloat16* v;
+  int64_t v_stride;
+  const uint8_t* kc;       // cache: slot rows of Hkv * 128 elements (bf16) or codes
+  const uint8_t* vc;
+  const uint8_t* k_exp;    // exponent bytes of a quantised cache: slot rows of Hkv bytes
+  const uint8_t* v_exp;
+  int64_t num_slots;
+  const int32_t* slots;    // slot list (cached rows of sequence b: slots[cu_s[b] .. cu_s[b+1])) or null
+  const int32_t* cu_s;
+  int64_t total_slots;
+  const int32_t* tables;   // block tables [B, table_stride], or null
+  int64_t table_stride;
+  int max_blocks;          // entries of a table row
+  int block_size;          // slots of a block
+  int block_shift;         // log2(block_size), or -1
+  const int32_t* ctx;      // cached rows per sequence (with tables)
+  int max_context;         // no sequence has more cached rows
+  const int32_t* cu_q;
+  const int32_t* cu_k;     // fresh rows per sequence, or null
+  int64_t total_q;
+  int64_t total_k;
+  int max_q;
+  int max_fresh;           // no sequence has more fresh rows
+  int B;
+  int Hq;
+  int Hkv;
+  int group;               // Hq / Hkv
+  float scale_log2;        // softmax_scale * log2(e)
+  int causal;
+  __nv_bfloat16* o;
+  int64_t o_stride;
+  int32_t* err;
+  // set by the launcher
+  int mtiles;              // row tiles per (sequence, KV head)
+  int splits;              // key splits per row tile
+  int split_chunks;        // key chunks of a split
+  float* part_o;           // [items * splits, rows, 128] partial outputs (splits > 1)
+  float2* part_ml;         // [items * splits, rows] (maximum, sum)
+};
+
+// How a launch is laid out, from sizes the host knows.
+struct ChunkPlan {
+  int mt;                  // 16-row tiles of a warp (1 or 2)
+  int mtiles;
+  int splits;
+  int split_chunks;
+  int64_t workspace_bytes;
+};
+
+ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int max_context, int max_fresh,
+                          int num_sms);
+
+cudaError_t launch_attn_chunk(ChunkArgs a, int format, const ChunkPlan& plan, void* workspace, cudaStream_t stream);
+
+}  // namespace dllm

@@ -10,6 +10,8 @@
 #include "dllm_attn.h"
 #include "attn_fwd.h"
 #include "kvcache.h"
+#include "kvquant.h"
+#include "attn_chunk.h"
 #include "select_kv.h"
 #include "rope.h"
 #include "step_plan.h"
@@ -291,6 +293,60 @@ int kv_copy_common(bool store, const void* key, int64_t key_stride, const void* 
   return DLLM_OK;
 }
 
+int kv_quant_common(bool store, const void* key, int64_t key_stride, const void* value, int64_t value_stride,
+                    const void* k_cache, const void* v_cache, const void* k_exp, const void* v_exp,
+                    const int32_t* slots, int64_t n_tokens, int heads, int head_dim, int format,
+                    int64_t num_slots, int32_t* err, void* stream) {
+  if (format != DLLM_KV_E4M3 && format != DLLM_KV_INT8)
+    return fail(DLLM_ERR_UNSUPPORTED, "format %d is not a quantised cache format", format);
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return fail(DLLM_ERR_UNSUPPORTED, "head_dim %d not supported (64, 128 or 256)", head_dim);
+  if (n_tokens < 0 || heads <= 0 || num_slots < 0) return fail(DLLM_ERR_INVALID_ARG, "negative size");
+  if (heads > (1 << 16)) return fail(DLLM_ERR_TOO_LARGE, "num_kv_heads %d too large", heads);
+  if (n_tokens == 0) return DLLM_OK;
+  if (!key || !value || !k_cache || !v_cache || !k_exp || !v_exp || !slots)
+    return fail(DLLM_ERR_INVALID_ARG, "null pointer");
+  const int64_t row = (int64_t)heads * head_dim;
+  if (key_stride < row || value_stride < row)
+    return fail(DLLM_ERR_INVALID_ARG, "token stride smaller than the cache row");
+  if (!aligned(key, 16) || !aligned(value, 16) || key_stride % 8 != 0 || value_stride % 8 != 0)
+    return fail(DLLM_ERR_ALIGNMENT, "key/value rows must start on 16-byte boundaries");
+  if (!aligned(k_cache, 16) || !aligned(v_cache, 16))
+    return fail(DLLM_ERR_ALIGNMENT, "caches must be 16-byte aligned");
+  if (n_tokens > ((int64_t)1 << 38) / row) return fail(DLLM_ERR_TOO_LARGE, "too many rows");
+  dllm::KvQuantArgs a;
+  a.key = const_cast<void*>(key);
+  a.value = const_cast<void*>(value);
+  a.key_stride = key_stride;
+  a.value_stride = value_stride;
+  a.k_cache = static_cast<uint8_t*>(const_cast<void*>(k_cache));
+  a.v_cache = static_cast<uint8_t*>(const_cast<void*>(v_cache));
+  a.k_exp = static_cast<uint8_t*>(const_cast<void*>(k_exp));
+  a.v_exp = static_cast<uint8_t*>(const_cast<void*>(v_exp));
+  a.slots = slots;
+  a.n_tokens = n_tokens;
+  a.num_slots = num_slots;
+  a.heads = heads;
+  a.err = err;
+  const bool wide = aligned(key, 32) && aligned(value, 32) && key_stride % 16 == 0 && value_stride % 16 == 0;
+  cudaError_t e = dllm::launch_kv_quant(a, store, format, head_dim, wide, reinterpret_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, store ? "store_kvcache_quant launch" : "load_kvcache_quant launch");
+  return DLLM_OK;
+}
+
+// Sizes of a chunk-attention launch; DLLM_OK or an error.
+int check_chunk_sizes(int format, int batch, int Hq, int Hkv, int max_q, int max_context, int max_fresh) {
+  if (format != DLLM_KV_BF16 && format != DLLM_KV_E4M3 && format != DLLM_KV_INT8)
+    return fail(DLLM_ERR_UNSUPPORTED, "cache format %d not supported", format);
+  if (Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0)
+    return fail(DLLM_ERR_UNSUPPORTED, "num_heads %d must be a positive multiple of num_kv_heads %d", Hq, Hkv);
+  if (batch < 0 || max_q < 0 || max_context < 0 || max_fresh < 0)
+    return fail(DLLM_ERR_INVALID_ARG, "negative size");
+  if (max_context > (1 << 30) || max_fresh > (1 << 30) || (int64_t)max_q * (Hq / Hkv) > (1 << 30))
+    return fail(DLLM_ERR_TOO_LARGE, "more than 2^30 rows of a sequence");
+  return DLLM_OK;
+}
+
 // Scheduler workspace of dllm_attn_varlen_fwd_static_ws: file-scope device
 // memory (one copy per device, zero when the module loads). The attention
 // kernel uses the first DLLM_SCHED_WORKSPACE_INTS words and leaves them zero;
@@ -338,6 +394,128 @@ int dllm_load_kvcache(void* key, int64_t key_stride, void* value, int64_t value_
                       int32_t* err_flag, void* stream) {
   return kv_copy_common(false, key, key_stride, value, value_stride, k_cache, v_cache,
                         slot_mapping, n_tokens, row_elems, elem_bytes, num_slots, err_flag, stream);
+}
+
+int dllm_store_kvcache_quant(const void* key, int64_t key_stride, const void* value, int64_t value_stride,
+                             void* k_cache, void* v_cache, void* k_exp, void* v_exp,
+                             const int32_t* slot_mapping, int64_t n_tokens, int num_kv_heads, int head_dim,
+                             int format, int64_t num_slots, int32_t* err_flag, void* stream) {
+  return kv_quant_common(true, key, key_stride, value, value_stride, k_cache, v_cache, k_exp, v_exp, slot_mapping,
+                         n_tokens, num_kv_heads, head_dim, format, num_slots, err_flag, stream);
+}
+
+int dllm_load_kvcache_quant(void* key, int64_t key_stride, void* value, int64_t value_stride,
+                            const void* k_cache, const void* v_cache, const void* k_exp, const void* v_exp,
+                            const int32_t* slot_mapping, int64_t n_tokens, int num_kv_heads, int head_dim,
+                            int format, int64_t num_slots, int32_t* err_flag, void* stream) {
+  return kv_quant_common(false, key, key_stride, value, value_stride, k_cache, v_cache, k_exp, v_exp, slot_mapping,
+                         n_tokens, num_kv_heads, head_dim, format, num_slots, err_flag, stream);
+}
+
+int64_t dllm_attn_chunk_workspace(int format, int batch, int num_heads, int num_kv_heads, int max_seqlen_q,
+                                  int max_context, int max_fresh) {
+  if (check_chunk_sizes(format, batch, num_heads, num_kv_heads, max_seqlen_q, max_context, max_fresh) != DLLM_OK)
+    return -1;
+  if (batch == 0 || max_seqlen_q == 0) return 0;
+  return dllm::plan_attn_chunk(format, batch, num_kv_heads, num_heads / num_kv_heads, max_seqlen_q, max_context,
+                               max_fresh, num_sms_of_current_device())
+      .workspace_bytes;
+}
+
+int dllm_attn_chunk_fwd(const void* q, int64_t q_tok_stride, const void* k, int64_t k_tok_stride, const void* v,
+                        int64_t v_tok_stride, const void* k_cache, const void* v_cache, const void* k_exp,
+                        const void* v_exp, int format, int64_t num_slots, const int32_t* block_tables,
+                        int64_t table_stride, int max_blocks, int block_size, const int32_t* context_lens,
+                        const int32_t* slots, const int32_t* cu_seqlens_slots, int64_t total_slots,
+                        int max_context, void* o, int64_t o_tok_stride, const int32_t* cu_seqlens_q,
+                        const int32_t* cu_seqlens_k, int batch, int max_seqlen_q, int max_fresh, int64_t total_q,
+                        int64_t total_k, int num_heads, int num_kv_heads, int head_dim, float softmax_scale,
+                        int causal, void* workspace, int64_t workspace_bytes, int32_t* err_flag, void* stream) {
+  if (head_dim != 128) return fail(DLLM_ERR_UNSUPPORTED, "head_dim %d not supported (only 128)", head_dim);
+  int rc = check_chunk_sizes(format, batch, num_heads, num_kv_heads, max_seqlen_q, max_context, max_fresh);
+  if (rc != DLLM_OK) return rc;
+  if (total_q < 0 || total_k < 0 || total_slots < 0 || num_slots < 0)
+    return fail(DLLM_ERR_INVALID_ARG, "negative size");
+  if (num_slots >= (int64_t)1 << 31) return fail(DLLM_ERR_TOO_LARGE, "too many cache slots");
+  if (!(softmax_scale > 0.f)) return fail(DLLM_ERR_INVALID_ARG, "softmax_scale must be > 0");
+  if (block_tables != nullptr && slots != nullptr)
+    return fail(DLLM_ERR_INVALID_ARG, "block tables and a slot list are both given");
+  const bool cached = block_tables != nullptr || slots != nullptr;
+  if (block_tables != nullptr) {
+    if (context_lens == nullptr) return fail(DLLM_ERR_INVALID_ARG, "block_tables without context_lens");
+    if (block_size <= 0 || max_blocks < 0 || table_stride < max_blocks)
+      return fail(DLLM_ERR_INVALID_ARG, "bad block table shape");
+  }
+  if (slots != nullptr && cu_seqlens_slots == nullptr)
+    return fail(DLLM_ERR_INVALID_ARG, "slots without cu_seqlens_slots");
+  if (cached && (k_cache == nullptr || v_cache == nullptr)) return fail(DLLM_ERR_INVALID_ARG, "cache is null");
+  if (cached && format != DLLM_KV_BF16 && (k_exp == nullptr || v_exp == nullptr))
+    return fail(DLLM_ERR_INVALID_ARG, "a quantised cache needs k_exp and v_exp");
+  if (!aligned(k_cache, 16) || !aligned(v_cache, 16))
+    return fail(DLLM_ERR_ALIGNMENT, "caches must be 16-byte aligned");
+  if ((k == nullptr) != (v == nullptr) || (k == nullptr) != (cu_seqlens_k == nullptr))
+    return fail(DLLM_ERR_INVALID_ARG, "k, v and cu_seqlens_k are given together");
+  if (batch == 0 || total_q == 0 || max_seqlen_q == 0) return DLLM_OK;
+  if (cu_seqlens_q == nullptr) return fail(DLLM_ERR_INVALID_ARG, "cu_seqlens_q is null");
+  if ((rc = check_rows("q", q, q_tok_stride, num_heads, total_q)) != DLLM_OK) return rc;
+  if ((rc = check_rows("o", o, o_tok_stride, num_heads, total_q)) != DLLM_OK) return rc;
+  if (k != nullptr) {
+    if ((rc = check_rows("k", k, k_tok_stride, num_kv_heads, total_k)) != DLLM_OK) return rc;
+    if ((rc = check_rows("v", v, v_tok_stride, num_kv_heads, total_k)) != DLLM_OK) return rc;
+  }
+  if (!cached) max_context = 0;
+  if (k == nullptr) max_fresh = 0;
+  const dllm::ChunkPlan plan =
+      dllm::plan_attn_chunk(format, batch, num_kv_heads, num_heads / num_kv_heads, max_seqlen_q, max_context,
+                            max_fresh, num_sms_of_current_device());
+  if (plan.workspace_bytes > 0) {
+    if (workspace == nullptr || workspace_bytes < plan.workspace_bytes)
+      return fail(DLLM_ERR_INVALID_ARG, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
+                  (long long)plan.workspace_bytes);
+    if (!aligned(workspace, 16)) return fail(DLLM_ERR_ALIGNMENT, "workspace is not 16-byte aligned");
+  }
+  dllm::ChunkArgs a = {};
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.q_stride = q_tok_stride;
+  a.k = static_cast<const __nv_bfloat16*>(k);
+  a.k_stride = k_tok_stride;
+  a.v = static_cast<const __nv_bfloat16*>(v);
+  a.v_stride = v_tok_stride;
+  a.kc = static_cast<const uint8_t*>(k_cache);
+  a.vc = static_cast<const uint8_t*>(v_cache);
+  a.k_exp = static_cast<const uint8_t*>(k_exp);
+  a.v_exp = static_cast<const uint8_t*>(v_exp);
+  a.num_slots = num_slots;
+  a.slots = slots;
+  a.cu_s = cu_seqlens_slots;
+  a.total_slots = total_slots;
+  a.tables = block_tables;
+  a.table_stride = table_stride;
+  a.max_blocks = max_blocks;
+  a.block_size = block_tables != nullptr ? block_size : 1;
+  a.block_shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if (a.block_size == 1 << s) a.block_shift = s;
+  a.ctx = context_lens;
+  a.max_context = max_context;
+  a.cu_q = cu_seqlens_q;
+  a.cu_k = cu_seqlens_k;
+  a.total_q = total_q;
+  a.total_k = total_k;
+  a.max_q = max_seqlen_q;
+  a.max_fresh = max_fresh;
+  a.B = batch;
+  a.Hq = num_heads;
+  a.Hkv = num_kv_heads;
+  a.group = num_heads / num_kv_heads;
+  a.scale_log2 = softmax_scale * 1.4426950408889634f;
+  a.causal = causal != 0;
+  a.o = static_cast<__nv_bfloat16*>(o);
+  a.o_stride = o_tok_stride;
+  a.err = err_flag;
+  cudaError_t e = dllm::launch_attn_chunk(a, format, plan, workspace, reinterpret_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "attn_chunk launch");
+  return DLLM_OK;
 }
 
 int dllm_attn_varlen_fwd(const void* q, int64_t q_tok_stride, const void* k, int64_t k_tok_stride,

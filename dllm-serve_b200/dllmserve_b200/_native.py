@@ -21,6 +21,12 @@ DLLM_ERR_CUDA = 5
 DLLM_DEV_SLOT_OUT_OF_RANGE = 1
 DLLM_DEV_WAIT_TIMEOUT = 2
 DLLM_DEV_BAD_SEQUENCE = 3
+DLLM_DEV_POSITION_OUT_OF_RANGE = 4
+DLLM_DEV_NON_FINITE = 5
+
+KV_BF16 = 0  # DLLM_KV_BF16
+KV_E4M3 = 1  # DLLM_KV_E4M3
+KV_INT8 = 2  # DLLM_KV_INT8
 
 SEQ_DESC_INTS = 8
 PLAN_SEQ_FIELDS = 10   # DLLM_PLAN_SEQ_FIELDS
@@ -40,6 +46,20 @@ SIGNATURES = {
     "dllm_last_error": ([], ctypes.c_char_p),
     "dllm_store_kvcache": ([_P, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _I, _I64, _P, _P], _I),
     "dllm_load_kvcache": ([_P, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _I, _I64, _P, _P], _I),
+    "dllm_store_kvcache_quant": (
+        [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, _I64, _I, _I, _I, _I64, _P, _P],
+        _I,
+    ),
+    "dllm_load_kvcache_quant": (
+        [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, _I64, _I, _I, _I, _I64, _P, _P],
+        _I,
+    ),
+    "dllm_attn_chunk_workspace": ([_I, _I, _I, _I, _I, _I, _I], _I64),
+    "dllm_attn_chunk_fwd": (
+        [_P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I, _I64, _P, _I64, _I, _I, _P, _P, _P, _I64, _I,
+         _P, _I64, _P, _P, _I, _I, _I, _I64, _I64, _I, _I, _I, _F, _I, _P, _I64, _P, _P],
+        _I,
+    ),
     "dllm_attn_varlen_fwd": (
         [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I, _I, _I64, _I64, _I, _I, _I, _F, _P, _P, _P],
         _I,

@@ -154,6 +154,79 @@ def _kv_copy(store, key, value, k_cache, v_cache, slot_mapping, D):
 
 
 # ---------------------------------------------------------------------------
+# Quantised KV cache
+# ---------------------------------------------------------------------------
+_KV_FORMATS = {torch.bfloat16: _native.KV_BF16, torch.float8_e4m3fn: _native.KV_E4M3, torch.int8: _native.KV_INT8}
+
+
+def store_kvcache_quant(key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping):
+    """``store_kvcache`` into a quantised cache: the row of every (token, kv
+    head) is stored as 8-bit codes with one power-of-two scale.
+
+    key, value: bfloat16 [N, num_kv_heads, D], D 64, 128 or 256, heads packed;
+    k_cache, v_cache: [blocks, block_size, num_kv_heads, D], contiguous,
+    ``torch.float8_e4m3fn`` or ``torch.int8``; k_exp, v_exp: uint8 [blocks,
+    block_size, num_kv_heads]; slot_mapping: int32 [N], each slot at most once
+    (negative: skipped).
+
+    With a the row's largest finite magnitude and M the format's largest value
+    (448 or 127), the scale is 2^e, e the smallest integer with a <= M * 2^e
+    (clamped to [-100, 119] / [-100, 121]); codes are x * 2^-e rounded to
+    nearest even and the byte e + 127 is kept. Infinities saturate, NaN is kept
+    (e4m3) or becomes 0 (int8); both set DLLM_DEV_NON_FINITE in the device
+    status word."""
+    _kv_quant(True, key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping)
+
+
+def load_kvcache_quant(key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping):
+    """``load_kvcache`` from a cache that ``store_kvcache_quant`` wrote: key,
+    value (bfloat16) receive code * 2^e, exactly. Negative slots give zero
+    rows, and so do slots past the cache, which also set the status word."""
+    _kv_quant(False, key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping)
+
+
+def _check_quant_cache(name, cache, exp, heads, head_dim) -> int:
+    """Validates a quantised cache and its exponent bytes; returns its slots."""
+    if cache.dim() < 3 or cache.shape[-2] != heads or cache.shape[-1] != head_dim or not cache.is_contiguous():
+        raise ValueError(f"{name}_cache must be contiguous [blocks, block_size, {heads}, {head_dim}]")
+    slots = cache.numel() // (heads * head_dim)
+    if exp.dtype is not torch.uint8 or not exp.is_contiguous() or exp.shape[-1] != heads or exp.numel() != slots * heads:
+        raise ValueError(f"{name}_exp must be contiguous uint8 [blocks, block_size, {heads}]")
+    return slots
+
+
+def _kv_quant(store, key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping):
+    if key.dim() != 3 or value.shape != key.shape:
+        raise ValueError("key and value must be [tokens, num_kv_heads, head_dim] of one shape")
+    N, H, D = key.shape
+    if key.dtype is not torch.bfloat16 or value.dtype is not torch.bfloat16:
+        raise ValueError("key and value must be bfloat16")
+    ks, vs = key.stride(), value.stride()
+    if ks[2] != 1 or ks[1] != D or vs[2] != 1 or vs[1] != D:
+        raise ValueError("key and value must have contiguous heads")
+    dev = _require_cuda(key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping)
+    fmt = _KV_FORMATS.get(k_cache.dtype, _native.KV_BF16)
+    if fmt == _native.KV_BF16 or v_cache.dtype is not k_cache.dtype:
+        raise ValueError("k_cache and v_cache must both be float8_e4m3fn or both int8")
+    slots = _check_quant_cache("k", k_cache, k_exp, H, D)
+    if _check_quant_cache("v", v_cache, v_exp, H, D) != slots:
+        raise ValueError("k_cache and v_cache hold different numbers of slots")
+    if slot_mapping.dtype is not torch.int32 or not slot_mapping.is_contiguous() or slot_mapping.numel() != N:
+        raise ValueError("slot_mapping must be contiguous int32 [tokens]")
+    if N == 0:
+        return
+    lib = _native.lib()
+    fn = lib.dllm_store_kvcache_quant if store else lib.dllm_load_kvcache_quant
+    with _on_device(dev):
+        rc = fn(key.data_ptr(), ks[0], value.data_ptr(), vs[0], k_cache.data_ptr(), v_cache.data_ptr(),
+                k_exp.data_ptr(), v_exp.data_ptr(), slot_mapping.data_ptr(), N, H, D, fmt, slots,
+                _status_ptr(dev), _stream_ptr())
+    if rc:
+        _native.check(rc, "store_kvcache_quant" if store else "load_kvcache_quant")
+    LAUNCHES[0] += 1
+
+
+# ---------------------------------------------------------------------------
 # Attention (attention.py:289-299, 235-265)
 # ---------------------------------------------------------------------------
 def _check_rows(name, t, heads, head_dim):
@@ -494,6 +567,168 @@ def _varlen_attention_rope(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, so
     if B > 0 and q.shape[0] > 0:
         LAUNCHES[0] += 1
     return out
+
+
+# ---------------------------------------------------------------------------
+# Attention of a chunk over a paged cache (attention.py:121-148)
+# ---------------------------------------------------------------------------
+_CHUNK_WS: dict = {}  # workspace bytes by launch sizes
+
+
+def chunk_attention(
+    q: torch.Tensor,
+    k_cache: torch.Tensor | None,
+    v_cache: torch.Tensor | None,
+    cu_seqlens_q: torch.Tensor,
+    max_seqlen_q: int,
+    softmax_scale: float | None = None,
+    *,
+    causal: bool = True,
+    block_tables: torch.Tensor | None = None,
+    context_lens: torch.Tensor | None = None,
+    slots: torch.Tensor | None = None,
+    cu_seqlens_slots: torch.Tensor | None = None,
+    max_context: int | None = None,
+    k: torch.Tensor | None = None,
+    v: torch.Tensor | None = None,
+    cu_seqlens_k: torch.Tensor | None = None,
+    max_seqlen_k: int | None = None,
+    k_exp: torch.Tensor | None = None,
+    v_exp: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of a chunk of new tokens over a paged KV cache.
+
+    q: bfloat16 [total_q, num_heads, 128], the sequences' chunks one after
+    another (``cu_seqlens_q`` int32 [B+1], none longer than ``max_seqlen_q``).
+    The keys of a sequence are its cached rows followed by its fresh rows:
+
+    * cached rows, from k_cache / v_cache [blocks, block_size, num_kv_heads,
+      128]: either ``block_tables`` (int32 [B, max_blocks]) with
+      ``context_lens`` (int32 [B]), or ``slots`` (int32) with
+      ``cu_seqlens_slots`` (int32 [B+1]), or neither (no cached rows).
+      ``max_context`` bounds the cached rows of a sequence (default: what the
+      table, or the slot list, can hold); the closer it is, the better the
+      work is spread. The cache is bfloat16, or float8_e4m3fn / int8 with the
+      exponent bytes ``k_exp`` / ``v_exp`` of ``store_kvcache_quant``.
+    * fresh rows, optional: ``k``, ``v`` (bfloat16 [total_k, num_kv_heads, 128])
+      with ``cu_seqlens_k`` (int32 [B+1], at most ``max_seqlen_k`` each; default
+      ``max_seqlen_q``).
+
+    ``causal``: the chunk's rows are the last positions of the keys, and row i
+    of Lq sees the first L - Lq + i + 1 of L keys; else every row sees all. A
+    row that sees no key is zero. Returns ``out`` (new by default)."""
+    if q.dim() != 3:
+        raise ValueError("q must be [tokens, num_heads, head_dim]")
+    Hq, D = q.shape[1], q.shape[2]
+    _check_rows("q", q, Hq, D)
+    if (k is None) != (v is None) or (k is None) != (cu_seqlens_k is None):
+        raise ValueError("k, v and cu_seqlens_k go together")
+    cached = block_tables is not None or slots is not None
+    if not cached and k is None:
+        raise ValueError("no keys: give block_tables, slots or fresh k and v")
+    if cached and (k_cache is None or v_cache is None):
+        raise ValueError("block_tables / slots need k_cache and v_cache")
+    dev = _require_cuda(q, cu_seqlens_q)
+    B = cu_seqlens_q.numel() - 1
+    _check_cu("cu_seqlens_q", cu_seqlens_q, B, dev)
+    fmt = _native.KV_BF16
+    Hkv = k.shape[1] if k is not None else k_cache.shape[-2]
+    k_ptr = v_ptr = cu_k_ptr = kx_ptr = vx_ptr = kc_ptr = vc_ptr = None
+    k_str = v_str = total_k = num_slots = max_fresh = 0
+    if k is not None:
+        _check_rows("k", k, Hkv, D)
+        _check_rows("v", v, Hkv, D)
+        if v.shape[0] != k.shape[0]:
+            raise ValueError("k and v have different row counts")
+        if k.device != dev or v.device != dev:
+            raise ValueError("all tensors must be on the same device")
+        _check_cu("cu_seqlens_k", cu_seqlens_k, B, dev)
+        k_ptr, k_str, v_ptr, v_str = k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0)
+        cu_k_ptr, total_k = cu_seqlens_k.data_ptr(), k.shape[0]
+        max_fresh = int(max_seqlen_q if max_seqlen_k is None else max_seqlen_k)
+    bt_ptr = ctx_ptr = sl_ptr = cus_ptr = None
+    table_stride = max_blocks = block_size = total_slots = 0
+    if cached:
+        fmt = _KV_FORMATS.get(k_cache.dtype)
+        if fmt is None or v_cache.dtype is not k_cache.dtype:
+            raise ValueError("k_cache and v_cache must both be bfloat16, float8_e4m3fn or int8")
+        if (k_cache.dim() != 4 or k_cache.shape[2] != Hkv or k_cache.shape[3] != D or v_cache.shape != k_cache.shape
+                or not k_cache.is_contiguous() or not v_cache.is_contiguous()):
+            raise ValueError(f"caches must be contiguous [blocks, block_size, {Hkv}, {D}]")
+        if k_cache.device != dev or v_cache.device != dev:
+            raise ValueError("all tensors must be on the same device")
+        block_size = k_cache.shape[1]
+        num_slots = k_cache.shape[0] * block_size
+        kc_ptr, vc_ptr = k_cache.data_ptr(), v_cache.data_ptr()
+        if fmt != _native.KV_BF16:
+            if k_exp is None or v_exp is None:
+                raise ValueError("a quantised cache needs k_exp and v_exp")
+            _check_quant_cache("k", k_cache, k_exp, Hkv, D)
+            _check_quant_cache("v", v_cache, v_exp, Hkv, D)
+            if k_exp.device != dev or v_exp.device != dev:
+                raise ValueError("all tensors must be on the same device")
+            kx_ptr, vx_ptr = k_exp.data_ptr(), v_exp.data_ptr()
+        if block_tables is not None:
+            if slots is not None:
+                raise ValueError("give block_tables or slots, not both")
+            if (block_tables.dtype is not torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] != B
+                    or block_tables.device != dev or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1)):
+                raise ValueError(f"block_tables must be int32 [{B}, max_blocks] with contiguous rows")
+            if (context_lens is None or context_lens.dtype is not torch.int32 or context_lens.numel() != B
+                    or not context_lens.is_contiguous() or context_lens.device != dev):
+                raise ValueError(f"context_lens must be contiguous int32 [{B}]")
+            max_blocks = block_tables.shape[1]
+            table_stride = block_tables.stride(0) if B > 1 else max(max_blocks, block_tables.stride(0))
+            bt_ptr, ctx_ptr = block_tables.data_ptr(), context_lens.data_ptr()
+            most = max_blocks * block_size
+        else:
+            if slots.dtype is not torch.int32 or slots.dim() != 1 or not slots.is_contiguous() or slots.device != dev:
+                raise ValueError("slots must be a contiguous 1-D int32 tensor")
+            if cu_seqlens_slots is None:
+                raise ValueError("slots need cu_seqlens_slots")
+            _check_cu("cu_seqlens_slots", cu_seqlens_slots, B, dev)
+            most = total_slots = slots.numel()
+            sl_ptr, cus_ptr = slots.data_ptr(), cu_seqlens_slots.data_ptr()
+        max_context = most if max_context is None else min(int(max_context), most)
+    else:
+        max_context = 0
+    if softmax_scale is None:
+        softmax_scale = D ** -0.5
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    else:
+        _check_rows("out", out, Hq, D)
+        if out.shape[0] != q.shape[0] or out.device != dev:
+            raise ValueError("out must have as many rows as q, on its device")
+    lib = _native.lib()
+    max_q = int(max_seqlen_q)
+    with _on_device(dev):
+        key = (fmt, B, Hq, Hkv, max_q, max_context, max_fresh, dev.index)
+        ws_bytes = _CHUNK_WS.get(key)
+        if ws_bytes is None:
+            ws_bytes = lib.dllm_attn_chunk_workspace(fmt, B, Hq, Hkv, max_q, max_context, max_fresh)
+            if len(_CHUNK_WS) > 4096:
+                _CHUNK_WS.clear()
+            _CHUNK_WS[key] = ws_bytes
+        # allocated per call on the current stream, so overlapping launches never share it
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
+        rc = lib.dllm_attn_chunk_fwd(
+            q.data_ptr(), q.stride(0), k_ptr, k_str, v_ptr, v_str, kc_ptr, vc_ptr, kx_ptr, vx_ptr, fmt, num_slots,
+            bt_ptr, table_stride, max_blocks, block_size, ctx_ptr, sl_ptr, cus_ptr, total_slots, max_context,
+            out.data_ptr(), out.stride(0), cu_seqlens_q.data_ptr(), cu_k_ptr, B, max_q, max_fresh, q.shape[0], total_k,
+            Hq, Hkv, D, softmax_scale, causal, None if ws is None else ws.data_ptr(), ws_bytes, _status_ptr(dev),
+            _stream_ptr())
+    if rc:
+        _native.check(rc, "chunk_attention")
+    if B > 0 and max_q > 0 and q.shape[0] > 0:
+        LAUNCHES[0] += 1 if ws is None else 2
+    return out
+
+
+def _check_cu(name, c, B, dev):
+    if c.dtype is not torch.int32 or c.numel() != B + 1 or not c.is_contiguous() or c.device != dev:
+        raise ValueError(f"{name} must be contiguous int32 [{B + 1}] on {dev}")
 
 
 # ---------------------------------------------------------------------------

@@ -31,6 +31,13 @@
  *                                (linear.py:186-190), one kernel over NVLink peer memory
  *   dllm_build_step_plan      <- the per-sequence metadata of attention.py:168-304 /
  *                                model_runner.py:240-321, on the device
+ *   dllm_store_kvcache_quant, dllm_load_kvcache_quant
+ *                             (no reference counterpart) the two copies above for a cache
+ *                                held in 8 bits per element
+ *   dllm_attn_chunk_fwd       <- the regular (non-diffusion) branches of Attention.forward
+ *                                (attention.py:121-148): causal prefill, prefill over block
+ *                                tables, decode; also over a quantised cache, and for the
+ *                                reuse step's [cached rows by slot ; fresh rows] over one
  *   dllm_select_kv_store      <- _select_important_head_kv (attention.py:344-413) or
  *                                _select_important_kv (attention.py:308-342), followed by
  *                                the k_prefix_suffix[idx] gather and store_kvcache of the
@@ -90,6 +97,12 @@ extern "C" {
 #define DLLM_DEV_WAIT_TIMEOUT 2
 #define DLLM_DEV_BAD_SEQUENCE 3
 #define DLLM_DEV_POSITION_OUT_OF_RANGE 4
+#define DLLM_DEV_NON_FINITE 5
+
+/* formats of a KV cache */
+#define DLLM_KV_BF16 0
+#define DLLM_KV_E4M3 1
+#define DLLM_KV_INT8 2
 
 /* Library version (major*10000 + minor*100 + patch). */
 DLLM_API int dllm_version(void);
@@ -119,6 +132,86 @@ DLLM_API int dllm_load_kvcache(void* key, int64_t key_stride, void* value, int64
                       const void* k_cache, const void* v_cache, const int32_t* slot_mapping,
                       int64_t n_tokens, int64_t row_elems, int elem_bytes, int64_t num_slots,
                       int32_t* err_flag, void* stream);
+
+/*
+ * dllm_store_kvcache / dllm_load_kvcache for a quantised cache (no reference
+ * counterpart; its cache is bf16).
+ *
+ * Format. The row x of one (slot, kv head), head_dim values, is one group. With a =
+ * the largest finite |x_i| and M = 448 (DLLM_KV_E4M3) or 127 (DLLM_KV_INT8), e is the
+ * smallest integer with a <= M * 2^e, clamped to [-100, 119] (e4m3) or [-100, 121]
+ * (int8); a = 0 gives e = -100. The codes are x_i * 2^-e rounded to nearest even
+ * (saturating), the group keeps the byte e + 127, and a code stands for code * 2^e.
+ * Both products are exact, so the code's rounding is the only one: at most half a step
+ * of the format, and every value a code stands for is a bf16 number. Byte 0, which the
+ * store never writes, stands for scale 0: a cache of zero bytes reads as zeros.
+ * Infinities are stored as +-M * 2^e, NaN as NaN (e4m3) or 0 (int8); either flags
+ * DLLM_DEV_NON_FINITE in err_flag.
+ *
+ * k_cache, v_cache: num_slots rows of num_kv_heads * head_dim bytes; k_exp, v_exp:
+ * num_slots rows of num_kv_heads bytes. key, value: bf16 [n_tokens, num_kv_heads,
+ * head_dim], heads packed, token strides in elements (multiples of 8), 16-byte
+ * aligned. head_dim: 64, 128 or 256. Slots as in dllm_store_kvcache: negative ones are
+ * skipped (store) or give zero rows (load), those >= num_slots also flag
+ * DLLM_DEV_SLOT_OUT_OF_RANGE. A slot that a store names twice ends with codes and
+ * exponent bytes of either row, not necessarily the same one: name each slot once.
+ */
+DLLM_API int dllm_store_kvcache_quant(const void* key, int64_t key_stride, const void* value,
+                                      int64_t value_stride, void* k_cache, void* v_cache, void* k_exp,
+                                      void* v_exp, const int32_t* slot_mapping, int64_t n_tokens,
+                                      int num_kv_heads, int head_dim, int format, int64_t num_slots,
+                                      int32_t* err_flag, void* stream);
+DLLM_API int dllm_load_kvcache_quant(void* key, int64_t key_stride, void* value, int64_t value_stride,
+                                     const void* k_cache, const void* v_cache, const void* k_exp,
+                                     const void* v_exp, const int32_t* slot_mapping, int64_t n_tokens,
+                                     int num_kv_heads, int head_dim, int format, int64_t num_slots,
+                                     int32_t* err_flag, void* stream);
+
+/*
+ * Attention of a chunk of new tokens over a paged KV cache (bf16 or quantised), bf16
+ * in/out, fp32 softmax and accumulation. Replaces, for the regular branches of
+ * Attention.forward (attention.py:121-148), flash_attn_varlen_func(causal=True,
+ * block_table=...) and flash_attn_with_kvcache(...).
+ *
+ * The keys of sequence b are [its C_b cached rows ; its F_b fresh rows]:
+ *   cached, by block table: row p is slot block_tables[b * table_stride + p / block_size]
+ *     * block_size + p % block_size, C_b = context_lens[b] <= max_context; table rows
+ *     have max_blocks entries, of which only the first ceil(C_b / block_size) are read;
+ *   cached, by slot list: row p is slots[cu_seqlens_slots[b] + p] (total_slots entries),
+ *     C_b <= max_context;
+ *   neither (both null): C_b = 0;
+ *   fresh: rows cu_seqlens_k[b] .. cu_seqlens_k[b+1] of k, v (bf16 [total_k, num_kv_heads,
+ *     128], at most max_fresh per sequence), or none (k, v, cu_seqlens_k null).
+ * With causal != 0 query row i of the chunk's Lq rows sees the first C_b + F_b - Lq + i + 1
+ * keys (the chunk's rows are the last Lq positions), else all of them. A row that sees no
+ * key is zero. Values at positions that a row does not see must be finite within the
+ * sequence's own keys; slots of no key of the sequence are not read.
+ *
+ * format: DLLM_KV_*; k_exp / v_exp as in dllm_store_kvcache_quant (null for bf16). Cache
+ * rows are num_kv_heads * 128 elements, num_slots of them. Slots or blocks out of range
+ * read as zero rows and flag DLLM_DEV_SLOT_OUT_OF_RANGE; lengths or offsets outside
+ * their buffers or bounds are cut there and flag DLLM_DEV_BAD_SEQUENCE.
+ * q, o: [total_q, num_heads, 128]; head_dim must be 128; max_seqlen_q bounds every Lq.
+ *
+ * workspace: device memory of at least dllm_attn_chunk_workspace(...) bytes, 16-byte
+ * aligned, whose contents need not be set; null if that is 0. Launches that may overlap
+ * need distinct ones. The result does not depend on the launch's timing (splits are
+ * merged in order).
+ */
+DLLM_API int64_t dllm_attn_chunk_workspace(int format, int batch, int num_heads, int num_kv_heads,
+                                           int max_seqlen_q, int max_context, int max_fresh);
+DLLM_API int dllm_attn_chunk_fwd(const void* q, int64_t q_tok_stride, const void* k, int64_t k_tok_stride,
+                                 const void* v, int64_t v_tok_stride, const void* k_cache,
+                                 const void* v_cache, const void* k_exp, const void* v_exp, int format,
+                                 int64_t num_slots, const int32_t* block_tables, int64_t table_stride,
+                                 int max_blocks, int block_size, const int32_t* context_lens,
+                                 const int32_t* slots, const int32_t* cu_seqlens_slots, int64_t total_slots,
+                                 int max_context, void* o, int64_t o_tok_stride,
+                                 const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int batch,
+                                 int max_seqlen_q, int max_fresh, int64_t total_q, int64_t total_k,
+                                 int num_heads, int num_kv_heads, int head_dim, float softmax_scale,
+                                 int causal, void* workspace, int64_t workspace_bytes, int32_t* err_flag,
+                                 void* stream);
 
 /*
  * Non-causal varlen attention, bf16 in/out, fp32 accumulation:

@@ -1,0 +1,463 @@
+"""Chunk attention over a paged KV cache against the 64-bit definition.
+
+The reference reads the same cache (the values its codes stand for), so the
+only errors are those of the operator's own roundings; the bound per output
+element is derived in ``oracle.kv_quant_ref.attention_bound``.
+"""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import inputs as I
+from oracle import kv_quant_ref as Q
+
+D = 128
+TYPES = {"bf16": torch.bfloat16, "e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+
+
+@pytest.fixture(scope="module")
+def dev():
+    d = torch.device("cuda:0")
+    torch.cuda.set_device(d)
+    from dllmserve_b200 import _native
+
+    _native.lib()
+    return d
+
+
+def _ops():
+    from dllmserve_b200 import ops
+
+    return ops
+
+
+def _cu(lens):
+    c = [0]
+    for n in lens:
+        c.append(c[-1] + n)
+    return torch.tensor(c, dtype=torch.int32)
+
+
+class Case:
+    """Inputs of one launch on the CPU, with caches whose unused rows are NaN."""
+
+    def __init__(self, seed, fmt, hq, hkv, nq, nc, nf, tables, page=16, spread=True):
+        g = I.gen(seed)
+        self.fmt, self.hq, self.hkv, self.page = fmt, hq, hkv, page
+        self.nq, self.nc, self.nf = nq, nc, nf
+        self.q = I.normal(g, (sum(nq) + 2, hq, D)).to(torch.bfloat16)  # two rows of no sequence
+        self.k = I.normal(g, (sum(nf), hkv, D)).to(torch.bfloat16) if nf else None
+        self.v = I.normal(g, (sum(nf), hkv, D)).to(torch.bfloat16) if nf else None
+        of = [-(-n // page) for n in nc]
+        pages = sum(of) + 2
+        order = torch.randperm(pages, generator=g)
+        self.tables = torch.full((len(nc), max(1, max(of) + 1)), -1, dtype=torch.int32)
+        lists, at = [], 0
+        for b, n in enumerate(of):
+            mine = order[at:at + n]
+            at += n
+            self.tables[b, :n] = mine.int()
+            every = (mine[:, None] * page + torch.arange(page)).flatten()[:nc[b]]
+            if not tables and b % 2:  # scattered rows
+                every = every[torch.randperm(nc[b], generator=g)]
+            lists.append(every)
+        self.use_tables = tables
+        self.slots = torch.cat(lists).int()
+        self.lists = lists
+        rows = [I.normal(g, (pages * page, hkv, D)) for _ in range(2)]
+        if spread:  # heads and tokens of different sizes
+            rows = [x * torch.exp2(torch.randint(-3, 3, (pages * page, hkv, 1), generator=g).float()) for x in rows]
+        used = torch.zeros(pages * page, dtype=torch.bool)
+        used[self.slots.long()] = True
+        self.values, self.caches, self.exps = [], [], []
+        for x in rows:
+            x = x.to(torch.bfloat16)
+            if fmt == "bf16":
+                x[~used] = float("nan")
+                self.values.append(x.double())
+                self.caches.append(x.view(pages, page, hkv, D))
+                self.exps.append(None)
+            else:
+                codes, e = Q.quantise(x, fmt)
+                self.values.append(Q.values(codes, e))
+                c = codes.float().to(TYPES[fmt])
+                byte = (e + 127).to(torch.uint8)
+                c.view(torch.uint8)[~used] = 0x7f
+                byte[~used] = 255
+                self.caches.append(c.view(pages, page, hkv, D))
+                self.exps.append(byte.view(pages, page, hkv))
+
+    def args(self, dev):
+        to = lambda t: None if t is None else t.to(dev)  # noqa: E731
+        kw = {"k_exp": to(self.exps[0]), "v_exp": to(self.exps[1])}
+        if self.use_tables:
+            kw |= {"block_tables": to(self.tables), "context_lens": torch.tensor(self.nc, dtype=torch.int32, device=dev)}
+        else:
+            kw |= {"slots": to(self.slots), "cu_seqlens_slots": _cu(self.nc).to(dev)}
+        if self.k is not None:
+            kw |= {"k": to(self.k), "v": to(self.v), "cu_seqlens_k": _cu(self.nf).to(dev), "max_seqlen_k": max(self.nf)}
+        return (to(self.q), to(self.caches[0]), to(self.caches[1]), _cu(self.nq).to(dev), max(self.nq)), kw
+
+    def check(self, out, causal, scale=D ** -0.5, seqs=None):
+        out = out.cpu().double()
+        start, fresh = 0, 0
+        for b, n in enumerate(self.nq):
+            keys, vals = (x[self.lists[b].long()] for x in self.values)
+            if self.k is not None:
+                keys = torch.cat([keys, self.k[fresh:fresh + self.nf[b]].double()])
+                vals = torch.cat([vals, self.v[fresh:fresh + self.nf[b]].double()])
+                fresh += self.nf[b]
+            got = out[start:start + n]
+            start += n
+            if seqs is not None and b not in seqs:
+                continue
+            o, mag, big = Q.chunk_attention(self.q[start - n:start], keys, vals, scale, causal)
+            off = (got - o).abs()
+            bound = Q.attention_bound(o, mag, big)
+            assert torch.isfinite(got).all(), f"sequence {b}"
+            worst = (off / bound).max().item() if off.numel() else 0.0
+            assert worst <= 1.0, f"sequence {b}: {worst:.2f} of the bound, off by {off.max():.3e}"
+
+
+SHAPES = [
+    # hq, hkv, query rows, cached rows, fresh rows (None: the cached rows hold the chunk's own)
+    (4, 4, [1], [1], None),
+    (4, 4, [1, 1, 1], [16, 17, 0], [1, 1, 1]),
+    (28, 4, [1, 1, 1, 1], [96, 5, 33, 130], None),
+    (7, 1, [1, 1], [300, 31], [1, 1]),
+    (8, 2, [3, 1, 5], [40, 64, 7], None),
+    (8, 8, [32, 32], [45, 152], [32, 32]),
+    (28, 4, [32, 7, 1], [50, 0, 111], [32, 7, 1]),
+    (2, 2, [70, 1, 33], [0, 200, 19], [70, 1, 33]),
+    (6, 2, [130, 12], [150, 300], None),
+    (3, 1, [9, 4], [5, 2], None),     # more query rows than keys: the first rows see none
+    (2, 1, [4, 0, 3], [10, 20, 0], [2, 5, 0]),  # fresh rows fewer or more than the chunk's, an empty chunk
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3", "int8"])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+@pytest.mark.parametrize("causal,tables", [(True, True), (False, False), (True, False)])
+def test_small(dev, fmt, shape, causal, tables):
+    hq, hkv, nq, nc, nf = SHAPES[shape]
+    c = Case(100 + shape, fmt, hq, hkv, nq, nc, nf, tables)
+    args, kw = c.args(dev)
+    out = torch.full(c.q.shape, 5.0, dtype=torch.bfloat16, device=dev)
+    got = _ops().chunk_attention(*args, causal=causal, out=out, **kw)
+    assert got is out
+    c.check(out, causal)
+    assert (out[sum(nq):] == 5).all()  # rows behind the last sequence are left as they were
+    assert _ops().read_device_status(dev) == 0
+
+
+LONG = [
+    # hq, hkv, query rows, cached rows, fresh rows, sequences checked against 64 bits
+    (28, 4, [1, 1, 1], [9000, 130, 4097], None, [0, 1, 2]),
+    (4, 4, [1, 1], [20000, 3], [1, 1], [0, 1]),
+    (8, 8, [32, 32], [2500, 1200], [32, 32], [1]),
+    (28, 4, [33, 20], [700, 1500], [33, 20], [0]),
+    (4, 2, [200], [600], [200], [0]),
+    (4, 2, [260, 3], [700, 400], None, [0, 1]),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3", "int8"])
+@pytest.mark.parametrize("shape", range(len(LONG)))
+@pytest.mark.parametrize("causal,tables", [(True, True), (False, False)])
+def test_long(dev, fmt, shape, causal, tables):
+    hq, hkv, nq, nc, nf, seqs = LONG[shape]
+    c = Case(300 + shape, "bf16" if fmt == "bf16" else fmt, hq, hkv, nq, nc, nf, tables, page=256, spread=shape % 2 == 0)
+    args, kw = c.args(dev)
+    out = _ops().chunk_attention(*args, causal=causal, max_context=max(nc), **kw)
+    c.check(out, causal, seqs=seqs)
+    again = _ops().chunk_attention(*args, causal=causal, max_context=max(nc), **kw)
+    assert torch.equal(again[:sum(nq)], out[:sum(nq)])  # the same bits every time
+    # a loose bound of the context changes the split of the work, not the result's accuracy
+    c.check(_ops().chunk_attention(*args, causal=causal, **kw), causal, seqs=seqs[:1])
+    assert _ops().read_device_status(dev) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+def test_fresh_only(dev, fmt):
+    """No cache at all: causal attention among the chunk's own rows."""
+    c = Case(7, "bf16", 6, 2, [33, 1, 140], [0, 0, 0], [33, 1, 140], True)
+    args, kw = c.args(dev)
+    for name in ("block_tables", "context_lens", "k_exp", "v_exp"):
+        kw.pop(name)
+    for causal in (True, False):
+        c.check(_ops().chunk_attention(args[0], None, None, *args[3:], causal=causal, **kw), causal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [1, 7, 48, 512])
+def test_page_sizes(dev, page):
+    c = Case(11 + page, "int8", 4, 2, [2, 1], [101, 64], [2, 1], True, page=page)
+    args, kw = c.args(dev)
+    c.check(_ops().chunk_attention(*args, **kw), True)
+    assert _ops().read_device_status(dev) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3", "int8"])
+def test_strides_and_scale(dev, fmt):
+    """Rows of a fused projection, table rows wider than the table, a slice of
+    the output buffer, and a scale of the caller's."""
+    c = Case(21, fmt, 8, 2, [17, 1, 40], [60, 3, 29], [17, 1, 40], True)
+    args, kw = c.args(dev)
+    n, pad = c.q.shape[0], 8
+    qkv = torch.full((n, 12 * D + pad), 3.0, dtype=torch.bfloat16, device=dev)
+    q = qkv[:, :8 * D].view(n, 8, D)
+    q.copy_(args[0])
+    m = c.k.shape[0]
+    k, v = qkv[:m, 8 * D:10 * D].view(m, 2, D), qkv[:m, 10 * D:12 * D].view(m, 2, D)
+    k.copy_(kw["k"])
+    v.copy_(kw["v"])
+    wide = torch.full((3, c.tables.shape[1] + 5), 1 << 30, dtype=torch.int32, device=dev)
+    wide[:, :c.tables.shape[1]] = kw["block_tables"]
+    buf = torch.full((n, 10 * D), 4.0, dtype=torch.bfloat16, device=dev)
+    out = buf[:, D:9 * D].view(n, 8, D)
+    kw |= {"k": k, "v": v, "block_tables": wide[:, :c.tables.shape[1]], "out": out}
+    _ops().chunk_attention(q, *args[1:], 0.25, causal=True, **kw)
+    c.check(out, True, scale=0.25)
+    assert (buf[:, :D] == 4).all() and (buf[:, 9 * D:] == 4).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3", "int8"])
+def test_large_scores(dev, fmt):
+    """Scores far apart (differences of hundreds): the running maximum moves by
+    a lot and most probabilities vanish."""
+    c = Case(31, fmt, 4, 2, [3, 40], [333, 70], [3, 40], False)
+    c.q = (c.q.float() * 30).to(torch.bfloat16)
+    args, kw = c.args(dev)
+    for causal in (True, False):
+        c.check(_ops().chunk_attention(*args, causal=causal, **kw), causal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+def test_bad_pages_and_lengths(dev, fmt):
+    """Pages outside the cache read as zero rows and are flagged; lengths past
+    their bounds are cut and flagged. Nothing outside the buffers is touched."""
+    ops = _ops()
+    c = Case(41, fmt, 4, 4, [1, 2], [40, 33], None, True)
+    args, kw = c.args(dev)
+    for bad in (10 ** 6, -3, 2 ** 31 - 1):
+        tables = kw["block_tables"].clone()
+        page = int(tables[0, 1])
+        tables[0, 1] = bad
+        out = ops.chunk_attention(*args, **{**kw, "block_tables": tables})
+        assert ops.read_device_status(dev) == 1
+        saved = [x.clone() for x in c.values]
+        for x in c.values:
+            x[page * 16:page * 16 + 16] = 0
+        c.check(out, True)
+        c.values = saved
+    # a context longer than its table row
+    ctx = torch.tensor([40, 10 ** 6], dtype=torch.int32, device=dev)
+    out = ops.chunk_attention(*args, **{**kw, "context_lens": ctx})
+    assert ops.read_device_status(dev) in (1, 3)
+    c.check(out, True, seqs=[0])
+    ctx = torch.tensor([40, -5], dtype=torch.int32, device=dev)
+    out = ops.chunk_attention(*args, **{**kw, "context_lens": ctx})
+    assert ops.read_device_status(dev) == 3
+    assert (out[1:3] == 0).all()
+    # a chunk longer than max_seqlen_q: the rows past it are not computed
+    out = torch.full_like(args[0], 5.0)
+    ops.chunk_attention(*args[:4], 1, out=out, **kw)
+    assert ops.read_device_status(dev) == 3
+    assert (out[2:] == 5).all()
+    # slots outside the cache
+    c = Case(42, fmt, 4, 4, [1, 2], [40, 33], None, False)
+    args, kw = c.args(dev)
+    slots = kw["slots"].clone()
+    slots[3], slots[50] = 10 ** 8, -1
+    out = ops.chunk_attention(*args, **{**kw, "slots": slots})
+    assert ops.read_device_status(dev) == 1
+    for x in c.values:
+        x[c.slots[3].long()] = 0
+        x[c.slots[50].long()] = 0
+    c.check(out, True)
+
+
+@pytest.mark.gpu
+def test_streams_and_graph(dev):
+    """Two streams at once, and a captured launch replayed on new contents."""
+    ops = _ops()
+    cases = [Case(51, "e4m3", 28, 4, [1, 1], [5000, 800], [1, 1], True, page=256),
+             Case(52, "int8", 8, 8, [1, 1], [4000, 1900], None, True, page=256)]
+    made = [c.args(dev) for c in cases]
+    streams = [torch.cuda.Stream(dev) for _ in cases]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[i].append(ops.chunk_attention(*made[i][0], **made[i][1]))
+    torch.cuda.synchronize()
+    for i, c in enumerate(cases):
+        c.check(outs[i][0], True)
+        for o in outs[i][1:]:
+            assert torch.equal(o[:2], outs[i][0][:2])
+    args, kw = made[0]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.chunk_attention(*args, **kw)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out[:2], outs[0][0][:2])
+    cases[0].q = -cases[0].q
+    args[0].copy_(cases[0].q)
+    cases[0].nc = [4000, 0]
+    cases[0].lists = [x[:n] for x, n in zip(cases[0].lists, cases[0].nc)]
+    kw["context_lens"].copy_(torch.tensor(cases[0].nc, dtype=torch.int32))
+    graph.replay()
+    torch.cuda.synchronize()
+    cases[0].check(out, True)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(dev):
+    """A cache of more than 2^31 elements, used at its far end."""
+    hkv, page = 32, 256
+    pages = 2200
+    cache = torch.zeros(pages, page, hkv, D, dtype=torch.float8_e4m3fn, device=dev)
+    vcache = torch.zeros_like(cache)
+    ke = torch.full((pages, page, hkv), 127, dtype=torch.uint8, device=dev)
+    c = Case(61, "e4m3", 32, 32, [1, 1], [300, 80], None, True, page=page)
+    n = c.caches[0].shape[0]
+    cache[-n:].view(torch.uint8).copy_(c.caches[0].to(dev).view(torch.uint8))
+    vcache[-n:].view(torch.uint8).copy_(c.caches[1].to(dev).view(torch.uint8))
+    ve = ke.clone()
+    ke[-n:], ve[-n:] = c.exps[0].to(dev), c.exps[1].to(dev)
+    args, kw = c.args(dev)
+    tables = torch.where(kw["block_tables"] >= 0, kw["block_tables"] + (pages - n), kw["block_tables"])
+    out = _ops().chunk_attention(args[0], cache, vcache, *args[3:], block_tables=tables.int(),
+                                 context_lens=kw["context_lens"], k_exp=ke, v_exp=ve)
+    c.check(out, True)
+    assert _ops().read_device_status(dev) == 0
+
+
+@pytest.mark.gpu
+def test_store_then_attend(dev):
+    """The operators as they are used together: prefill in two chunks, then
+    decode steps, over a quantised cache, each step storing its rows first."""
+    ops = _ops()
+    for fmt in ("e4m3", "int8"):
+        g = I.gen(71)
+        hq, hkv, page = 14, 2, 16
+        lens = [37, 90]
+        pages = 12
+        kc = torch.zeros(pages, page, hkv, D, dtype=torch.uint8, device=dev).view(TYPES[fmt])
+        vc = torch.zeros_like(kc)
+        ke = torch.zeros(pages, page, hkv, dtype=torch.uint8, device=dev)
+        ve = torch.zeros_like(ke)
+        tables = torch.randperm(pages, generator=g)[:12].view(2, 6).int()
+        total = [0, 0]
+        seen = [[torch.zeros(0, hkv, D, dtype=torch.float64)] * 2 for _ in lens]
+        for step in ([20, 64], [17, 26], [1, 1], [1, 1]):
+            n = sum(step)
+            q, k, v = (I.normal(g, (n, h, D)).to(torch.bfloat16) for h in (hq, hkv, hkv))
+            pos = [torch.arange(total[b], total[b] + step[b]) for b in range(2)]
+            slots = torch.cat([tables[b][p // page].long() * page + p % page for b, p in enumerate(pos)]).int()
+            ops.store_kvcache_quant(k.to(dev), v.to(dev), kc, vc, ke, ve, slots.to(dev))
+            total = [t + s for t, s in zip(total, step)]
+            out = ops.chunk_attention(q.to(dev), kc, vc, _cu(step).to(dev), max(step), block_tables=tables.to(dev),
+                                      context_lens=torch.tensor(total, dtype=torch.int32, device=dev), k_exp=ke, v_exp=ve)
+            at = 0
+            for b, s in enumerate(step):
+                rows = slice(at, at + s)
+                at += s
+                seen[b] = [torch.cat([old, Q.values(*Q.quantise(x[rows], fmt))]) for old, x in zip(seen[b], (k, v))]
+                o, mag, big = Q.chunk_attention(q[rows], *seen[b], D ** -0.5, True)
+                assert ((out[rows].cpu().double() - o).abs() <= Q.attention_bound(o, mag, big)).all()
+        assert ops.read_device_status(dev) == 0
+
+
+def test_refusals():
+    """Bad arguments are refused before any device work."""
+    from dllmserve_b200 import _native, ops
+
+    lib = _native.lib()
+
+    def call(**kw):
+        a = dict(q=64, qs=512, k=None, ks=0, v=None, vs=0, kc=64, vc=64, ke=64, ve=64, fmt=1, slots_n=64, bt=64, bts=4,
+                 mb=4, bs=16, ctx=64, sl=None, cus=None, ts=0, mc=64, o=64, os=512, cuq=64, cuk=None, B=1, mq=1, mf=0,
+                 tq=1, tk=0, hq=4, hkv=4, hd=128, sc=ctypes.c_float(0.1), ca=1, ws=None, wb=0)
+        a.update(kw)
+        return lib.dllm_attn_chunk_fwd(*a.values(), None, None)
+
+    E = _native
+    assert call(hd=64) == E.DLLM_ERR_UNSUPPORTED
+    assert call(fmt=3) == E.DLLM_ERR_UNSUPPORTED
+    assert call(hq=6) == E.DLLM_ERR_UNSUPPORTED
+    assert call(B=-1) == E.DLLM_ERR_INVALID_ARG
+    assert call(sc=ctypes.c_float(0.0)) == E.DLLM_ERR_INVALID_ARG
+    assert call(sc=ctypes.c_float(math.nan)) == E.DLLM_ERR_INVALID_ARG
+    assert call(sl=64, cus=64) == E.DLLM_ERR_INVALID_ARG       # tables and a slot list
+    assert call(ctx=None) == E.DLLM_ERR_INVALID_ARG
+    assert call(bs=0) == E.DLLM_ERR_INVALID_ARG
+    assert call(bts=3) == E.DLLM_ERR_INVALID_ARG
+    assert call(bt=None, sl=64) == E.DLLM_ERR_INVALID_ARG      # slots without offsets
+    assert call(kc=None) == E.DLLM_ERR_INVALID_ARG
+    assert call(ke=None) == E.DLLM_ERR_INVALID_ARG
+    assert call(kc=72) == E.DLLM_ERR_ALIGNMENT
+    assert call(k=64) == E.DLLM_ERR_INVALID_ARG                # k without v
+    assert call(cuq=None) == E.DLLM_ERR_INVALID_ARG
+    assert call(q=72) == E.DLLM_ERR_ALIGNMENT
+    assert call(qs=516) == E.DLLM_ERR_ALIGNMENT
+    assert call(os=500) == E.DLLM_ERR_INVALID_ARG
+    assert call(slots_n=2 ** 31) == E.DLLM_ERR_TOO_LARGE
+    assert call(mc=2 ** 30 + 1) == E.DLLM_ERR_TOO_LARGE
+    assert call(B=0) == E.DLLM_OK
+    assert call(mc=100000, mb=10000, bts=10000) == E.DLLM_ERR_INVALID_ARG  # no workspace for the splits
+    assert "workspace" in lib.dllm_last_error().decode()
+    ws = lib.dllm_attn_chunk_workspace
+    assert ws(1, 1, 4, 4, 1, 100000, 0) > 0
+    assert ws(1, 64, 32, 32, 1, 64, 0) == 0
+    assert ws(9, 1, 4, 4, 1, 64, 0) == -1
+    q = torch.zeros(1, 4, 128, dtype=torch.bfloat16)
+    cu = torch.tensor([0, 1], dtype=torch.int32)
+    with pytest.raises(ValueError, match="no keys"):
+        ops.chunk_attention(q, None, None, cu, 1)
+    with pytest.raises(ValueError, match="go together"):
+        ops.chunk_attention(q, None, None, cu, 1, k=q)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.chunk_attention(q, None, None, cu, 1, k=q, v=q, cu_seqlens_k=cu)
+
+
+@pytest.mark.gpu
+def test_refusals_on_device_tensors(dev):
+    ops = _ops()
+    c = Case(81, "int8", 4, 2, [1, 2], [20, 9], [1, 2], True)
+    args, kw = c.args(dev)
+    q, kc, vc, cu, mq = args
+
+    def refused(*a, **k):
+        with pytest.raises(ValueError):
+            ops.chunk_attention(*(a or args), **{**kw, **k})
+
+    refused(q.float(), kc, vc, cu, mq)
+    refused(q, kc, vc.view(torch.uint8), cu, mq)
+    refused(q, kc[:, :, :1], vc, cu, mq)
+    refused(q, kc, vc[:1], cu, mq)
+    refused(q, kc, vc, cu.long(), mq)
+    refused(k_exp=None)
+    refused(v_exp=kw["v_exp"].int())
+    refused(block_tables=kw["block_tables"].long())
+    refused(block_tables=kw["block_tables"][:1])
+    refused(block_tables=kw["block_tables"].t().contiguous().t())
+    refused(context_lens=None)
+    refused(slots=c.slots.to(dev))
+    refused(k=kw["k"][:, :1])
+    refused(cu_seqlens_k=kw["cu_seqlens_k"][:2])
+    refused(out=torch.empty_like(q[:1]))
+    refused(softmax_scale=0.0)
+    y = torch.zeros(3, 4, 64, dtype=torch.bfloat16, device=dev)
+    with pytest.raises(NotImplementedError):
+        ops.chunk_attention(y, None, None, cu, 2, k=y, v=y, cu_seqlens_k=cu)
