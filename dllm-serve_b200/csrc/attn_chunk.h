@@ -55,7 +55,7 @@ struct ChunkArgs {
 
 // How a launch is laid out, from sizes the host knows.
 struct ChunkPlan {
-  int mt;                  // 16-row tiles of a warp (1 or 2)
+  int rows;                // packed rows of a tile: 8, 16 or 32
   int mtiles;
   int splits;
   int split_chunks;

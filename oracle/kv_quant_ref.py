@@ -77,7 +77,23 @@ def chunk_attention(q, keys, vals, scale, causal):
     return o, mag, big
 
 
-def attention_bound(o, mag, big):
+def small_probability_floor(vals, heads):
+    """What a quantised cache's f16 probabilities add to the bound, [heads].
+
+    Over a quantised cache p_j 2^(e_j - E + 15) is rounded to f16, E the largest
+    exponent of the values met. Above 2^-14 that is 2^-11 of its value (the
+    bound's 2^-8 covers it); below, at most half of f16's smallest step, 2^-25,
+    which the product with the code c_j and the unit 2^(E - 15) turns into
+    2^-25 |c_j| 2^(E - 15) <= 2^-40 M 2^E. E is the smallest with
+    max |v| <= M 2^E, so M 2^E < 2 max |v|: at most 2^-39 max |v| for each of
+    the sequence's keys (those a row does not see included: E may be theirs).
+    It matters only where the output is that small against the head's largest
+    value, as when every key of weight has a zero in that dimension."""
+    top = vals.double().abs().amax((0, 2)) * vals.shape[0] * 2.0 ** -39 if vals.shape[0] else torch.zeros(vals.shape[1])
+    return top.double().repeat_interleave(heads // vals.shape[1])
+
+
+def attention_bound(o, mag, big, floor=None):
     """Largest error the operator's roundings explain, per output element.
 
     Probabilities are rounded to bf16 before the second product (2^-8 of each
@@ -86,6 +102,7 @@ def attention_bound(o, mag, big):
     sum |q k| scale each (twice the usual bound, for accumulation in any order
     with truncation), which changes each probability by that fraction, in the
     numerator and in the normaliser; exponentials, sums and the final division
-    add less than 2^-16 relative."""
+    add less than 2^-16 relative. ``floor`` [heads]: an absolute part."""
     e32 = 2 * 256 * 2.0 ** -24 * big.unsqueeze(-1) + 2.0 ** -16
-    return (2.0 ** -8 + e32) * mag * 1.01 + 2.0 ** -8 * o.abs() * 1.01 + 1e-30
+    bound = (2.0 ** -8 + e32) * mag * 1.01 + 2.0 ** -8 * o.abs() * 1.01 + 1e-30
+    return bound if floor is None else bound + floor.view(1, -1, 1)

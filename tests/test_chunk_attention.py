@@ -115,7 +115,8 @@ class Case:
                 continue
             o, mag, big = Q.chunk_attention(self.q[start - n:start], keys, vals, scale, causal)
             off = (got - o).abs()
-            bound = Q.attention_bound(o, mag, big)
+            floor = None if self.fmt == "bf16" else Q.small_probability_floor(vals, self.hq)
+            bound = Q.attention_bound(o, mag, big, floor)
             assert torch.isfinite(got).all(), f"sequence {b}"
             worst = (off / bound).max().item() if off.numel() else 0.0
             assert worst <= 1.0, f"sequence {b}: {worst:.2f} of the bound, off by {off.max():.3e}"
@@ -237,6 +238,28 @@ def test_large_scores(dev, fmt):
     args, kw = c.args(dev)
     for causal in (True, False):
         c.check(_ops().chunk_attention(*args, causal=causal, **kw), causal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("step", [1, 6, 30])
+def test_value_sizes_far_apart(dev, fmt, step):
+    """Value rows whose exponents rise, fall and jump along the sequence by up
+    to 2^90, with weight on the small ones: the unit of the outputs moves, and
+    chunks whose values lie far below it take the wider operands."""
+    for seed, order in ((91, 1), (92, -1), (93, 0)):
+        c = Case(seed, fmt, 4, 2, [2, 1, 33], [300, 410, 200], [2, 1, 33], True)
+        for b, at in enumerate(c.lists):
+            n = len(at)
+            e = (torch.arange(n) * 3 // n) * step * (order or 1)
+            if order == 0:  # jumps from key to key
+                e = torch.randint(0, 3, (n,), generator=I.gen(seed + b)) * step
+            byte = c.exps[1].view(-1, 2)[at].int() + e.int()[:, None]
+            assert byte.min() >= 27 and byte.max() <= 240
+            c.exps[1].view(-1, 2)[at] = byte.to(torch.uint8)
+            c.values[1][at] *= torch.exp2(e.double())[:, None, None]
+        args, kw = c.args(dev)
+        c.check(_ops().chunk_attention(*args, causal=True, **kw), True)
 
 
 @pytest.mark.gpu
@@ -375,7 +398,8 @@ def test_store_then_attend(dev):
                 at += s
                 seen[b] = [torch.cat([old, Q.values(*Q.quantise(x[rows], fmt))]) for old, x in zip(seen[b], (k, v))]
                 o, mag, big = Q.chunk_attention(q[rows], *seen[b], D ** -0.5, True)
-                assert ((out[rows].cpu().double() - o).abs() <= Q.attention_bound(o, mag, big)).all()
+                bound = Q.attention_bound(o, mag, big, Q.small_probability_floor(seen[b][1], hq))
+                assert ((out[rows].cpu().double() - o).abs() <= bound).all()
         assert ops.read_device_status(dev) == 0
 
 
