@@ -19,7 +19,7 @@ REPO = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 OUT = os.path.join(HERE, "dllmserve_b200", "libdllm_attn.so")
-SOURCES = ["attn_fwd.cu", "attn_fwd_split.cu", "attn_chunk.cu", "kvcache.cu", "kvquant.cu", "select_kv.cu",
+SOURCES = ["attn_fwd.cu", "attn_fwd_split.cu", "attn_chunk.cu", "attn_chunk_mma.cu", "kvcache.cu", "kvquant.cu", "select_kv.cu",
            "rope.cu", "step_plan.cu", "oproj_ar.cu", "capi.cu"]
 
 NVCC_FLAGS = [

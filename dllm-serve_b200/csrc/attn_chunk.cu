@@ -16,11 +16,10 @@
 //      the row's largest lose bits.
 //   P: p * 2^(e_v - E + 15), E the largest value exponent this warp has met
 //      (O is in units of 2^(E - 15) and is rescaled when E grows). p <= 1, so
-//      nothing overflows, and with e_v >= E - 14 every p >= 2^-15 keeps 11
-//      bits, smaller ones an absolute error below 2^-25: closer than bf16
-//      probabilities in both cases. A chunk with a value further below E
-//      takes bf16 operands instead (rare: value rows of one head whose sizes
-//      differ by more than 2^14).
+//      nothing overflows; down to 2^-14 these keep 11 bits, and below that the
+//      rounding is at most 2^-25, i.e. 2^-39 of the largest |v| met once
+//      multiplied by the code and the unit. bf16 probabilities (2^-8 of p)
+//      would be further off for every value above 2^-31 of the largest.
 //
 // A CTA takes one tile of packed rows (row r of the chunk for query head g of
 // the KV head's group is packed row r * group + g) and one split of the keys;
@@ -43,11 +42,10 @@
 
 #include <algorithm>
 #include <atomic>
-#include <type_traits>
 
 #include "common.cuh"
 #include "kvquant.cuh"
-#include "attn_chunk.h"
+#include "attn_chunk.cuh"
 
 namespace dllm {
 namespace chunk {
@@ -66,7 +64,7 @@ constexpr int chunk_keys() { return kFmt == kFmtBf16 ? 16 : 32; }
 
 constexpr uint32_t kOffStages = 0;
 constexpr uint32_t kOffScales = kOffStages + kWarps * kStages * kStageBytes;
-constexpr uint32_t kScaleBytes = 34 * 8;                               // 32 (K, V) scales, the exponent range
+constexpr uint32_t kScaleBytes = 34 * 8;                               // 32 (K, V) scales, the largest exponent
 constexpr uint32_t kOffRowFactor = kOffScales + kWarps * kStages * kScaleBytes;  // float per packed row
 constexpr uint32_t kOffQ = kOffRowFactor + 32 * 4;
 constexpr int kNoExp = -(1 << 30);      // no value exponent met
@@ -108,7 +106,7 @@ DLLM_DEVICE void mma16816_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t 
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Four codes -> two words of f16 (or bf16) pairs, unscaled (exact).
+// Four codes -> two words of f16 pairs, unscaled (exact).
 template <int kFmt>
 DLLM_DEVICE void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
   if constexpr (kFmt == kFmtE4m3) {
@@ -126,14 +124,6 @@ DLLM_DEVICE void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
     hi = *reinterpret_cast<uint32_t*>(&q);
   }
 }
-template <int kFmt>
-DLLM_DEVICE void codes_to_bf16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  float y[4];
-  decode4<kFmt>(w, 1.f, y);
-  lo = pack_bf16x2(y[0], y[1]);
-  hi = pack_bf16x2(y[2], y[3]);
-}
-
 DLLM_DEVICE uint32_t pack_f16x2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -159,62 +149,6 @@ DLLM_DEVICE uint32_t v_unit(uint32_t unit, uint32_t key) {
 }
 
 }  // namespace
-
-// Sizes of one sequence, every value checked against the buffers it indexes.
-struct Seq {
-  int64_t q_begin, s_begin, k_begin;
-  int Lq, nc, nk;
-};
-
-DLLM_DEVICE Seq load_seq(const ChunkArgs& a, int b, bool report) {
-  Seq s;
-  bool bad = false;
-  auto range = [&](const int32_t* cu, int64_t total, int64_t& begin, int& n, int most) {
-    const int64_t lo = cu[b], hi = cu[b + 1];
-    begin = min(max(lo, (int64_t)0), total);
-    const int64_t end = min(max(hi, begin), total);
-    n = (int)min(end - begin, (int64_t)most);
-    bad |= lo != begin || hi != begin + n;
-  };
-  range(a.cu_q, a.total_q, s.q_begin, s.Lq, a.max_q);
-  s.k_begin = 0;
-  s.nk = 0;
-  if (a.cu_k != nullptr) range(a.cu_k, a.total_k, s.k_begin, s.nk, a.max_fresh);
-  s.s_begin = 0;
-  if (a.tables != nullptr) {
-    const int c = a.ctx[b];
-    s.nc = min(max(c, 0), a.max_context);
-    bad |= c != s.nc;
-  } else if (a.slots != nullptr) {
-    range(a.cu_s, a.total_slots, s.s_begin, s.nc, a.max_context);
-  } else {
-    s.nc = 0;
-  }
-  if (bad && report) set_error(a.err, kDevBadSequence);
-  return s;
-}
-
-// Key chunks of a row tile: the cached rows in chunks of KB keys, then the
-// fresh rows in chunks of kFreshKeys, both cut at the last key any row of the
-// tile sees.
-struct Span {
-  int nc, nk;      // keys to walk in each segment
-  int cached;      // chunks of the cached segment
-  int total;       // all chunks
-};
-
-template <int kFmt>
-DLLM_DEVICE Span tile_span(const ChunkArgs& a, const Seq& s, int last_row) {
-  constexpr int KB = chunk_keys<kFmt>();
-  int64_t seen = (int64_t)s.nc + s.nk;
-  if (a.causal) seen = min(seen, max((int64_t)0, seen - s.Lq + last_row + 1));
-  Span r;
-  r.nc = (int)min(seen, (int64_t)s.nc);
-  r.nk = (int)(seen - r.nc);
-  r.cached = (r.nc + KB - 1) / KB;
-  r.total = r.cached + (r.nk + kFreshKeys - 1) / kFreshKeys;
-  return r;
-}
 
 // Running state of a warp's rows: thread (g, t) holds rows 8 r + g of its
 // 16-row tiles, r < kR (kR = 1: the tile has at most eight rows, so the upper
@@ -316,17 +250,15 @@ DLLM_DEVICE void chunk_step(uint32_t ks, uint32_t vs, uint32_t scales, uint32_t 
   }
   // the value exponents of the chunk against the unit of O
   float ufac = 1.f, grow = 1.f;  // P times this; O times this
-  bool narrow = true;            // f16 operands for the second product
   if constexpr (kQuant && kCodes) {
-    int2 ev;  // largest and smallest value exponent of the chunk (kNoExp, INT_MAX: no live value)
-    asm volatile("ld.shared.v2.s32 {%0, %1}, [%2];" : "=r"(ev.x), "=r"(ev.y) : "r"(scales + 32 * 8));
-    if (ev.x != kNoExp) {
-      if (ev.x > w.e) {
-        grow = w.e == kNoExp ? 1.f : pow2(w.e - ev.x);
-        w.e = ev.x;
+    int ev;  // largest value exponent of the chunk (kNoExp: no live value)
+    asm volatile("ld.shared.s32 %0, [%1];" : "=r"(ev) : "r"(scales + 32 * 8));
+    if (ev != kNoExp) {
+      if (ev > w.e) {
+        grow = w.e == kNoExp ? 1.f : pow2(w.e - ev);
+        w.e = ev;
       }
-      ufac = pow2(ev.x - w.e);
-      narrow = ev.y >= w.e - 14;
+      ufac = pow2(ev - w.e);
     }
   } else if constexpr (kQuant) {
     if (w.e == kNoExp) w.e = 0;
@@ -392,16 +324,8 @@ DLLM_DEVICE void chunk_step(uint32_t ks, uint32_t vs, uint32_t scales, uint32_t 
         for (int j = 0; j < 16; ++j) w.o[mt][j][2 * r] *= f, w.o[mt][j][2 * r + 1] *= f;
       }
   }
-  // outputs: probabilities are rounded to f16 (2^-11 of their value, see above) or bf16 (2^-8)
-  auto outputs = [&](auto half) {
-    constexpr bool kHalf = decltype(half)::value;
-    auto pack = [](float lo, float hi) { return kHalf ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi); };
-    auto expand = [](uint32_t c, uint32_t& lo, uint32_t& hi) {
-      if constexpr (kHalf)
-        codes_to_f16<kCodes ? kFmt : kFmtE4m3>(c, lo, hi);
-      else
-        codes_to_bf16<kCodes ? kFmt : kFmtE4m3>(c, lo, hi);
-    };
+  // outputs: probabilities are rounded to f16 (see above) or bf16 (2^-8 of their value)
+  auto pack = [](float lo, float hi) { return kCodes ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi); };
 #pragma unroll
     for (int u = 0; u < NT / 2; ++u) {
       uint32_t pa[kMT][4];
@@ -417,7 +341,7 @@ DLLM_DEVICE void chunk_step(uint32_t ks, uint32_t vs, uint32_t scales, uint32_t 
       auto product = [&](int j, uint32_t b0, uint32_t b1) {
 #pragma unroll
         for (int mt = 0; mt < kMT; ++mt) {
-          if constexpr (kHalf)
+          if constexpr (kCodes)
             mma16816_f16(w.o[mt][j], pa[mt][0], pa[mt][1], pa[mt][2], pa[mt][3], b0, b1);
           else
             mma16816(w.o[mt][j], pa[mt][0], pa[mt][1], pa[mt][2], pa[mt][3], b0, b1);
@@ -455,23 +379,14 @@ DLLM_DEVICE void chunk_step(uint32_t ks, uint32_t vs, uint32_t scales, uint32_t 
           uint32_t vb[4][2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            expand(__byte_perm(x[2 * e][i], x[2 * e + 1][i], 0x5140), vb[0][e], vb[1][e]);
-            expand(__byte_perm(x[2 * e][i], x[2 * e + 1][i], 0x7362), vb[2][e], vb[3][e]);
+            codes_to_f16<kFmt>(__byte_perm(x[2 * e][i], x[2 * e + 1][i], 0x5140), vb[0][e], vb[1][e]);
+            codes_to_f16<kFmt>(__byte_perm(x[2 * e][i], x[2 * e + 1][i], 0x7362), vb[2][e], vb[3][e]);
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) product(4 * i + j, vb[j][0], vb[j][1]);
         }
       }
     }
-  };
-  if constexpr (kCodes) {
-    if (narrow)
-      outputs(std::true_type{});
-    else
-      outputs(std::false_type{});
-  } else {
-    outputs(std::false_type{});
-  }
 }
 
 template <int kFmt, int kMT, int kR>
@@ -495,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_chunk_kernel(const __grid_co
   const int row0 = mtile * kRows;           // first packed row
   const int rows = sq.Lq * a.group - row0;  // packed rows left
   if (rows <= 0) return;
-  const Span sp = tile_span<kFmt>(a, sq, (row0 + min(rows, kRows) - 1) / a.group);
+  const Span sp = tile_span<KB, kFreshKeys>(a, sq, (row0 + min(rows, kRows) - 1) / a.group);
   const int c_begin = split * a.split_chunks;
   const int c_end = min(sp.total, c_begin + a.split_chunks);
   if (split > 0 && c_begin >= c_end) return;  // this split has no keys (split 0 writes empty rows)
@@ -573,17 +488,17 @@ __global__ void __launch_bounds__(kThreads, 2) attn_chunk_kernel(const __grid_co
     cp_async_commit();
   };
   // Scales of chunk i, issued by the last issue(): 2^e of each key, 2^(e - e_max + 15) of
-  // each value, then the values' largest and smallest exponent.
+  // each value, then the values' largest exponent.
   auto put_scales = [&](int i) {
     if constexpr (kQuant) {
       if (i < n_mine && c_begin + warp + i * kWarps < sp.cached) {
         const uint32_t at = scale0 + (i % kStages) * kScaleBytes;
         const int ev = (int)pend_v - 127;
-        const int hi = __reduce_max_sync(0xffffffffu, pend_v != 0 ? ev : kNoExp);
-        const int lo = __reduce_min_sync(0xffffffffu, pend_v != 0 ? ev : 0x7fffffff);
-        const float2 x = make_float2(exp_scale(pend_k), pend_v != 0 ? pow2(ev - hi + 15) : 0.f);
+        const bool live = pend_v != 0 && pend_v != kNanByte;
+        const int hi = __reduce_max_sync(0xffffffffu, live ? ev : kNoExp);
+        const float2 x = make_float2(exp_scale(pend_k), live ? pow2(ev - hi + 15) : exp_scale(pend_v));
         asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at + lane * 8), "f"(x.x), "f"(x.y) : "memory");
-        if (lane == 0) asm volatile("st.shared.v2.s32 [%0], {%1, %2};" ::"r"(at + 32 * 8), "r"(hi), "r"(lo) : "memory");
+        if (lane == 0) asm volatile("st.shared.s32 [%0], %1;" ::"r"(at + 32 * 8), "r"(hi) : "memory");
       }
     }
   };
@@ -750,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_chunk_kernel(const __grid_co
 // lane four dimensions. The splits' maxima and sums are read 32 at a time, one
 // per lane, and their outputs eight at a time, so that no load waits for
 // another.
-template <int kFmt, int kRows>
+template <int KB, int FB, int kRows>
 __global__ void __launch_bounds__(256) attn_chunk_merge_kernel(const __grid_constant__ ChunkArgs a) {
   griddep_wait();
   griddep_launch_dependents();
@@ -765,7 +680,7 @@ __global__ void __launch_bounds__(256) attn_chunk_merge_kernel(const __grid_cons
   const int row0 = mtile * kRows;
   const int rows = sq.Lq * a.group - row0;
   if (row >= rows) return;
-  const Span sp = tile_span<kFmt>(a, sq, (row0 + min(rows, kRows) - 1) / a.group);
+  const Span sp = tile_span<KB, FB>(a, sq, (row0 + min(rows, kRows) - 1) / a.group);
   if (sp.total <= a.split_chunks) return;  // written by its only split
   const int n = (sp.total + a.split_chunks - 1) / a.split_chunks;
   const int64_t at = item * a.splits * kRows + row;
@@ -827,8 +742,8 @@ cudaError_t launch(const ChunkArgs& a, cudaStream_t stream) {
   e = launch_pdl(attn_chunk_kernel<kFmt, kMT, kR>, dim3((unsigned)(items * a.splits)), dim3(kThreads),
                  smem_bytes<kMT>(), stream, a);
   if (e != cudaSuccess || a.splits == 1) return e;
-  return launch_pdl(attn_chunk_merge_kernel<kFmt, kRows>, dim3((unsigned)((items * kRows + 7) / 8)), dim3(256), 0,
-                    stream, a);
+  return launch_pdl(attn_chunk_merge_kernel<chunk_keys<kFmt>(), kFreshKeys, kRows>,
+                    dim3((unsigned)((items * kRows + 7) / 8)), dim3(256), 0, stream, a);
 }
 
 template <int kFmt>
@@ -842,7 +757,19 @@ ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int 
                           int num_sms) {
   ChunkPlan p;
   const int64_t rows = (int64_t)max_q * group;
-  p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+  p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : kChunkMmaRows;
+  if (p.rows == kChunkMmaRows) {
+    // One CTA per SM. Splits only while SMs would have nothing to do, and four
+    // tiles of keys at least for each.
+    p.mtiles = (int)((rows + kChunkMmaRows - 1) / kChunkMmaRows);
+    const int64_t tiles = ((int64_t)max_context + 127) / 128 + ((int64_t)max_fresh + 127) / 128;
+    const int64_t units = (int64_t)B * Hkv * p.mtiles;
+    const int64_t splits = std::max<int64_t>(1, std::min(units > 0 ? num_sms / units : 1, tiles / 4));
+    p.split_chunks = (int)std::max<int64_t>(1, (tiles + splits - 1) / splits);
+    p.splits = (int)std::max<int64_t>(1, (tiles + p.split_chunks - 1) / p.split_chunks);
+    p.workspace_bytes = p.splits > 1 ? units * p.splits * p.rows * (chunk::kD * 4 + 8) : 0;
+    return p;
+  }
   p.mtiles = (int)((rows + p.rows - 1) / p.rows);
   const int kb = format == kFmtBf16 ? 16 : 32;
   const int64_t chunks = ((int64_t)max_context + kb - 1) / kb + ((int64_t)max_fresh + 15) / 16;
@@ -863,13 +790,23 @@ ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int 
   return p;
 }
 
-cudaError_t launch_attn_chunk(ChunkArgs a, int format, const ChunkPlan& plan, void* workspace, cudaStream_t stream) {
+cudaError_t launch_attn_chunk(ChunkArgs a, int format, const ChunkPlan& plan, const ChunkMaps& maps, void* workspace,
+                              int num_sms, cudaStream_t stream) {
   a.mtiles = plan.mtiles;
   a.splits = plan.splits;
   a.split_chunks = plan.split_chunks;
   const int64_t rows = (int64_t)a.B * a.Hkv * a.mtiles * a.splits * plan.rows;
   a.part_o = reinterpret_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * chunk::kD);
+  if (plan.rows == kChunkMmaRows) {
+    const int64_t items = (int64_t)a.B * a.Hkv * a.mtiles;
+    if (items * a.splits > 0x7fffffffLL) return cudaErrorInvalidValue;
+    a.total_units = (int)(items * a.splits);
+    cudaError_t e = launch_attn_chunk_mma(maps.k, maps.v, maps.kc, maps.vc, a, format, num_sms, stream);
+    if (e != cudaSuccess || a.splits == 1) return e;
+    return launch_pdl(chunk::attn_chunk_merge_kernel<128, 128, kChunkMmaRows>,
+                      dim3((unsigned)(items * (kChunkMmaRows / 8))), dim3(256), 0, stream, a);
+  }
   switch (format) {
     case kFmtBf16: return chunk::launch_rows<kFmtBf16>(a, plan.rows, stream);
     case kFmtE4m3: return chunk::launch_rows<kFmtE4m3>(a, plan.rows, stream);

@@ -3,6 +3,7 @@
 #pragma once
 
 #include <cstdint>
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 
@@ -49,13 +50,16 @@ struct ChunkArgs {
   int mtiles;              // row tiles per (sequence, KV head)
   int splits;              // key splits per row tile
   int split_chunks;        // key chunks of a split
+  int total_units;         // items * splits
   float* part_o;           // [items * splits, rows, 128] partial outputs (splits > 1)
   float2* part_ml;         // [items * splits, rows] (maximum, sum)
 };
 
+constexpr int kChunkMmaRows = 128;  // packed rows of a tile of the tcgen05 kernel
+
 // How a launch is laid out, from sizes the host knows.
 struct ChunkPlan {
-  int rows;                // packed rows of a tile: 8, 16 or 32
+  int rows;                // packed rows of a tile: 8 or 16 (attn_chunk.cu), 128 (attn_chunk_mma.cu)
   int mtiles;
   int splits;
   int split_chunks;
@@ -65,6 +69,18 @@ struct ChunkPlan {
 ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int max_context, int max_fresh,
                           int num_sms);
 
-cudaError_t launch_attn_chunk(ChunkArgs a, int format, const ChunkPlan& plan, void* workspace, cudaStream_t stream);
+// Tensor maps of a 128-row launch: fresh k / v (bf16 boxes of 64 x 1 x 128, 128-byte
+// swizzle), caches (the same, or 8-bit boxes of 128 x 1 x 128, no swizzle).
+struct ChunkMaps {
+  CUtensorMap k, v, kc, vc;
+};
+
+// maps: read only by 128-row launches.
+cudaError_t launch_attn_chunk(ChunkArgs a, int format, const ChunkPlan& plan, const ChunkMaps& maps, void* workspace,
+                              int num_sms, cudaStream_t stream);
+
+cudaError_t launch_attn_chunk_mma(const CUtensorMap& tmK, const CUtensorMap& tmV, const CUtensorMap& tmKc,
+                                  const CUtensorMap& tmVc, const ChunkArgs& a, int format, int num_sms,
+                                  cudaStream_t stream);
 
 }  // namespace dllm

@@ -92,6 +92,22 @@ int encode_rows_map(CUtensorMap* m, const void* ptr, int64_t rows, int heads, in
   return DLLM_OK;
 }
 
+// 3-D map over the codes of a quantised cache [slots, heads, 128] (one byte
+// each): box (128, 1, 128), no swizzle: 128 rows of 128 bytes.
+int encode_codes_map(CUtensorMap* m, const void* ptr, int64_t slots, int heads) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (enc == nullptr) return fail(DLLM_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[3] = {128, (cuuint64_t)heads, (cuuint64_t)slots};
+  cuuint64_t strides[2] = {128, (cuuint64_t)heads * 128};
+  cuuint32_t box[3] = {128, 1, 128};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(ptr), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(DLLM_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return DLLM_OK;
+}
+
 // 2-D map over a row-major bf16 matrix [rows, cols] (row stride in elements):
 // box (64 columns, box_rows rows), 128-byte swizzle (UMMA SW128 K-major).
 int encode_matrix_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t cols, int64_t row_stride,
@@ -513,7 +529,25 @@ int dllm_attn_chunk_fwd(const void* q, int64_t q_tok_stride, const void* k, int6
   a.o = static_cast<__nv_bfloat16*>(o);
   a.o_stride = o_tok_stride;
   a.err = err_flag;
-  cudaError_t e = dllm::launch_attn_chunk(a, format, plan, workspace, reinterpret_cast<cudaStream_t>(stream));
+  dllm::ChunkMaps maps = {};
+  if (plan.rows == dllm::kChunkMmaRows) {
+    if (k != nullptr) {
+      if ((rc = encode_rows_map(&maps.k, k, total_k, num_kv_heads, k_tok_stride, 128)) != DLLM_OK) return rc;
+      if ((rc = encode_rows_map(&maps.v, v, total_k, num_kv_heads, v_tok_stride, 128)) != DLLM_OK) return rc;
+    }
+    if (cached && num_slots > 0) {
+      const int64_t row = (int64_t)num_kv_heads * 128;
+      for (int i = 0; i < 2; ++i) {
+        CUtensorMap* m = i == 0 ? &maps.kc : &maps.vc;
+        const void* p = i == 0 ? k_cache : v_cache;
+        rc = format == DLLM_KV_BF16 ? encode_rows_map(m, p, num_slots, num_kv_heads, row, 128)
+                                    : encode_codes_map(m, p, num_slots, num_kv_heads);
+        if (rc != DLLM_OK) return rc;
+      }
+    }
+  }
+  cudaError_t e = dllm::launch_attn_chunk(a, format, plan, maps, workspace, num_sms_of_current_device(),
+                                          reinterpret_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "attn_chunk launch");
   return DLLM_OK;
 }

@@ -75,14 +75,21 @@ __global__ void __launch_bounds__(kThreads) kv_quant_kernel(KvQuantArgs a) {
       load32<kWide>(value, v);
     }
     // the lanes of a group are one token's, so they are all live or all idle
-    bool bad_k, bad_v;
+    uint32_t bad_k, bad_v;
     uint32_t mk = finite_max16(k, bad_k), mv = finite_max16(v, bad_v);
     uint32_t both = mk | (mv << 16);
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1) both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, o));
-    if (bad_k || bad_v) set_error(a.err, kDevNonFinite);
+    uint32_t ek = exp_byte<kFmt>(both & 0xffffu), ev = exp_byte<kFmt>(both >> 16);
+    if (__any_sync(0xffffffffu, (bad_k | bad_v) != 0)) {
+      uint32_t nan = (bad_k >> 1) | (bad_v & 2);  // bit 0: a NaN in the K row, bit 1: in the V row
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) nan |= __shfl_xor_sync(0xffffffffu, nan, o);
+      if (nan & 1) ek = kNanByte;
+      if (nan & 2) ev = kNanByte;
+      if (bad_k | bad_v) set_error(a.err, kDevNonFinite);
+    }
     if (!ok) return;
-    const uint32_t ek = exp_byte<kFmt>(both & 0xffffu), ev = exp_byte<kFmt>(both >> 16);
     *reinterpret_cast<uint4*>(a.k_cache + code) = quantise16<kFmt>(k, ek);
     *reinterpret_cast<uint4*>(a.v_cache + code) = quantise16<kFmt>(v, ev);
     if (part == 0) {
@@ -96,8 +103,8 @@ __global__ void __launch_bounds__(kThreads) kv_quant_kernel(KvQuantArgs a) {
       const uint4 ck = __ldg(reinterpret_cast<const uint4*>(a.k_cache + code));
       const uint4 cv = __ldg(reinterpret_cast<const uint4*>(a.v_cache + code));
       const uint32_t ek = a.k_exp[ex], ev = a.v_exp[ex];
-      dequantise16<kFmt>(ck, exp_scale(ek), k);
-      dequantise16<kFmt>(cv, exp_scale(ev), v);
+      dequantise16<kFmt>(ck, ek, k);
+      dequantise16<kFmt>(cv, ev, v);
     }
     store32<kWide>(key, k);
     store32<kWide>(value, v);

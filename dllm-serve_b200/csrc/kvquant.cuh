@@ -9,7 +9,8 @@
 // the exponent field of 2^e as a float; byte 0 (a slot never written) reads as
 // scale zero. e is clamped to [-100, e_max]: the lower end keeps every
 // nonzero dequantised value a normal bf16 number, the upper end keeps it
-// finite (the codes saturate there).
+// finite (the codes saturate there). Byte 255 marks a group with a NaN: all of
+// it reads as NaN.
 #pragma once
 
 #include "common.cuh"
@@ -47,8 +48,12 @@ DLLM_DEVICE uint32_t exp_byte(uint32_t amax) {
   return (uint32_t)min(max(b, kMinExpByte), KvFormat<kFmt>::kMaxByte);
 }
 
-// 2^(byte - 127), 0 for byte 0.
-DLLM_DEVICE float exp_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
+constexpr uint32_t kNanByte = 255;
+
+// 2^(byte - 127), 0 for byte 0, NaN for kNanByte.
+DLLM_DEVICE float exp_scale(uint32_t byte) {
+  return byte == kNanByte ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
+}
 
 // Four codes (in memory order) of y = x * 2^-e.
 template <int kFmt>
@@ -59,7 +64,7 @@ DLLM_DEVICE uint32_t encode4(float y0, float y1, float y2, float y3) {
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(y3), "f"(y2));
     return (uint32_t)lo | ((uint32_t)hi << 16);
   } else {
-    // NaN converts to 0, infinities saturate
+    // infinities saturate
     const int c0 = min(max(__float2int_rn(y0), -127), 127), c1 = min(max(__float2int_rn(y1), -127), 127);
     const int c2 = min(max(__float2int_rn(y2), -127), 127), c3 = min(max(__float2int_rn(y3), -127), 127);
     const uint32_t lo = __byte_perm((uint32_t)c0, (uint32_t)c1, 0x0040);
@@ -68,36 +73,14 @@ DLLM_DEVICE uint32_t encode4(float y0, float y1, float y2, float y3) {
   }
 }
 
-// Four codes -> values times `scale`, float32 (exact: scale is a power of two).
-template <int kFmt>
-DLLM_DEVICE void decode4(uint32_t w, float scale, float (&y)[4]) {
-  if constexpr (kFmt == kFmtE4m3) {
-    uint32_t h0, h1;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h0) : "h"((uint16_t)(w & 0xffffu)));
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h1) : "h"((uint16_t)(w >> 16)));
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h0));
-    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-    y[0] = a.x * scale;
-    y[1] = a.y * scale;
-    y[2] = b.x * scale;
-    y[3] = b.y * scale;
-  } else {
-    // byte + 128 into the low mantissa bits of 2^23, then subtract 2^23 + 128
-    const uint32_t u = w ^ 0x80808080u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      y[i] = (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + i)) - 8388736.f) * scale;
-  }
-}
-
-// Largest finite bf16 magnitude of eight words (pairs of bf16), and whether any
-// value is not finite.
-DLLM_DEVICE uint32_t finite_max16(const uint32_t (&w)[8], bool& bad) {
+// Largest finite bf16 magnitude of eight words (pairs of bf16). bad: 1 if any
+// value is infinite, 2 if any is NaN.
+DLLM_DEVICE uint32_t finite_max16(const uint32_t (&w)[8], uint32_t& bad) {
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
   m = max(m & 0xffffu, m >> 16);
-  bad = m >= 0x7f80u;
+  bad = m > 0x7f80u ? 2 : m == 0x7f80u ? 1 : 0;
   if (bad) {
     m = 0;
 #pragma unroll
@@ -113,6 +96,7 @@ DLLM_DEVICE uint32_t finite_max16(const uint32_t (&w)[8], bool& bad) {
 // Quantises 16 bf16 values (eight words) with the group's exponent byte.
 template <int kFmt>
 DLLM_DEVICE uint4 quantise16(const uint32_t (&w)[8], uint32_t byte) {
+  if (byte == kNanByte) return make_uint4(0, 0, 0, 0);
   const float inv = __uint_as_float((254u - byte) << 23);  // 2^-e
   uint32_t c[4];
 #pragma unroll
@@ -124,16 +108,94 @@ DLLM_DEVICE uint4 quantise16(const uint32_t (&w)[8], uint32_t byte) {
   return make_uint4(c[0], c[1], c[2], c[3]);
 }
 
-// 16 codes -> 16 bf16 values (eight words), exact.
+// Expansion of codes to bf16, exact. No conversion instruction: e4m3
+// conversions run at 16 per cycle and SM, the exponentials' rate, which the
+// attention kernels need for those.
+//
+// e4m3: the code s eeee mmm, put into a bf16 as s 0000eeee mmm0000, is the
+// value times 2^-120 (subnormal codes included, as subnormal bf16); one
+// product by 2^(120 + e) follows, or two where that is no bf16 (e > 7).
+// int8: the code + 128 in the low mantissa bits of 2^23 is 2^23 + 128 + code;
+// one fma by 2^e takes the bias off, or a subtraction and a product where
+// 2^(23 + e) is no float (e > 100).
+// Groups that need the second form are rare: `exp_is_big`.
 template <int kFmt>
-DLLM_DEVICE void dequantise16(uint4 c, float scale, uint32_t (&w)[8]) {
+DLLM_DEVICE bool exp_is_big(uint32_t byte) {
+  return kFmt == kFmtE4m3 ? byte > 7 + 127 : byte > 100 + 127;  // (a NaN's byte too)
+}
+
+// What a group's codes are multiplied by (not for big exponents).
+template <int kFmt>
+DLLM_DEVICE float2 code_scale(uint32_t byte) {
+  if constexpr (kFmt == kFmtE4m3) {
+    const uint32_t s = byte == 0 ? 0u : (byte + 120) << 7;
+    return make_float2(__uint_as_float(s | (s << 16)), 0.f);  // a bf16 pair
+  } else {
+    const float s = exp_scale(byte);
+    return make_float2(s, -8388736.f * s);
+  }
+}
+
+// e4m3 codes of a word as four bf16, times 2^-120.
+DLLM_DEVICE void e4m3_bits(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const uint32_t h = ((w >> 4) & 0x07070707u) | (w & 0x80808080u);  // upper bytes
+  const uint32_t l = (w & 0x0f0f0f0fu) << 4;                        // lower bytes
+  lo = __byte_perm(l, h, 0x5140);
+  hi = __byte_perm(l, h, 0x7362);
+}
+
+DLLM_DEVICE uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 z = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&z);
+}
+
+// 16 codes -> 16 bf16 values (eight words), with code_scale() of the group.
+template <int kFmt>
+DLLM_DEVICE void expand16(uint4 c, float2 scale, uint32_t (&w)[8]) {
   const uint32_t cs[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float y[4];
-    decode4<kFmt>(cs[i], scale, y);
-    w[2 * i] = pack_bf16x2(y[0], y[1]);
-    w[2 * i + 1] = pack_bf16x2(y[2], y[3]);
+    if constexpr (kFmt == kFmtE4m3) {
+      uint32_t lo, hi;
+      e4m3_bits(cs[i], lo, hi);
+      w[2 * i] = mul_bf16x2(lo, __float_as_uint(scale.x));
+      w[2 * i + 1] = mul_bf16x2(hi, __float_as_uint(scale.x));
+    } else {
+      const uint32_t u = cs[i] ^ 0x80808080u;
+      float y[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) y[k] = fmaf(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + k)), scale.x, scale.y);
+      w[2 * i] = pack_bf16x2(y[0], y[1]);
+      w[2 * i + 1] = pack_bf16x2(y[2], y[3]);
+    }
+  }
+}
+
+// The same for any exponent byte.
+template <int kFmt>
+DLLM_DEVICE void dequantise16(uint4 c, uint32_t byte, uint32_t (&w)[8]) {
+  if (!exp_is_big<kFmt>(byte)) {
+    expand16<kFmt>(c, code_scale<kFmt>(byte), w);
+    return;
+  }
+  const uint32_t cs[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (kFmt == kFmtE4m3) {
+      const uint32_t s = byte == kNanByte ? 0x7fc0u : (byte + 6) << 7;  // 2^114, then 2^(e + 6)
+      uint32_t lo, hi;
+      e4m3_bits(cs[i], lo, hi);
+      w[2 * i] = mul_bf16x2(mul_bf16x2(lo, 0x78807880u), s | (s << 16));
+      w[2 * i + 1] = mul_bf16x2(mul_bf16x2(hi, 0x78807880u), s | (s << 16));
+    } else {
+      const float s = exp_scale(byte);
+      const uint32_t u = cs[i] ^ 0x80808080u;
+      float y[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) y[k] = (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + k)) - 8388736.f) * s;
+      w[2 * i] = pack_bf16x2(y[0], y[1]);
+      w[2 * i + 1] = pack_bf16x2(y[2], y[3]);
+    }
   }
 }
 

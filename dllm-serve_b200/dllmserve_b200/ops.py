@@ -172,8 +172,8 @@ def store_kvcache_quant(key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping
     With a the row's largest finite magnitude and M the format's largest value
     (448 or 127), the scale is 2^e, e the smallest integer with a <= M * 2^e
     (clamped to [-100, 119] / [-100, 121]); codes are x * 2^-e rounded to
-    nearest even and the byte e + 127 is kept. Infinities saturate, NaN is kept
-    (e4m3) or becomes 0 (int8); both set DLLM_DEV_NON_FINITE in the device
+    nearest even and the byte e + 127 is kept. Infinities saturate, a row with
+    a NaN reads as NaN throughout; both set DLLM_DEV_NON_FINITE in the device
     status word."""
     _kv_quant(True, key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping)
 

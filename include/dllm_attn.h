@@ -145,8 +145,9 @@ DLLM_API int dllm_load_kvcache(void* key, int64_t key_stride, void* value, int64
  * Both products are exact, so the code's rounding is the only one: at most half a step
  * of the format, and every value a code stands for is a bf16 number. Byte 0, which the
  * store never writes, stands for scale 0: a cache of zero bytes reads as zeros.
- * Infinities are stored as +-M * 2^e, NaN as NaN (e4m3) or 0 (int8); either flags
- * DLLM_DEV_NON_FINITE in err_flag.
+ * Infinities are stored as +-M * 2^e; a group with a NaN keeps byte 255 and reads as NaN
+ * throughout (e4m3's own NaN code is never written and must not be in a cache that these
+ * entry points read). Either flags DLLM_DEV_NON_FINITE in err_flag.
  *
  * k_cache, v_cache: num_slots rows of num_kv_heads * head_dim bytes; k_exp, v_exp:
  * num_slots rows of num_kv_heads bytes. key, value: bf16 [n_tokens, num_kv_heads,

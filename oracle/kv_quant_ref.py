@@ -16,7 +16,7 @@ TOP = {"e4m3": (448.0, 119), "int8": (127.0, 121)}
 def exponent(row: torch.Tensor, fmt: str) -> int:
     """The smallest e with a <= M * 2^e, a the row's largest finite magnitude."""
     top, e_max = TOP[fmt]
-    x = row.double().abs()
+    x = row.double().abs()  # (a row with a NaN has no value of its own: the cache marks it)
     x = x[torch.isfinite(x)]
     a = float(x.max()) if x.numel() else 0.0
     if a == 0.0:

@@ -183,6 +183,47 @@ def test_long(dev, fmt, shape, causal, tables):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3", "int8"])
+@pytest.mark.parametrize("tables", [True, False])
+def test_many_units(dev, fmt, tables):
+    """More row tiles than the GPU has SMs, of unequal lengths, so that a CTA
+    takes several one after another: each sequence's rows equal, bit for bit,
+    those of a launch of its own, and a few are held to the 64-bit bound."""
+    g = I.gen(17)
+    n = 90
+    nq = torch.randint(0, 60, (n,), generator=g).tolist()
+    nc = torch.randint(0, 500, (n,), generator=g).tolist()
+    nc[3], nc[40], nq[7], nq[40] = 0, 0, 0, 33
+    nf = [x if i % 3 else min(x, 17) for i, x in enumerate(nq)]
+    c = Case(18, fmt, 12, 4, nq, nc, nf, tables, page=128, spread=False)
+    args, kw = c.args(dev)
+    ops = _ops()
+    for causal in (False, True):
+        out = ops.chunk_attention(*args, causal=causal, max_context=512, **kw)
+        c.check(out, causal, seqs=[3, 7, 11, 40])
+        for _ in range(3):  # launches back to back
+            again = ops.chunk_attention(*args, causal=causal, max_context=512, **kw)
+        assert torch.equal(again[:sum(nq)], out[:sum(nq)])
+        cu, cuk, cus = (_cu(x).tolist() for x in (nq, nf, nc))
+        for b in range(0, n, 4):
+            if nq[b] == 0:
+                continue
+            one = dict(kw)
+            one |= {"k": kw["k"][cuk[b]:cuk[b + 1]], "v": kw["v"][cuk[b]:cuk[b + 1]], "cu_seqlens_k": _cu([nf[b]]).to(dev)}
+            if tables:
+                one |= {"block_tables": kw["block_tables"][b:b + 1], "context_lens": kw["context_lens"][b:b + 1]}
+            else:
+                one |= {"slots": kw["slots"][cus[b]:cus[b + 1]], "cu_seqlens_slots": _cu([nc[b]]).to(dev)}
+            if nf[b] == 0 and nc[b] == 0:
+                assert (out[cu[b]:cu[b + 1]] == 0).all()
+                continue
+            alone = ops.chunk_attention(args[0][cu[b]:cu[b + 1]], *args[1:3], _cu([nq[b]]).to(dev), max(nq),
+                                        causal=causal, max_context=512, **one)
+            assert torch.equal(alone, out[cu[b]:cu[b + 1]]), b
+    assert ops.read_device_status(dev) == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
 def test_fresh_only(dev, fmt):
     """No cache at all: causal attention among the chunk's own rows."""
