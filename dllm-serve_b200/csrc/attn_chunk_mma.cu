@@ -12,19 +12,22 @@
 // softmax of a union). Probabilities are rounded to bf16 (2^-8 of their value).
 //
 // Quantised caches: 8-bit rows are brought into shared memory as they are
-// (TMA, or one bulk copy per row where the slots are scattered) and a fourth
-// warpgroup expands them into the bf16 stages that the matrix instructions
+// (TMA, or one bulk copy per row where the slots are scattered) and two more
+// warpgroups expand them into the bf16 stages that the matrix instructions
 // read. Every value a code stands for is a bf16 number, so this rounds
 // nothing, and the rest of the kernel is the same for every format. HBM and
 // L2 carry one byte per element.
 //
-// Roles (16 warps):
+// Roles (16 warps, 20 with a quantised cache):
 //   warps 0-3, 4-7  softmax warpgroups: columns 0-63 / 64-127 of every tile
 //   warp 8          loader of K: bf16 stages, or the raw K ring of a quantised cache
 //   warp 9          issues the MMAs, owns TMEM
 //   warp 10         loader of V
-//   warps 12-15     stage Q; with a quantised cache fill the bf16 stages: expand
-//                   cached tiles, load fresh ones
+//   warps 12-15     bf16: stage Q. Quantised: fill the K ring (expand cached
+//                   tiles, load fresh ones)
+//   warps 16-19     quantised: stage Q, fill the V ring
+// One warpgroup for both rings was the bottleneck: 1,560 cycles to expand a
+// tile of K or V, 4,270 per KV tile against 2,290 of the bf16 kernel.
 // TMEM (512 columns): S buffers [0,128) [128,256), O of each warpgroup at 256
 // and 384; P (bf16) over the first 32 columns of its half of S. MMA order per
 // tile j: PV(j) of both halves, then QK(j+2).
@@ -49,7 +52,6 @@ constexpr int kD = 128;
 constexpr int kTileM = kChunkMmaRows;
 constexpr int kTileN = 128;
 constexpr int kHalfN = 64;
-constexpr int kThreads = 512;
 constexpr uint32_t kTileBytes = 128 * kD * 2;  // bf16 tile
 constexpr uint32_t kChunkBytes = 128 * 128;    // its 64-column half; also an 8-bit tile
 constexpr int kRaw = 2;                        // stages of each raw ring
@@ -57,6 +59,11 @@ constexpr int kRaw = 2;                        // stages of each raw ring
 template <int kFmt>
 struct Layout {
   static constexpr bool kQuant = kFmt != kFmtBf16;
+  // Registers: the softmax warpgroups take those that the other roles do not need.
+  // bf16: 512 x 128 = 256 x 168 + 256 x 88; quantised: 640 x 96 = 256 x 144 + 384 x 64.
+  static constexpr int kThreads = kQuant ? 640 : 512;
+  static constexpr int kRegsSoftmax = kQuant ? 144 : 168;
+  static constexpr int kRegsOther = kQuant ? 64 : 88;
   static constexpr int kStagesK = kQuant ? 2 : 3;
   static constexpr int kStagesV = kQuant ? 2 : 3;
   // arrivals that complete a bf16 stage: the four expanding warps, or the loader's
@@ -169,6 +176,14 @@ DLLM_DEVICE void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32
                : "memory");
 }
 
+template <int kRegs, bool kMore>
+DLLM_DEVICE void set_max_registers() {
+  if constexpr (kMore)
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+  else
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+
 // The matrix instructions with descriptors given as their low words: the high
 // word (stride 1024, 128-byte swizzle) is the same for every tile here, and
 // one 32-bit word per operand keeps the issuing thread's registers few.
@@ -219,7 +234,7 @@ DLLM_DEVICE float exp_store_half(const uint32_t (&s)[2][32], float sl2, float m,
 }  // namespace
 
 template <int kFmt>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
     attn_chunk_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                           const __grid_constant__ CUtensorMap tmKc, const __grid_constant__ CUtensorMap tmVc,
                           const __grid_constant__ ChunkArgs a) {
@@ -278,11 +293,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   griddep_wait();
   griddep_launch_dependents();
 
-  // The softmax warpgroups take registers that the other roles do not need:
-  // 256 x 168 + 256 x 88 = 512 x 128 (stated inside each role's branch, where
-  // the compiler takes it into account).
+  // Register counts are stated inside each role's branch, where the compiler
+  // takes them into account.
   if (warp >= 8 && warp < 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    set_max_registers<S::kRegsOther, false>();
     if (warp == 8 || warp == 10) {
     // ---------------------------------------------------------------- loaders
     const bool is_k = warp == 8;
@@ -549,22 +563,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   }
   } else if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    set_max_registers<S::kRegsOther, false>();
     // ------------------------------------------------- Q staging and expansion
-    const int tid = threadIdx.x - 12 * 32;
-    uint32_t q_it = 0, k_it = 0, v_it = 0, rk = 0, rv = 0, land = 0;
+    // Quantised caches: warps 12-15 fill the K ring, warps 16-19 the V ring; the last four of the
+    // CTA stage Q (with a quantised cache while the first K tile is expanded).
+    const bool is_k = kQuant && warp < 16;
+    const int lead = kQuant && !is_k ? 16 : 12;  // this warpgroup's first warp
+    const int tid = threadIdx.x - lead * 32;
+    const int nst = is_k ? kStagesK : kStagesV;
+    const int bfull = is_k ? S::BAR_KFULL : S::BAR_VFULL, bempty = is_k ? S::BAR_KEMPTY : S::BAR_VEMPTY;
+    const int rfull = S::BAR_RFULL + (is_k ? 0 : kRaw), rempty = S::BAR_REMPTY + (is_k ? 0 : kRaw);
+    const uint32_t ring = is_k ? S::kOffK : S::kOffV;
+    uint32_t q_it = 0;  // units whose Q was staged
+    uint32_t n = 0;     // ring positions filled; every position is filled by this warpgroup, in order, so each
+                        // wait below is for the phase right before (a wait by parity cannot tell phases two apart)
+    uint32_t raw_it = 0, land = 0;
     bool ok = true;
-    // expands the raw tile of ring position `r` into bf16 ring position `n`
-    auto expand = [&](bool is_k, uint32_t r, uint32_t n) -> bool {
-      const int nst = is_k ? kStagesK : kStagesV, st = n % nst, rs = r % kRaw;
+    // expands the raw tile `raw_it` into ring position n
+    auto expand = [&]() -> bool {
+      const int st = n % nst, rs = raw_it % kRaw;
+      if (!mbar_wait_warp(bar(rfull + rs), (raw_it / kRaw) & 1, abort_flag)) return false;
+      if (n >= (uint32_t)nst && !mbar_wait_warp(bar(bempty + st), (n / nst - 1) & 1, abort_flag)) return false;
       const int rb = (is_k ? 0 : kRaw) + rs;
-      if (!mbar_wait_warp(bar(S::BAR_RFULL + rb), (r / kRaw) & 1, abort_flag)) return false;
-      if (n >= (uint32_t)nst &&
-          !mbar_wait_warp(bar((is_k ? S::BAR_KEMPTY : S::BAR_VEMPTY) + st), (n / nst - 1) & 1, abort_flag))
-        return false;
       const uint8_t* src = smem + S::kOffRaw + rb * kChunkBytes;
       const uint8_t* ex = smem + S::kOffExp + rb * 128;
-      uint8_t* dst = smem + (is_k ? S::kOffK : S::kOffV) + st * kTileBytes;
+      uint8_t* dst = smem + ring + st * kTileBytes;
       const int un = tid & 7;  // 16 codes: 16-byte units 2 un, 2 un + 1 of the row's bf16 form
       const int r0 = tid >> 3;
       uint32_t e[8];
@@ -610,38 +633,34 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_proxy_async_smem();  // generic-proxy writes -> tensor-core reads
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(bar((is_k ? S::BAR_KFULL : S::BAR_VFULL) + st));
-        mbar_arrive(bar(S::BAR_REMPTY + rb));
+        mbar_arrive(bar(bfull + st));
+        mbar_arrive(bar(rempty + rs));
       }
       return true;
     };
-    // Loads a fresh tile into ring position `n` by TMA: warp 12 issues it, the others arrive. Every
-    // position of both rings is filled by these warps, in order, so each wait here is for the phase
-    // right before the one it fills (a wait by parity cannot tell phases two apart).
-    auto direct = [&](bool is_k, uint32_t n, const Unit& t, const KvTile& kt) -> bool {
-      const int nst = is_k ? kStagesK : kStagesV, st = n % nst;
-      if (n >= (uint32_t)nst &&
-          !mbar_wait_warp(bar((is_k ? S::BAR_KEMPTY : S::BAR_VEMPTY) + st), (n / nst - 1) & 1, abort_flag))
-        return false;
-      const uint32_t full = bar((is_k ? S::BAR_KFULL : S::BAR_VFULL) + st);
-      if (warp != 12) {
+    // loads a fresh tile into ring position n by TMA: the first warp issues it, the others arrive
+    auto direct = [&](int hkv, const KvTile& kt) -> bool {
+      const int st = n % nst;
+      if (n >= (uint32_t)nst && !mbar_wait_warp(bar(bempty + st), (n / nst - 1) & 1, abort_flag)) return false;
+      const uint32_t full = bar(bfull + st);
+      if (warp != lead) {
         if (lane == 0) mbar_arrive(full);
         return true;
       }
       const bool clear = !is_k && (kt.valid & 15) != 0;
       const uint32_t fb = clear ? bar(S::BAR_VLAND) : full;
-      const uint32_t dst = base + (is_k ? S::kOffK : S::kOffV) + st * kTileBytes;
+      const uint32_t dst = ring + st * kTileBytes;
       if (lane == 0) {
         const uint64_t pol = policy_evict_last();
         const CUtensorMap* mp = is_k ? &tmK : &tmV;
         mbar_arrive_expect_tx(fb, kTileBytes);
-        tma_load_3d(dst, mp, fb, 0, t.hkv, (int)kt.row, pol);
-        tma_load_3d(dst + kChunkBytes, mp, fb, 64, t.hkv, (int)kt.row, pol);
+        tma_load_3d(base + dst, mp, fb, 0, hkv, (int)kt.row, pol);
+        tma_load_3d(base + dst + kChunkBytes, mp, fb, 64, hkv, (int)kt.row, pol);
       }
       if (clear) {
         if (!mbar_wait_warp(fb, land & 1, abort_flag)) return false;
         ++land;
-        clear_tail(smem + (dst - base), kt.valid, lane);
+        clear_tail(smem + dst, kt.valid, lane);
         if (lane == 0) mbar_arrive(full);
       }
       return true;
@@ -649,55 +668,52 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int u = blockIdx.x; u < total_units && ok; u += gridDim.x) {
       const Unit t = decode_unit(u, a, false);
       if (!t.valid || t.nkv == 0) continue;
-      if (q_it > 0) ok = mbar_wait_warp(bar(S::BAR_QEMPTY), (q_it - 1) & 1, abort_flag);
-      if (!ok) break;
-      ++q_it;
+      if (!is_k) {
+        if (q_it > 0) ok = mbar_wait_warp(bar(S::BAR_QEMPTY), (q_it - 1) & 1, abort_flag);
+        if (!ok) break;
+        ++q_it;
 #pragma unroll 1
-      for (int i0 = 0; i0 < 16; i0 += 8) {
-        uint4 val[8];
+        for (int i0 = 0; i0 < 16; i0 += 4) {
+          uint4 val[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int p = (i0 + i) * 8 + (tid >> 4);
-          val[i] = make_uint4(0, 0, 0, 0);
-          if (p < t.rows) {
-            const int r = (t.row0 + p) / a.group, h = t.hkv * a.group + (t.row0 + p) - r * a.group;
-            val[i] = __ldg(reinterpret_cast<const uint4*>(a.q + (t.sq.q_begin + r) * a.q_stride + (int64_t)h * kD) + (tid & 15));
+          for (int i = 0; i < 4; ++i) {
+            const int p = (i0 + i) * 8 + (tid >> 4);
+            val[i] = make_uint4(0, 0, 0, 0);
+            if (p < t.rows) {
+              const int r = (t.row0 + p) / a.group, h = t.hkv * a.group + (t.row0 + p) - r * a.group;
+              val[i] = __ldg(reinterpret_cast<const uint4*>(a.q + (t.sq.q_begin + r) * a.q_stride + (int64_t)h * kD) + (tid & 15));
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int p = (i0 + i) * 8 + (tid >> 4), c = tid & 15;
+            *reinterpret_cast<uint4*>(smem + S::kOffQ + (c >> 3) * kChunkBytes + p * 128 + (((c & 7) ^ (p & 7)) << 4)) = val[i];
           }
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int p = (i0 + i) * 8 + (tid >> 4), c = tid & 15;
-          *reinterpret_cast<uint4*>(smem + S::kOffQ + (c >> 3) * kChunkBytes + p * 128 + (((c & 7) ^ (p & 7)) << 4)) = val[i];
-        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(S::BAR_QFULL));
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(S::BAR_QFULL));
       if constexpr (kQuant) {
-        // K tiles run one ahead of V tiles
-        for (int j = 0; j <= t.nkv && ok; ++j) {
-          if (j < t.nkv) {
-            ok = t.t0 + j < t.sp.cached ? expand(true, rk++, k_it) : direct(true, k_it, t, kv_tile(t, j));
-            ++k_it;
-          }
-          if (ok && j > 0) {
-            ok = t.t0 + j - 1 < t.sp.cached ? expand(false, rv++, v_it) : direct(false, v_it, t, kv_tile(t, j - 1));
-            ++v_it;
+        for (int j = 0; j < t.nkv && ok; ++j, ++n) {
+          if (t.t0 + j < t.sp.cached) {
+            ok = expand();
+            ++raw_it;
+          } else {
+            ok = direct(t.hkv, kv_tile(t, j));
           }
         }
       }
     }
-    if (kQuant && warp == 12 && lane == 0 && *abort_flag) {
+    if (kQuant && warp == lead && lane == 0 && *abort_flag) {
       // Drain: fresh tiles' copies that may still be in flight.
-      for (uint32_t n = (k_it > (uint32_t)kStagesK ? k_it - kStagesK : 0); n < k_it; ++n)
-        mbar_wait_drain(bar(S::BAR_KFULL + n % kStagesK), (n / kStagesK) & 1, 100000000ull);
-      for (uint32_t n = (v_it > (uint32_t)kStagesV ? v_it - kStagesV : 0); n < v_it; ++n)
-        mbar_wait_drain(bar(S::BAR_VFULL + n % kStagesV), (n / kStagesV) & 1, 100000000ull);
-      mbar_wait_drain(bar(S::BAR_VLAND), land & 1, 100000000ull);
+      for (uint32_t i = (n > (uint32_t)nst ? n - nst : 0); i < n; ++i)
+        mbar_wait_drain(bar(bfull + i % nst), (i / nst) & 1, 100000000ull);
+      if (!is_k) mbar_wait_drain(bar(S::BAR_VLAND), land & 1, 100000000ull);
     }
     __syncwarp();
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    set_max_registers<S::kRegsSoftmax, true>();
     // ---------------------------------------------------------------- softmax
     const int wg = warp >> 2;           // 0: keys 0-63 of a tile, 1: keys 64-127
     const int wq = warp & 3;
@@ -879,7 +895,7 @@ cudaError_t launch(const CUtensorMap& tmK, const CUtensorMap& tmV, const CUtenso
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
-  return launch_pdl(attn_chunk_mma_kernel<kFmt>, dim3(std::min(a.total_units, num_sms)), dim3(kThreads),
+  return launch_pdl(attn_chunk_mma_kernel<kFmt>, dim3(std::min(a.total_units, num_sms)), dim3(Layout<kFmt>::kThreads),
                     Layout<kFmt>::kSmemBytes, stream, tmK, tmV, tmKc, tmVc, a);
 }
 
