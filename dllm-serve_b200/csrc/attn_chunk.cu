@@ -802,7 +802,7 @@ cudaError_t launch_attn_chunk(ChunkArgs a, int format, const ChunkPlan& plan, co
     const int64_t items = (int64_t)a.B * a.Hkv * a.mtiles;
     if (items * a.splits > 0x7fffffffLL) return cudaErrorInvalidValue;
     a.total_units = (int)(items * a.splits);
-    cudaError_t e = launch_attn_chunk_mma(maps.k, maps.v, maps.kc, maps.vc, a, format, num_sms, stream);
+    cudaError_t e = launch_attn_chunk_mma(maps, a, format, num_sms, stream);
     if (e != cudaSuccess || a.splits == 1) return e;
     return launch_pdl(chunk::attn_chunk_merge_kernel<128, 128, kChunkMmaRows>,
                       dim3((unsigned)(items * (kChunkMmaRows / 8))), dim3(256), 0, stream, a);

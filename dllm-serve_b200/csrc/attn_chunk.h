@@ -70,17 +70,17 @@ ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int 
                           int num_sms);
 
 // Tensor maps of a 128-row launch: fresh k / v (bf16 boxes of 64 x 1 x 128, 128-byte
-// swizzle), caches (the same, or 8-bit boxes of 128 x 1 x 128, no swizzle).
+// swizzle); caches (the same, or 8-bit boxes of 128 x 1 x 128, no swizzle); caches as
+// [slots, Hkv * 128] matrices with boxes of one 128-byte row, for scattered slots.
 struct ChunkMaps {
-  CUtensorMap k, v, kc, vc;
+  CUtensorMap k, v, kc, vc, kg, vg;
 };
 
 // maps: read only by 128-row launches.
 cudaError_t launch_attn_chunk(ChunkArgs a, int format, const ChunkPlan& plan, const ChunkMaps& maps, void* workspace,
                               int num_sms, cudaStream_t stream);
 
-cudaError_t launch_attn_chunk_mma(const CUtensorMap& tmK, const CUtensorMap& tmV, const CUtensorMap& tmKc,
-                                  const CUtensorMap& tmVc, const ChunkArgs& a, int format, int num_sms,
+cudaError_t launch_attn_chunk_mma(const ChunkMaps& maps, const ChunkArgs& a, int format, int num_sms,
                                   cudaStream_t stream);
 
 }  // namespace dllm

@@ -12,7 +12,7 @@
 // softmax of a union). Probabilities are rounded to bf16 (2^-8 of their value).
 //
 // Quantised caches: 8-bit rows are brought into shared memory as they are
-// (TMA, or one bulk copy per row where the slots are scattered) and two more
+// (TMA boxes, or four rows at a time where the slots are scattered) and two more
 // warpgroups expand them into the bf16 stages that the matrix instructions
 // read. Every value a code stands for is a bf16 number, so this rounds
 // nothing, and the rest of the kernel is the same for every format. HBM and
@@ -170,10 +170,14 @@ DLLM_DEVICE void clear_tail(uint8_t* tile, int valid, int lane) {
   __syncwarp();
 }
 
-DLLM_DEVICE void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
+// Four rows (any order) of a 2-D tensor map whose box is one row: they land one
+// after another. A row index past the map's end gives zeros.
+DLLM_DEVICE void tma_gather4(uint32_t dst, const void* tmap, uint32_t bar, int x, const int (&r)[4]) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+      : "memory");
 }
 
 template <int kRegs, bool kMore>
@@ -237,6 +241,7 @@ template <int kFmt>
 __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
     attn_chunk_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                           const __grid_constant__ CUtensorMap tmKc, const __grid_constant__ CUtensorMap tmVc,
+                          const __grid_constant__ CUtensorMap tmKg, const __grid_constant__ CUtensorMap tmVg,
                           const __grid_constant__ ChunkArgs a) {
   using S = Layout<kFmt>;
   constexpr bool kQuant = S::kQuant;
@@ -308,11 +313,10 @@ __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
     const int rfull = S::BAR_RFULL + (is_k ? 0 : kRaw), rempty = S::BAR_REMPTY + (is_k ? 0 : kRaw);
     const uint32_t raw_ring = base + S::kOffRaw + (is_k ? 0 : kRaw * kChunkBytes);
     const uint32_t exp_ring = base + S::kOffExp + (is_k ? 0 : kRaw * 128);
-    const uint8_t* cache = is_k ? a.kc : a.vc;
     const uint8_t* exps = is_k ? a.k_exp : a.v_exp;
     const CUtensorMap* mfresh = is_k ? &tmK : &tmV;
     const CUtensorMap* mcache = is_k ? &tmKc : &tmVc;
-    const int row_bytes = kQuant ? kD : 2 * kD;  // a (slot, head) row
+    const CUtensorMap* mgather = is_k ? &tmKg : &tmVg;
     uint32_t done = 0;                           // tiles passed in the bf16 ring
     uint32_t raw_done = 0;                       // tiles issued into the raw ring
     uint32_t land = 0;                           // partial V tiles landed
@@ -326,17 +330,18 @@ __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
         if (kQuant && kt.fresh) break;  // the expanding warps load fresh tiles, which come last
         const int st = done % nst;
         // cached tiles: this lane's four rows 4 * lane + i, and whether the tile is one run of slots
-        int64_t sl[4], s0 = 0;
+        int sl[4], s0 = 0;
         bool contig = true;
         if (!kt.fresh) {
           if (table != nullptr && a.block_size % kTileN == 0) {
             // the tile lies inside one block
             const int blk = kt.pos / a.block_size;
             const int e = blk < a.max_blocks ? table[blk] : -1;
-            s0 = e < 0 ? -1 : (int64_t)e * a.block_size + kt.pos % a.block_size;
-            contig = s0 >= 0 && s0 + kt.valid <= a.num_slots;
+            const int64_t at = e < 0 ? -1 : (int64_t)e * a.block_size + kt.pos % a.block_size;
+            const bool in = at >= 0 && at < a.num_slots;
+            s0 = in ? (int)at : (int)a.num_slots;  // past the cache: the copy brings zeros
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sl[i] = s0 < 0 ? -1 : s0 + 4 * lane + i;
+            for (int i = 0; i < 4; ++i) sl[i] = in ? s0 + 4 * lane + i : -1;
           } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -346,14 +351,15 @@ __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
                 if (table != nullptr) {
                   const int blk = pos / a.block_size;
                   const int e = blk < a.max_blocks ? table[blk] : -1;
-                  if (e >= 0) sl[i] = (int64_t)e * a.block_size + pos % a.block_size;
+                  const int64_t at = e < 0 ? -1 : (int64_t)e * a.block_size + pos % a.block_size;
+                  sl[i] = at < a.num_slots ? (int)at : -1;
                 } else {
                   sl[i] = a.slots[t.sq.s_begin + pos];
                 }
               }
             }
             s0 = __shfl_sync(0xffffffffu, sl[0], 0);
-            contig = s0 >= 0 && s0 + kt.valid <= a.num_slots;
+            contig = s0 >= 0 && (int64_t)s0 + kt.valid <= a.num_slots;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               if (4 * lane + i < kt.valid && sl[i] != s0 + 4 * lane + i) contig = false;
@@ -378,24 +384,20 @@ __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
           if (contig) {
             if (lane == 0) {
               mbar_arrive_expect_tx(fb, kChunkBytes);
-              tma_load_3d(dst, mcache, fb, 0, t.hkv, (int)s0, pol);
+              tma_load_3d(dst, mcache, fb, 0, t.hkv, s0, pol);
             }
           } else {
-            int n = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) n += sl[i] >= 0 ? 1 : 0;
-            n = __reduce_add_sync(0xffffffffu, n);
-            if (lane == 0) mbar_arrive_expect_tx(fb, n * kD);
+            if (lane == 0) mbar_arrive_expect_tx(fb, kChunkBytes);
             __syncwarp();
+            int r[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (sl[i] >= 0)
-                bulk_load(dst + (4 * lane + i) * kD, cache + (sl[i] * a.Hkv + t.hkv) * (int64_t)kD, kD, fb);
+            for (int i = 0; i < 4; ++i) r[i] = sl[i] >= 0 ? sl[i] : (int)a.num_slots;
+            tma_gather4(dst + 4 * lane * kD, mgather, fb, t.hkv * kD, r);
           }
           uint32_t e4 = 0;
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (sl[i] >= 0) e4 |= (uint32_t)exps[sl[i] * a.Hkv + t.hkv] << (8 * i);
+            if (sl[i] >= 0) e4 |= (uint32_t)exps[(int64_t)sl[i] * a.Hkv + t.hkv] << (8 * i);
           *reinterpret_cast<uint32_t*>(smem + (exp_ring - base) + rs * 128 + 4 * lane) = e4;
           __syncwarp();
           if (lane == 0) mbar_arrive(fb);
@@ -407,46 +409,28 @@ __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
         const uint32_t dst = ring + st * kTileBytes;
         uint8_t* tile = smem + (dst - base);
         const bool clear = !is_k && (kt.valid & 15) != 0;
+        const uint32_t fb = bar(clear ? S::BAR_VLAND : bfull + st);
+        if (lane == 0) mbar_arrive_expect_tx(fb, kTileBytes);
+        __syncwarp();
         if (kt.fresh || contig) {
-          const uint32_t fb = bar(clear ? S::BAR_VLAND : bfull + st);
           if (lane == 0) {
-            mbar_arrive_expect_tx(fb, kTileBytes);
             const CUtensorMap* mp = kt.fresh ? mfresh : mcache;
-            const int row = kt.fresh ? (int)kt.row : (int)s0;
+            const int row = kt.fresh ? (int)kt.row : s0;
             tma_load_3d(dst, mp, fb, 0, t.hkv, row, pol);
             tma_load_3d(dst + kChunkBytes, mp, fb, 64, t.hkv, row, pol);
           }
-          if (clear) {
-            ok = mbar_wait_warp(bar(S::BAR_VLAND), land & 1, abort_flag);
-            if (!ok) break;
-            ++land;
-            clear_tail(tile, kt.valid, lane);
-            if (lane == 0) mbar_arrive(bar(bfull + st));
-          }
         } else {
-          // scattered slots: the warp gathers the rows (half a row per step), dead rows as zeros
-#pragma unroll 1
-          for (int r0 = 0; r0 < kTileN; r0 += 16) {
-            uint4 val[8];
+          int r[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int r = r0 + 2 * i + (lane >> 4);
-              const int own = r >> 2;
-              const int64_t x0 = __shfl_sync(0xffffffffu, sl[0], own), x1 = __shfl_sync(0xffffffffu, sl[1], own);
-              const int64_t x2 = __shfl_sync(0xffffffffu, sl[2], own), x3 = __shfl_sync(0xffffffffu, sl[3], own);
-              const int64_t s = (r & 2) ? ((r & 1) ? x3 : x2) : ((r & 1) ? x1 : x0);
-              val[i] = make_uint4(0, 0, 0, 0);
-              if (s >= 0)
-                val[i] = __ldg(reinterpret_cast<const uint4*>(cache + (s * a.Hkv + t.hkv) * (int64_t)row_bytes) + (lane & 15));
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int r = r0 + 2 * i + (lane >> 4), c = lane & 15;
-              *reinterpret_cast<uint4*>(tile + (c >> 3) * kChunkBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = val[i];
-            }
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
+          for (int i = 0; i < 4; ++i) r[i] = sl[i] >= 0 ? sl[i] : (int)a.num_slots;
+          tma_gather4(dst + 4 * lane * 128, mgather, fb, t.hkv * kD, r);
+          tma_gather4(dst + kChunkBytes + 4 * lane * 128, mgather, fb, t.hkv * kD + 64, r);
+        }
+        if (clear) {
+          ok = mbar_wait_warp(fb, land & 1, abort_flag);
+          if (!ok) break;
+          ++land;
+          clear_tail(tile, kt.valid, lane);
           if (lane == 0) mbar_arrive(bar(bfull + st));
         }
         }
@@ -883,8 +867,7 @@ __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
 }
 
 template <int kFmt>
-cudaError_t launch(const CUtensorMap& tmK, const CUtensorMap& tmV, const CUtensorMap& tmKc, const CUtensorMap& tmVc,
-                   const ChunkArgs& a, int num_sms, cudaStream_t stream) {
+cudaError_t launch(const ChunkMaps& m, const ChunkArgs& a, int num_sms, cudaStream_t stream) {
   static std::atomic<bool> attr_set[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -896,18 +879,17 @@ cudaError_t launch(const CUtensorMap& tmK, const CUtensorMap& tmV, const CUtenso
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
   return launch_pdl(attn_chunk_mma_kernel<kFmt>, dim3(std::min(a.total_units, num_sms)), dim3(Layout<kFmt>::kThreads),
-                    Layout<kFmt>::kSmemBytes, stream, tmK, tmV, tmKc, tmVc, a);
+                    Layout<kFmt>::kSmemBytes, stream, m.k, m.v, m.kc, m.vc, m.kg, m.vg, a);
 }
 
 }  // namespace chunk128
 
-cudaError_t launch_attn_chunk_mma(const CUtensorMap& tmK, const CUtensorMap& tmV, const CUtensorMap& tmKc,
-                                  const CUtensorMap& tmVc, const ChunkArgs& a, int format, int num_sms,
+cudaError_t launch_attn_chunk_mma(const ChunkMaps& maps, const ChunkArgs& a, int format, int num_sms,
                                   cudaStream_t stream) {
   switch (format) {
-    case kFmtBf16: return chunk128::launch<kFmtBf16>(tmK, tmV, tmKc, tmVc, a, num_sms, stream);
-    case kFmtE4m3: return chunk128::launch<kFmtE4m3>(tmK, tmV, tmKc, tmVc, a, num_sms, stream);
-    default: return chunk128::launch<kFmtInt8>(tmK, tmV, tmKc, tmVc, a, num_sms, stream);
+    case kFmtBf16: return chunk128::launch<kFmtBf16>(maps, a, num_sms, stream);
+    case kFmtE4m3: return chunk128::launch<kFmtE4m3>(maps, a, num_sms, stream);
+    default: return chunk128::launch<kFmtInt8>(maps, a, num_sms, stream);
   }
 }
 

@@ -108,6 +108,24 @@ int encode_codes_map(CUtensorMap* m, const void* ptr, int64_t slots, int heads) 
   return DLLM_OK;
 }
 
+// 2-D map over a cache as a matrix of slots, `row` elements each (bf16 or one
+// byte): box of one row of 128 bytes, swizzled like encode_rows_map's (bf16) or
+// not (codes), for gathers of single rows.
+int encode_gather_map(CUtensorMap* m, const void* ptr, int64_t slots, int64_t row, bool bf16) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (enc == nullptr) return fail(DLLM_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[2] = {(cuuint64_t)row, (cuuint64_t)slots};
+  cuuint64_t strides[1] = {(cuuint64_t)row * (bf16 ? 2 : 1)};
+  cuuint32_t box[2] = {bf16 ? 64u : 128u, 1};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr),
+                   dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   bf16 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(DLLM_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return DLLM_OK;
+}
+
 // 2-D map over a row-major bf16 matrix [rows, cols] (row stride in elements):
 // box (64 columns, box_rows rows), 128-byte swizzle (UMMA SW128 K-major).
 int encode_matrix_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t cols, int64_t row_stride,
@@ -543,6 +561,11 @@ int dllm_attn_chunk_fwd(const void* q, int64_t q_tok_stride, const void* k, int6
         rc = format == DLLM_KV_BF16 ? encode_rows_map(m, p, num_slots, num_kv_heads, row, 128)
                                     : encode_codes_map(m, p, num_slots, num_kv_heads);
         if (rc != DLLM_OK) return rc;
+        // tiles that are no run of slots: from a slot list, or from blocks smaller than a tile
+        if (slots != nullptr || block_size % 128 != 0) {
+          rc = encode_gather_map(i == 0 ? &maps.kg : &maps.vg, p, num_slots, row, format == DLLM_KV_BF16);
+          if (rc != DLLM_OK) return rc;
+        }
       }
     }
   }

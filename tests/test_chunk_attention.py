@@ -304,48 +304,51 @@ def test_value_sizes_far_apart(dev, fmt, step):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("fmt", ["bf16", "int8"])
-def test_bad_pages_and_lengths(dev, fmt):
+@pytest.mark.parametrize("fmt", ["bf16", "int8", "e4m3"])
+@pytest.mark.parametrize("nq,page", [([1, 2], 16), ([20, 33], 16), ([20, 33], 128)])
+def test_bad_pages_and_lengths(dev, fmt, nq, page):
     """Pages outside the cache read as zero rows and are flagged; lengths past
     their bounds are cut and flagged. Nothing outside the buffers is touched."""
     ops = _ops()
-    c = Case(41, fmt, 4, 4, [1, 2], [40, 33], None, True)
+    n = sum(nq)
+    nc = [2 * page + 8, page + 30]
+    c = Case(41, fmt, 4, 4, nq, nc, None, True, page=page)
     args, kw = c.args(dev)
     for bad in (10 ** 6, -3, 2 ** 31 - 1):
         tables = kw["block_tables"].clone()
-        page = int(tables[0, 1])
+        at = int(tables[0, 1])
         tables[0, 1] = bad
         out = ops.chunk_attention(*args, **{**kw, "block_tables": tables})
         assert ops.read_device_status(dev) == 1
         saved = [x.clone() for x in c.values]
         for x in c.values:
-            x[page * 16:page * 16 + 16] = 0
+            x[at * page:at * page + page] = 0
         c.check(out, True)
         c.values = saved
     # a context longer than its table row
-    ctx = torch.tensor([40, 10 ** 6], dtype=torch.int32, device=dev)
+    ctx = torch.tensor([nc[0], 10 ** 6], dtype=torch.int32, device=dev)
     out = ops.chunk_attention(*args, **{**kw, "context_lens": ctx})
     assert ops.read_device_status(dev) in (1, 3)
     c.check(out, True, seqs=[0])
-    ctx = torch.tensor([40, -5], dtype=torch.int32, device=dev)
+    ctx = torch.tensor([nc[0], -5], dtype=torch.int32, device=dev)
     out = ops.chunk_attention(*args, **{**kw, "context_lens": ctx})
     assert ops.read_device_status(dev) == 3
-    assert (out[1:3] == 0).all()
+    assert (out[nq[0]:n] == 0).all()
     # a chunk longer than max_seqlen_q: the rows past it are not computed
     out = torch.full_like(args[0], 5.0)
-    ops.chunk_attention(*args[:4], 1, out=out, **kw)
+    ops.chunk_attention(*args[:4], nq[0], out=out, **kw)
     assert ops.read_device_status(dev) == 3
-    assert (out[2:] == 5).all()
+    assert (out[2 * nq[0]:] == 5).all()
     # slots outside the cache
-    c = Case(42, fmt, 4, 4, [1, 2], [40, 33], None, False)
+    c = Case(42, fmt, 4, 4, nq, nc, None, False, page=page)
     args, kw = c.args(dev)
     slots = kw["slots"].clone()
-    slots[3], slots[50] = 10 ** 8, -1
+    slots[3], slots[nc[0] + 10] = 10 ** 8, -1
     out = ops.chunk_attention(*args, **{**kw, "slots": slots})
     assert ops.read_device_status(dev) == 1
     for x in c.values:
         x[c.slots[3].long()] = 0
-        x[c.slots[50].long()] = 0
+        x[c.slots[nc[0] + 10].long()] = 0
     c.check(out, True)
 
 
