@@ -572,8 +572,11 @@ __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
       const uint8_t* src = smem + S::kOffRaw + rb * kChunkBytes;
       const uint8_t* ex = smem + S::kOffExp + rb * 128;
       uint8_t* dst = smem + ring + st * kTileBytes;
-      const int un = tid & 7;  // 16 codes: 16-byte units 2 un, 2 un + 1 of the row's bf16 form
-      const int r0 = tid >> 3;
+      // This thread's 16 codes are unit `un` of rows r0 + 16 i; their bf16 form is 16-byte units
+      // 2 un, 2 un + 1 of the row (half un / 4 of the tile). Neighbouring rows change places for the
+      // upper units: eight lanes then read eight different units and write eight different banks.
+      const int un = tid & 7;
+      const int r0 = (tid >> 3) ^ (un >> 2);
       uint32_t e[8];
       bool big = false;
 #pragma unroll
@@ -581,16 +584,12 @@ __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
         e[i] = ex[i * 16 + r0];
         big |= exp_is_big<kFmt>(e[i]);
       }
-      // row i * 16 + r0 has the parity and swizzle of r0. The two halves of a row alternate so that
-      // eight lanes write eight different banks.
-      const bool odd = un >> 2;
       const int x = (2 * un) & 7;
-      uint8_t* d0 = dst + (un >> 2) * kChunkBytes + r0 * 128 + (((odd ? x + 1 : x) ^ (r0 & 7)) << 4);
-      uint8_t* d1 = dst + (un >> 2) * kChunkBytes + r0 * 128 + (((odd ? x : x + 1) ^ (r0 & 7)) << 4);
+      uint8_t* d0 = dst + (un >> 2) * kChunkBytes + r0 * 128 + ((x ^ (r0 & 7)) << 4);
+      uint8_t* d1 = dst + (un >> 2) * kChunkBytes + r0 * 128 + (((x + 1) ^ (r0 & 7)) << 4);
       auto put = [&](int i, const uint32_t (&w)[8]) {
-        const uint4 lo = make_uint4(w[0], w[1], w[2], w[3]), hi = make_uint4(w[4], w[5], w[6], w[7]);
-        *reinterpret_cast<uint4*>(d0 + i * 2048) = odd ? hi : lo;
-        *reinterpret_cast<uint4*>(d1 + i * 2048) = odd ? lo : hi;
+        *reinterpret_cast<uint4*>(d0 + i * 2048) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4*>(d1 + i * 2048) = make_uint4(w[4], w[5], w[6], w[7]);
       };
       src += r0 * kD + un * 16;
       if (!__any_sync(0xffffffffu, big)) {
@@ -715,6 +714,9 @@ __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
       if (!t.valid) continue;
       const int qr = (t.row0 + row_in_tile) / a.group;  // row of the chunk
       const int seen = (int)(a.causal ? min(t.L, max((int64_t)0, t.L - t.sq.Lq + qr + 1)) : t.L);
+      // A warp whose 32 rows lie past the unit's last one only keeps the barriers going (its rows
+      // of P hold anything: rows of a product do not mix).
+      const bool idle = wq * 32 >= t.rows;
       float m = -INFINITY;  // running max (log2 units), -inf until a visible key
       float l = 0.f;
       for (int j = 0; j < t.nkv; ++j, ++g) {
@@ -724,7 +726,7 @@ __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
         if (!ok) break;
         tc_fence_after();
         const uint32_t tS = tmem + lane_base + sb * 128 + wg * kHalfN;
-        if (kt.valid > wg * kHalfN) {
+        if (!idle && kt.valid > wg * kHalfN) {
           uint32_t s[2][32];
           tmem_ld32(tS, s[0]);
           tmem_ld32(tS + 32, s[1]);
@@ -822,6 +824,7 @@ __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
         ++o_it;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
+          if (idle) break;
           uint32_t oa[32], ob[32];
           tmem_ld32(tOa + wg * kHalfN + c * 32, oa);
           tmem_ld32(tOb + wg * kHalfN + c * 32, ob);
