@@ -724,6 +724,45 @@ __global__ void __launch_bounds__(256) attn_chunk_merge_kernel(const __grid_cons
   *reinterpret_cast<uint2*>(a.o + (sq.q_begin + r) * a.o_stride + (int64_t)h * kD + lane * 4) = out;
 }
 
+// The cached rows of every sequence as bf16 rows, one after another: 16 codes
+// of K and of V per thread, items (position, head, unit) of a sequence in
+// order along x, sequences along y.
+template <int kFmt>
+__global__ void __launch_bounds__(256) expand_rows_kernel(const __grid_constant__ ChunkArgs a, uint4* k_out, uint4* v_out) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const int b = blockIdx.y;
+  const Seq sq = load_seq(a, b, false);
+  const int per_row = a.Hkv * 8;
+  const int64_t first = (int64_t)blockIdx.x * 256;
+  const int p0 = (int)(first / per_row);
+  const uint32_t at = (uint32_t)(first - (int64_t)p0 * per_row) + threadIdx.x;
+  const int pos = p0 + (int)(at / (uint32_t)per_row);
+  if (pos >= sq.nc) return;
+  const int item = (int)(at % (uint32_t)per_row);
+  int64_t slot;
+  if (a.tables != nullptr) {
+    const int blk = a.block_shift >= 0 ? pos >> a.block_shift : pos / a.block_size;
+    const int e = blk < a.max_blocks ? a.tables[b * a.table_stride + blk] : -1;
+    slot = e < 0 ? -1 : (int64_t)e * a.block_size + (pos - blk * a.block_size);
+  } else {
+    slot = a.slots[sq.s_begin + pos];
+  }
+  uint32_t k[8] = {}, v[8] = {};
+  if (slot >= 0 && slot < a.num_slots) {
+    const int64_t code = slot * per_row + item, ex = slot * a.Hkv + (item >> 3);
+    dequantise16<kFmt>(__ldg(reinterpret_cast<const uint4*>(a.kc) + code), a.k_exp[ex], k);
+    dequantise16<kFmt>(__ldg(reinterpret_cast<const uint4*>(a.vc) + code), a.v_exp[ex], v);
+  } else if (item == 0) {
+    set_error(a.err, kDevSlotOutOfRange);
+  }
+  const int64_t o = (((int64_t)b * a.dense + pos) * per_row + item) * 2;
+  k_out[o] = make_uint4(k[0], k[1], k[2], k[3]);
+  k_out[o + 1] = make_uint4(k[4], k[5], k[6], k[7]);
+  v_out[o] = make_uint4(v[0], v[1], v[2], v[3]);
+  v_out[o + 1] = make_uint4(v[4], v[5], v[6], v[7]);
+}
+
 template <int kFmt, int kMT, int kR>
 cudaError_t launch(const ChunkArgs& a, cudaStream_t stream) {
   static std::atomic<bool> attr_set[64];
@@ -755,7 +794,8 @@ cudaError_t launch_rows(const ChunkArgs& a, int rows, cudaStream_t stream) {
 
 ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int max_context, int max_fresh,
                           int num_sms) {
-  ChunkPlan p;
+  constexpr int kDenseTiles = 4;
+  ChunkPlan p = {};
   const int64_t rows = (int64_t)max_q * group;
   p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : kChunkMmaRows;
   if (p.rows == kChunkMmaRows) {
@@ -768,6 +808,17 @@ ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int 
     p.split_chunks = (int)std::max<int64_t>(1, (tiles + splits - 1) / splits);
     p.splits = (int)std::max<int64_t>(1, (tiles + p.split_chunks - 1) / p.split_chunks);
     p.workspace_bytes = p.splits > 1 ? units * p.splits * p.rows * (chunk::kD * 4 + 8) : 0;
+    // Every row tile of a (sequence, KV head) expands the quantised rows it reads. From four row
+    // tiles on they are expanded once instead, into bf16 rows that all tiles read, unless that
+    // copy would be larger than 1 GiB.
+    const int64_t cap = ((int64_t)max_context + 127) / 128 * 128;
+    const int64_t bytes = 2 * (int64_t)B * cap * Hkv * chunk::kD * 2;
+    if (format != kFmtBf16 && p.mtiles >= kDenseTiles && bytes > 0 && bytes <= ((int64_t)1 << 30) &&
+        (int64_t)B * cap < ((int64_t)1 << 31) && B < 65536) {
+      p.dense = (int)cap;
+      p.dense_bytes = bytes;
+      p.workspace_bytes += bytes;
+    }
     return p;
   }
   p.mtiles = (int)((rows + p.rows - 1) / p.rows);
@@ -790,19 +841,35 @@ ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int 
   return p;
 }
 
+cudaError_t launch_expand_rows(const ChunkArgs& a, int format, void* k_out, void* v_out, cudaStream_t stream) {
+  const int64_t items = (int64_t)a.max_context * a.Hkv * 8;
+  const dim3 grid((unsigned)((items + 255) / 256), (unsigned)a.B);
+  return format == kFmtE4m3
+             ? launch_pdl(chunk::expand_rows_kernel<kFmtE4m3>, grid, dim3(256), 0, stream, a, (uint4*)k_out, (uint4*)v_out)
+             : launch_pdl(chunk::expand_rows_kernel<kFmtInt8>, grid, dim3(256), 0, stream, a, (uint4*)k_out, (uint4*)v_out);
+}
+
 cudaError_t launch_attn_chunk(ChunkArgs a, int format, const ChunkPlan& plan, const ChunkMaps& maps, void* workspace,
                               int num_sms, cudaStream_t stream) {
   a.mtiles = plan.mtiles;
   a.splits = plan.splits;
   a.split_chunks = plan.split_chunks;
   const int64_t rows = (int64_t)a.B * a.Hkv * a.mtiles * a.splits * plan.rows;
-  a.part_o = reinterpret_cast<float*>(workspace);
+  a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.dense_bytes);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * chunk::kD);
   if (plan.rows == kChunkMmaRows) {
     const int64_t items = (int64_t)a.B * a.Hkv * a.mtiles;
     if (items * a.splits > 0x7fffffffLL) return cudaErrorInvalidValue;
     a.total_units = (int)(items * a.splits);
-    cudaError_t e = launch_attn_chunk_mma(maps, a, format, num_sms, stream);
+    a.dense = plan.dense;
+    cudaError_t e = cudaSuccess;
+    if (plan.dense > 0) {
+      e = launch_expand_rows(a, format, workspace, static_cast<uint8_t*>(workspace) + plan.dense_bytes / 2, stream);
+      if (e != cudaSuccess) return e;
+      a.num_slots = (int64_t)a.B * plan.dense;
+      format = kFmtBf16;
+    }
+    e = launch_attn_chunk_mma(maps, a, format, num_sms, stream);
     if (e != cudaSuccess || a.splits == 1) return e;
     return launch_pdl(chunk::attn_chunk_merge_kernel<128, 128, kChunkMmaRows>,
                       dim3((unsigned)(items * (kChunkMmaRows / 8))), dim3(256), 0, stream, a);

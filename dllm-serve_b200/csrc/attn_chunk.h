@@ -46,6 +46,9 @@ struct ChunkArgs {
   __nv_bfloat16* o;
   int64_t o_stride;
   int32_t* err;
+  // Dense cached rows (128-row launches): the cached rows of sequence b are rows b * dense +
+  // position of kc / vc (bf16), as expand_rows() laid them out. 0: by table or slot list.
+  int dense;
   // set by the launcher
   int mtiles;              // row tiles per (sequence, KV head)
   int splits;              // key splits per row tile
@@ -63,6 +66,8 @@ struct ChunkPlan {
   int mtiles;
   int splits;
   int split_chunks;
+  int dense;               // rows per sequence of the expanded copy of a quantised cache's rows, 0: none
+  int64_t dense_bytes;     // its bytes (K, then V), at the workspace's start
   int64_t workspace_bytes;
 };
 
@@ -79,6 +84,10 @@ struct ChunkMaps {
 // maps: read only by 128-row launches.
 cudaError_t launch_attn_chunk(ChunkArgs a, int format, const ChunkPlan& plan, const ChunkMaps& maps, void* workspace,
                               int num_sms, cudaStream_t stream);
+
+// Expands the cached rows of every sequence to bf16: rows b * dense + position of
+// k_out, v_out [B * dense, Hkv, 128].
+cudaError_t launch_expand_rows(const ChunkArgs& a, int format, void* k_out, void* v_out, cudaStream_t stream);
 
 cudaError_t launch_attn_chunk_mma(const ChunkMaps& maps, const ChunkArgs& a, int format, int num_sms,
                                   cudaStream_t stream);

@@ -333,7 +333,11 @@ __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
         int sl[4], s0 = 0;
         bool contig = true;
         if (!kt.fresh) {
-          if (table != nullptr && a.block_size % kTileN == 0) {
+          if (!kQuant && a.dense > 0) {
+            s0 = t.b * a.dense + kt.pos;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sl[i] = s0 + 4 * lane + i;
+          } else if (table != nullptr && a.block_size % kTileN == 0) {
             // the tile lies inside one block
             const int blk = kt.pos / a.block_size;
             const int e = blk < a.max_blocks ? table[blk] : -1;

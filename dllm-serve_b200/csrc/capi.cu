@@ -553,8 +553,14 @@ int dllm_attn_chunk_fwd(const void* q, int64_t q_tok_stride, const void* k, int6
       if ((rc = encode_rows_map(&maps.k, k, total_k, num_kv_heads, k_tok_stride, 128)) != DLLM_OK) return rc;
       if ((rc = encode_rows_map(&maps.v, v, total_k, num_kv_heads, v_tok_stride, 128)) != DLLM_OK) return rc;
     }
-    if (cached && num_slots > 0) {
-      const int64_t row = (int64_t)num_kv_heads * 128;
+    const int64_t row = (int64_t)num_kv_heads * 128;
+    if (plan.dense > 0) {
+      // the expanded copy, K rows then V rows
+      const int64_t rows = (int64_t)batch * plan.dense;
+      const uint8_t* ws = static_cast<const uint8_t*>(workspace);
+      if ((rc = encode_rows_map(&maps.kc, ws, rows, num_kv_heads, row, 128)) != DLLM_OK) return rc;
+      if ((rc = encode_rows_map(&maps.vc, ws + plan.dense_bytes / 2, rows, num_kv_heads, row, 128)) != DLLM_OK) return rc;
+    } else if (cached && num_slots > 0) {
       for (int i = 0; i < 2; ++i) {
         CUtensorMap* m = i == 0 ? &maps.kc : &maps.vc;
         const void* p = i == 0 ? k_cache : v_cache;
