@@ -677,10 +677,10 @@ __global__ void __launch_bounds__(256) attn_chunk_merge_kernel(const __grid_cons
   const int mtile = (int)(item % a.mtiles);
   const int hkv = (int)(item / a.mtiles % a.Hkv), b = (int)(item / a.mtiles / a.Hkv);
   const Seq sq = load_seq(a, b, false);
-  const int row0 = mtile * kRows;
-  const int rows = sq.Lq * a.group - row0;
+  const int row0 = mtile * a.tile_rows;
+  const int rows = min(sq.Lq * a.group - row0, a.tile_rows);
   if (row >= rows) return;
-  const Span sp = tile_span<KB, FB>(a, sq, (row0 + min(rows, kRows) - 1) / a.group);
+  const Span sp = tile_span<KB, FB>(a, sq, (row0 + rows - 1) / a.group);
   if (sp.total <= a.split_chunks) return;  // written by its only split
   const int n = (sp.total + a.split_chunks - 1) / a.split_chunks;
   const int64_t at = item * a.splits * kRows + row;
@@ -801,9 +801,10 @@ ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int 
   if (p.rows == kChunkMmaRows) {
     // One CTA per SM. Splits only while SMs would have nothing to do, and four
     // tiles of keys at least for each.
-    p.mtiles = (int)((rows + kChunkMmaRows - 1) / kChunkMmaRows);
+    p.tile_rows = p.unit_rows = kChunkMmaRows / group * group;  // whole chunk rows
+    p.mtiles = (int)((rows + p.tile_rows - 1) / p.tile_rows);
     const int64_t tiles = ((int64_t)max_context + 127) / 128 + ((int64_t)max_fresh + 127) / 128;
-    const int64_t units = (int64_t)B * Hkv * p.mtiles;
+    int64_t units = (int64_t)B * Hkv * p.mtiles;
     const int64_t splits = std::max<int64_t>(1, std::min(units > 0 ? num_sms / units : 1, tiles / 4));
     p.split_chunks = (int)std::max<int64_t>(1, (tiles + splits - 1) / splits);
     p.splits = (int)std::max<int64_t>(1, (tiles + p.split_chunks - 1) / p.split_chunks);
@@ -819,8 +820,15 @@ ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int 
       p.dense_bytes = bytes;
       p.workspace_bytes += bytes;
     }
+    // Two row tiles per unit where every SM still has one.
+    const int64_t pairs = (rows + 2 * p.tile_rows - 1) / (2 * p.tile_rows);
+    if ((format == kFmtBf16 || p.dense > 0) && p.mtiles >= 2 && (int64_t)B * Hkv * pairs >= num_sms) {
+      p.unit_rows = 2 * p.tile_rows;
+      p.mtiles = (int)pairs;
+    }
     return p;
   }
+  p.tile_rows = p.unit_rows = p.rows;
   p.mtiles = (int)((rows + p.rows - 1) / p.rows);
   const int kb = format == kFmtBf16 ? 16 : 32;
   const int64_t chunks = ((int64_t)max_context + kb - 1) / kb + ((int64_t)max_fresh + 15) / 16;
@@ -851,6 +859,8 @@ cudaError_t launch_expand_rows(const ChunkArgs& a, int format, void* k_out, void
 
 cudaError_t launch_attn_chunk(ChunkArgs a, int format, const ChunkPlan& plan, const ChunkMaps& maps, void* workspace,
                               int num_sms, cudaStream_t stream) {
+  a.tile_rows = plan.tile_rows;
+  a.unit_rows = plan.unit_rows;
   a.mtiles = plan.mtiles;
   a.splits = plan.splits;
   a.split_chunks = plan.split_chunks;

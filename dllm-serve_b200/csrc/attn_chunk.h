@@ -50,7 +50,9 @@ struct ChunkArgs {
   // position of kc / vc (bf16), as expand_rows() laid them out. 0: by table or slot list.
   int dense;
   // set by the launcher
-  int mtiles;              // row tiles per (sequence, KV head)
+  int tile_rows;           // packed rows of a tile that are used
+  int unit_rows;           // packed rows of a work unit: one or two (128-row launches) tiles
+  int mtiles;              // work units per (sequence, KV head)
   int splits;              // key splits per row tile
   int split_chunks;        // key chunks of a split
   int total_units;         // items * splits
@@ -63,6 +65,7 @@ constexpr int kChunkMmaRows = 128;  // packed rows of a tile of the tcgen05 kern
 // How a launch is laid out, from sizes the host knows.
 struct ChunkPlan {
   int rows;                // packed rows of a tile: 8 or 16 (attn_chunk.cu), 128 (attn_chunk_mma.cu)
+  int tile_rows, unit_rows;
   int mtiles;
   int splits;
   int split_chunks;
@@ -74,11 +77,12 @@ struct ChunkPlan {
 ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int max_context, int max_fresh,
                           int num_sms);
 
-// Tensor maps of a 128-row launch: fresh k / v (bf16 boxes of 64 x 1 x 128, 128-byte
+// Tensor maps of a 128-row launch: q (boxes of 64 dimensions, a KV head's group of heads, as
+// many rows as fit 128); fresh k / v (bf16 boxes of 64 x 1 x 128, 128-byte
 // swizzle); caches (the same, or 8-bit boxes of 128 x 1 x 128, no swizzle); caches as
 // [slots, Hkv * 128] matrices with boxes of one 128-byte row, for scattered slots.
 struct ChunkMaps {
-  CUtensorMap k, v, kc, vc, kg, vg;
+  CUtensorMap q, k, v, kc, vc, kg, vg;
 };
 
 // maps: read only by 128-row launches.

@@ -2,14 +2,21 @@
 // more than 16 query rows per KV head (diffusion blocks, prefill chunks):
 // tcgen05 + TMEM + TMA, sm_100a.
 //
-// A work unit is (sequence b, KV head, tile of 128 packed rows, split of the
-// keys); packed row p of a (sequence, KV head) is row p / group of the chunk
-// for head p % group of the KV head's group, so grouped heads share every key
-// tile they read. Keys come in tiles of 128: the sequence's cached rows, then
-// its fresh rows, cut at the last key that a row of the unit sees. Each KV
-// tile's 128 columns are split between two softmax warpgroups, each with its
-// own running maximum, sum and accumulator, merged once per unit (exact:
-// softmax of a union). Probabilities are rounded to bf16 (2^-8 of their value).
+// A work unit is (sequence b, KV head, one or two tiles of packed rows, split
+// of the keys); packed row p of a (sequence, KV head) is row p / group of the
+// chunk for head p % group of the KV head's group, so grouped heads share every
+// key tile they read. A row tile holds as many whole chunk rows as fit 128
+// packed rows (all 128 where the group divides them). Keys come in tiles of
+// 128: the sequence's cached rows, then its fresh rows, cut at the last key
+// that a row of the unit sees. Probabilities are rounded to bf16 (2^-8 of
+// their value).
+//
+// One row tile ("single"): each KV tile's 128 columns are split between two
+// softmax warpgroups, each with its own running maximum, sum and accumulator,
+// merged once per unit (exact: softmax of a union). Two row tiles ("pair",
+// bf16 rows, launches with at least one such unit per SM): a warpgroup per row
+// tile, and every key tile read from L2 serves both: the single form needs 64
+// KB per 2,290 cycles and SM, close to what L2 delivers.
 //
 // Quantised caches: 8-bit rows are brought into shared memory as they are
 // (TMA boxes, or four rows at a time where the slots are scattered) and two more
@@ -18,19 +25,20 @@
 // nothing, and the rest of the kernel is the same for every format. HBM and
 // L2 carry one byte per element.
 //
-// Roles (16 warps, 20 with a quantised cache):
-//   warps 0-3, 4-7  softmax warpgroups: columns 0-63 / 64-127 of every tile
+// Roles (12 warps, 20 with a quantised cache):
+//   warps 0-3, 4-7  softmax warpgroups
 //   warp 8          loader of K: bf16 stages, or the raw K ring of a quantised cache
 //   warp 9          issues the MMAs, owns TMEM
 //   warp 10         loader of V
-//   warps 12-15     bf16: stage Q. Quantised: fill the K ring (expand cached
-//                   tiles, load fresh ones)
-//   warps 16-19     quantised: stage Q, fill the V ring
+//   warp 11         loader of Q
+//   warps 12-15     quantised: fill the K ring (expand cached tiles, load fresh ones)
+//   warps 16-19     quantised: fill the V ring
 // One warpgroup for both rings was the bottleneck: 1,560 cycles to expand a
 // tile of K or V, 4,270 per KV tile against 2,290 of the bf16 kernel.
-// TMEM (512 columns): S buffers [0,128) [128,256), O of each warpgroup at 256
-// and 384; P (bf16) over the first 32 columns of its half of S. MMA order per
-// tile j: PV(j) of both halves, then QK(j+2).
+// TMEM (512 columns): S buffers [0,128) [128,256), accumulators at 256 and 384;
+// P (bf16) over the first columns of S (pair) or of each half of it (single).
+// MMA order per KV tile j: single PV(j) of both halves, then QK(j+2); pair, for
+// each row tile, PV(j), then QK(j+1).
 #include <algorithm>
 #include <atomic>
 #include <cuda.h>
@@ -56,20 +64,21 @@ constexpr uint32_t kTileBytes = 128 * kD * 2;  // bf16 tile
 constexpr uint32_t kChunkBytes = 128 * 128;    // its 64-column half; also an 8-bit tile
 constexpr int kRaw = 2;                        // stages of each raw ring
 
-template <int kFmt>
+template <int kFmt, bool kPair>
 struct Layout {
   static constexpr bool kQuant = kFmt != kFmtBf16;
   // Registers: the softmax warpgroups take those that the other roles do not need.
-  // bf16: 512 x 128 = 256 x 168 + 256 x 88; quantised: 640 x 96 = 256 x 144 + 384 x 64.
-  static constexpr int kThreads = kQuant ? 640 : 512;
-  static constexpr int kRegsSoftmax = kQuant ? 144 : 168;
+  // bf16: 384 x 168 = 256 x 208 + 128 x 88; quantised: 640 x 96 = 256 x 144 + 384 x 64.
+  static constexpr int kThreads = kQuant ? 640 : 384;
+  static constexpr int kRegsSoftmax = kQuant ? 144 : 208;
   static constexpr int kRegsOther = kQuant ? 64 : 88;
+  static constexpr int kTilesQ = kPair ? 2 : 1;
   static constexpr int kStagesK = kQuant ? 2 : 3;
-  static constexpr int kStagesV = kQuant ? 2 : 3;
+  static constexpr int kStagesV = kQuant || kPair ? 2 : 3;
   // arrivals that complete a bf16 stage: the four expanding warps, or the loader's
   static constexpr int kFull = kQuant ? 4 : 1;
   static constexpr uint32_t kOffQ = 0;
-  static constexpr uint32_t kOffK = kOffQ + kTileBytes;
+  static constexpr uint32_t kOffK = kOffQ + kTilesQ * kTileBytes;
   static constexpr uint32_t kOffV = kOffK + kStagesK * kTileBytes;
   static constexpr uint32_t kOffRaw = kOffV + kStagesV * kTileBytes;  // K ring, V ring
   static constexpr uint32_t kOffExp = kOffRaw + (kQuant ? 2 * kRaw * kChunkBytes : 0);  // exponent bytes of each raw stage
@@ -82,9 +91,9 @@ struct Layout {
   static constexpr int BAR_VEMPTY = BAR_VFULL + kStagesV;
   static constexpr int BAR_SFULL = BAR_VEMPTY + kStagesV;  // 2: S buffer holds QK of a tile
   static constexpr int BAR_PFULL = BAR_SFULL + 2;          // 2: both P halves written
-  static constexpr int BAR_OREADY = BAR_PFULL + 2;         // PVs of one more tile completed
-  static constexpr int BAR_OFULL = BAR_OREADY + 1;         // a unit's last PVs completed
-  static constexpr int BAR_XML = BAR_OFULL + 1;            // warpgroup 1's (max, sum) published
+  static constexpr int BAR_OREADY = BAR_PFULL + 2;         // single: PVs of one more tile completed
+  static constexpr int BAR_OFULL = BAR_OREADY + 1;         // 2: a unit's last PVs (of a row tile) completed
+  static constexpr int BAR_XML = BAR_OFULL + 2;            // warpgroup 1's (max, sum) published
   static constexpr int BAR_XF = BAR_XML + 1;               // the merge factors published
   static constexpr int BAR_DRAIN = BAR_XF + 1;
   static constexpr int BAR_VLAND = BAR_DRAIN + 1;          // a partial V tile landed
@@ -100,7 +109,7 @@ struct Layout {
 struct Unit {
   bool valid;
   int b, hkv, item, split;
-  int row0, rows;      // first packed row of the tile; packed rows from there on
+  int row0, rows;      // first packed row, number of packed rows (at most a.unit_rows)
   Seq sq;
   Span sp;             // tiles of the whole row tile
   int t0, nkv;         // this split's tiles
@@ -119,15 +128,15 @@ DLLM_DEVICE Unit decode_unit(int u, const ChunkArgs& a, bool report) {
   r.b = bh / a.Hkv;
   r.hkv = bh - r.b * a.Hkv;
   r.item = bh * a.mtiles + mt;
-  r.row0 = mt * kTileM;
+  r.row0 = mt * a.unit_rows;
   r.sq = load_seq(a, r.b, report && r.hkv == 0 && mt == 0 && r.split == 0);
-  r.rows = r.sq.Lq * a.group - r.row0;
+  r.rows = min(r.sq.Lq * a.group - r.row0, a.unit_rows);
   r.L = (int64_t)r.sq.nc + r.sq.nk;
   r.valid = r.rows > 0;
   r.t0 = r.nkv = 0;
   r.sp = Span{};
   if (!r.valid) return r;
-  r.sp = tile_span<kTileN, kTileN>(a, r.sq, (r.row0 + min(r.rows, kTileM) - 1) / a.group);
+  r.sp = tile_span<kTileN, kTileN>(a, r.sq, (r.row0 + r.rows - 1) / a.group);
   r.t0 = r.split * a.split_chunks;
   r.nkv = min(r.sp.total, r.t0 + a.split_chunks) - r.t0;
   if (r.split > 0 && r.nkv <= 0) r.valid = false;  // split 0 writes rows without keys
@@ -235,15 +244,159 @@ DLLM_DEVICE float exp_store_half(const uint32_t (&s)[2][32], float sl2, float m,
   return (acc[0] + acc[1]) + (acc[2] + acc[3]);
 }
 
+// The same for a whole tile's 128 columns, over the S buffer's first 64.
+DLLM_DEVICE float exp_store_tile(const uint32_t (&s)[4][32], float sl2, float m, uint32_t tS) {
+  const float neg_m = -m;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t pk[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float p0 = ex2_approx(fmaf(__uint_as_float(s[c][2 * e]), sl2, neg_m));
+      const float p1 = ex2_approx(fmaf(__uint_as_float(s[c][2 * e + 1]), sl2, neg_m));
+      acc[(2 * e) & 3] += p0;
+      acc[(2 * e + 1) & 3] += p1;
+      pk[e] = pack_bf16x2(p0, p1);
+    }
+    tmem_st16(tS + c * 16, pk);
+  }
+  return (acc[0] + acc[1]) + (acc[2] + acc[3]);
+}
+
 }  // namespace
 
-template <int kFmt>
-__global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
-    attn_chunk_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                          const __grid_constant__ CUtensorMap tmKc, const __grid_constant__ CUtensorMap tmVc,
+// Softmax warpgroup w of a pair launch: row tile w of every unit, KV tile by KV
+// tile. PV(j-1) was issued before QK(j), so when S(j) is there the accumulator
+// holds every earlier tile and may be rescaled.
+template <typename S>
+DLLM_DEVICE void softmax_pair(const ChunkArgs& a, uint32_t tmem, uint32_t bar0, volatile int* abort_flag) {
+  auto bar = [&](int i) -> uint32_t { return bar0 + 8u * (uint32_t)i; };
+  const int lane = threadIdx.x & 31;
+  const int wg = threadIdx.x >> 7, wq = (threadIdx.x >> 5) & 3;
+  const uint32_t lane_base = (uint32_t)(wq * 32) << 16;
+  const uint32_t tS = tmem + lane_base + wg * 128;
+  const uint32_t tO = tmem + lane_base + 256 + wg * 128;
+  const float sl2 = a.scale_log2;
+  uint32_t s_it = 0, o_it = 0;
+  for (int u = blockIdx.x; u < a.total_units; u += gridDim.x) {
+    const Unit t = decode_unit(u, a, false);
+    if (!t.valid || t.rows <= wg * a.tile_rows) continue;
+    const int rows = min(t.rows - wg * a.tile_rows, a.tile_rows);  // of this tile
+    const int p = t.row0 + wg * a.tile_rows + (threadIdx.x & 127);
+    const int qr = p / a.group;  // row of the chunk
+    const int seen = (int)(a.causal ? min(t.L, max((int64_t)0, t.L - t.sq.Lq + qr + 1)) : t.L);
+    const bool row_ok = (int)(threadIdx.x & 127) < rows;
+    float m = -INFINITY, l = 0.f;
+    for (int j = 0; j < t.nkv; ++j) {
+      const KvTile kt = kv_tile(t, j);
+      if (!mbar_wait_warp(bar(S::BAR_SFULL + wg), s_it & 1, abort_flag)) return;
+      ++s_it;
+      tc_fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, s[c]);
+      tmem_wait_ld();
+      const int nv = min(kt.valid, seen - kt.pos);  // this row's visible columns
+      if (__any_sync(0xffffffffu, nv < kTileN)) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (c * 32 + e >= nv) s[c][e] = __float_as_uint(-INFINITY);
+      }
+      float mq[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float x = __uint_as_float(s[c][0]);
+#pragma unroll
+        for (int e = 1; e < 31; e += 2) x = max3f(x, __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+        mq[c] = fmaxf(x, __uint_as_float(s[c][31]));
+      }
+      const float mxs = max3f(mq[0], mq[1], fmaxf(mq[2], mq[3])) * sl2;
+      // Lazy rescaling: a stale maximum stays while the new one exceeds it by at most 8 (log2
+      // units), so P stays <= 256; a row's first visible key sets it (its accumulator holds zeros).
+      const bool first = m == -INFINITY;
+      // (rows past the tile's last hold another sequence's queries: they decide nothing)
+      const bool rescale = __any_sync(0xffffffffu, row_ok && !first && mxs > m + 8.f);
+      float alpha = 1.f;
+      if (first) {
+        m = mxs;
+      } else if (rescale) {
+        const float mn = fmaxf(m, mxs);
+        alpha = ex2_approx(m - mn);
+        m = mn;
+        l *= alpha;
+      }
+      l += exp_store_tile(s, sl2, m == -INFINITY ? 0.f : m, tS);  // hidden columns give exact zeros
+      if (rescale) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          tmem_ld32(tO + c * 32, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+          tmem_st32(tO + c * 32, o);
+        }
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(S::BAR_PFULL + wg));
+    }
+    // Epilogue: O / l -> bf16. A 4x4 transpose of 16-byte vectors inside each lane quad lets every
+    // store write 8 rows x 64 contiguous bytes instead of 32 rows x 16.
+    const int h = t.hkv * a.group + p - qr * a.group;
+    __nv_bfloat16* orow = a.o + (t.sq.q_begin + qr) * a.o_stride + (int64_t)h * kD;
+    if (t.nkv > 0) {
+      if (!mbar_wait_warp(bar(S::BAR_OFULL + wg), o_it & 1, abort_flag)) return;
+      ++o_it;
+      tc_fence_after();
+      const float inv = l == 0.f ? 0.f : 1.f / l;  // no visible key: zero row
+      const bool none = m == -INFINITY;
+      const int qj = lane & 3;
+      __nv_bfloat16* quad[4];
+      bool live[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        quad[r] = reinterpret_cast<__nv_bfloat16*>(
+            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(orow), (lane & ~3) + r));
+        live[r] = __shfl_sync(0xffffffffu, row_ok ? 1 : 0, (lane & ~3) + r) != 0;
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t o[32];
+        tmem_ld32(tO + c * 32, o);
+        tmem_wait_ld();
+        uint4 v[4];
+        auto val = [&](int e) { return none ? 0.f : __uint_as_float(o[e]) * inv; };
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[e] = make_uint4(pack_bf16x2(val(8 * e), val(8 * e + 1)), pack_bf16x2(val(8 * e + 2), val(8 * e + 3)),
+                            pack_bf16x2(val(8 * e + 4), val(8 * e + 5)), pack_bf16x2(val(8 * e + 6), val(8 * e + 7)));
+        quad_transpose16(v, qj);  // v[r] = vector qj of the quad's row r
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (live[r]) reinterpret_cast<uint4*>(quad[r] + c * 32)[qj] = v[r];
+      }
+      // O is read out; the next unit's first PV may overwrite it once this
+      // warpgroup arrives on its first P barrier (program order + fence).
+      tc_fence_before();
+    } else if (row_ok) {
+      uint4* dst = reinterpret_cast<uint4*>(orow);
+      for (int v = 0; v < kD / 8; ++v) dst[v] = make_uint4(0, 0, 0, 0);
+    }
+  }
+}
+
+template <int kFmt, bool kPair>
+__global__ void __launch_bounds__(Layout<kFmt, kPair>::kThreads, 1)
+    attn_chunk_mma_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                          const __grid_constant__ CUtensorMap tmV,                          const __grid_constant__ CUtensorMap tmKc, const __grid_constant__ CUtensorMap tmVc,
                           const __grid_constant__ CUtensorMap tmKg, const __grid_constant__ CUtensorMap tmVg,
                           const __grid_constant__ ChunkArgs a) {
-  using S = Layout<kFmt>;
+  using S = Layout<kFmt, kPair>;
   constexpr bool kQuant = S::kQuant;
   constexpr int kStagesK = S::kStagesK, kStagesV = S::kStagesV;
   extern __shared__ uint8_t smem_raw[];
@@ -260,7 +413,7 @@ __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kOffMisc + 16);
 
   if (threadIdx.x == 0) {
-    mbar_init(bar(S::BAR_QFULL), 4);
+    mbar_init(bar(S::BAR_QFULL), 1);
     mbar_init(bar(S::BAR_QEMPTY), 1);
     for (int s = 0; s < kStagesK; ++s) {
       mbar_init(bar(S::BAR_KFULL + s), S::kFull);
@@ -272,10 +425,10 @@ __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(S::BAR_SFULL + i), 1);
-      mbar_init(bar(S::BAR_PFULL + i), 8);  // one arrival per softmax warp
+      mbar_init(bar(S::BAR_PFULL + i), kPair ? 4 : 8);  // one arrival per warp that writes this P
+      mbar_init(bar(S::BAR_OFULL + i), 1);
     }
     mbar_init(bar(S::BAR_OREADY), 1);
-    mbar_init(bar(S::BAR_OFULL), 1);
     mbar_init(bar(S::BAR_XML), 128);  // every thread of warpgroup 1
     mbar_init(bar(S::BAR_XF), 128);   // every thread of warpgroup 0
     mbar_init(bar(S::BAR_DRAIN), 1);
@@ -486,10 +639,87 @@ __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
             mma_ts(d, p + s * 8, b + (4 * h + s) * (2048 >> 4), idesc_pv, (acc || s > 0) ? 1u : 0u);
         }
       };
+      // pair: row tile i against KV tiles: S(i) = Q(i) K^T, O(i) (+)= P(i) V
+      auto qk_tile = [&](int i, int kst, int n_rows) {
+        const uint32_t idesc = n_rows == kTileN ? idesc_qk_full : make_idesc_bf16(128, (n_rows + 15) & ~15, false);
+        const uint32_t x = dq + i * kStageStep, b = dk0 + kst * kStageStep;
+#pragma unroll
+        for (int s = 0; s < kD / 16; ++s) {
+          const uint32_t off = ((s >> 2) * kChunkBytes + (s & 3) * 32) >> 4;
+          mma_ss(tmem + i * 128, x + off, b + off, idesc, s > 0 ? 1u : 0u);
+        }
+      };
+      auto pv_tile = [&](int i, int vst, int ksteps, bool acc) {
+        const uint32_t b = dv0 + vst * kStageStep;
+        const uint32_t d = tmem + 256 + i * 128, p = tmem + i * 128;
+        if (ksteps == 8) {
+#pragma unroll
+          for (int s = 0; s < 8; ++s) mma_ts(d, p + s * 8, b + s * (2048 >> 4), idesc_pv, (acc || s > 0) ? 1u : 0u);
+        } else {
+          for (int s = 0; s < ksteps; ++s) mma_ts(d, p + s * 8, b + s * (2048 >> 4), idesc_pv, (acc || s > 0) ? 1u : 0u);
+        }
+      };
       uint32_t q_it = 0, k_it = 0, v_it = 0;
-      uint32_t g = 0;  // KV tiles whose PVs were issued (all units), = S tile index
+      uint32_t p_it[2] = {0, 0};
       bool ok = true;
-      for (int u = blockIdx.x; u < total_units && ok; u += gridDim.x) {
+      for (int u = blockIdx.x; kPair && u < total_units && ok; u += gridDim.x) {
+        const Unit t = decode_unit(u, a, false);
+        if (!t.valid || t.nkv == 0) continue;
+        const int nt = t.rows > a.tile_rows ? 2 : 1;
+        ok = mbar_wait(bar(S::BAR_QFULL), q_it & 1, abort_flag);
+        if (!ok) break;
+        ++q_it;
+        {
+          const int kst = k_it % kStagesK;
+          ok = mbar_wait(bar(S::BAR_KFULL + kst), (k_it / kStagesK) & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const int valid = kv_tile(t, 0).valid;
+          for (int i = 0; i < nt; ++i) {
+            qk_tile(i, kst, valid);
+            umma_commit(bar(S::BAR_SFULL + i));
+          }
+          umma_commit(bar(S::BAR_KEMPTY + kst));
+          ++k_it;
+          if (t.nkv == 1) umma_commit(bar(S::BAR_QEMPTY));
+        }
+        for (int j = 0; j < t.nkv && ok; ++j) {
+          const int ks = (kv_tile(t, j).valid + 15) >> 4;  // 1..8 K-steps
+          const int vst = v_it % kStagesV, kst = k_it % kStagesK;
+          ok = mbar_wait(bar(S::BAR_VFULL + vst), (v_it / kStagesV) & 1, abort_flag);
+          if (!ok) break;
+          const bool more = j + 1 < t.nkv;
+          const int next = more ? kv_tile(t, j + 1).valid : 0;
+          for (int i = 0; i < nt && ok; ++i) {
+            ok = mbar_wait(bar(S::BAR_PFULL + i), p_it[i] & 1, abort_flag);
+            if (!ok) break;
+            ++p_it[i];
+            tc_fence_after();
+            pv_tile(i, vst, ks, j > 0);
+            if (more) {
+              if (i == 0) {
+                ok = mbar_wait(bar(S::BAR_KFULL + kst), (k_it / kStagesK) & 1, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+              }
+              qk_tile(i, kst, next);
+              umma_commit(bar(S::BAR_SFULL + i));
+            } else {
+              umma_commit(bar(S::BAR_OFULL + i));
+            }
+          }
+          if (!ok) break;
+          umma_commit(bar(S::BAR_VEMPTY + vst));
+          ++v_it;
+          if (more) {
+            umma_commit(bar(S::BAR_KEMPTY + kst));
+            ++k_it;
+            if (j + 2 == t.nkv) umma_commit(bar(S::BAR_QEMPTY));  // last QK issued
+          }
+        }
+      }
+      uint32_t g = 0;  // KV tiles whose PVs were issued (all units), = S tile index
+      for (int u = blockIdx.x; !kPair && u < total_units && ok; u += gridDim.x) {
         const Unit t = decode_unit(u, a, false);
         if (!t.valid || t.nkv == 0) continue;
         ok = mbar_wait(bar(S::BAR_QFULL), q_it & 1, abort_flag);
@@ -549,20 +779,45 @@ __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
       mbar_wait_drain(bar(S::BAR_DRAIN), 0, 100000000ull);
     }
     __syncwarp();
-  }
-  } else if (warp >= 12) {
+    } else {
+      // ------------------------------------------------------------- loader of Q
+      // The box brings all heads of the KV head's group for a tile's chunk rows: packed order.
+      const uint64_t pol = policy_evict_first();
+      const uint32_t half_bytes = a.tile_rows * 128;
+      uint32_t q_it = 0;  // units whose Q was loaded
+      bool ok = true;
+      for (int u = blockIdx.x; u < total_units && ok; u += gridDim.x) {
+        const Unit t = decode_unit(u, a, false);
+        if (!t.valid || t.nkv == 0) continue;
+        if (q_it > 0) ok = mbar_wait_warp(bar(S::BAR_QEMPTY), (q_it - 1) & 1, abort_flag);
+        if (!ok) break;
+        ++q_it;
+        if (lane == 0) {
+          const int nt = t.rows > a.tile_rows ? 2 : 1;
+          mbar_arrive_expect_tx(bar(S::BAR_QFULL), nt * 2 * half_bytes);
+          for (int i = 0; i < nt; ++i) {
+            const uint32_t dst = base + S::kOffQ + i * kTileBytes;
+            const int row = (int)t.sq.q_begin + (t.row0 + i * a.tile_rows) / a.group;
+            tma_load_3d(dst, &tmQ, bar(S::BAR_QFULL), 0, t.hkv * a.group, row, pol);
+            tma_load_3d(dst + kChunkBytes, &tmQ, bar(S::BAR_QFULL), 64, t.hkv * a.group, row, pol);
+          }
+        }
+        __syncwarp();
+      }
+      if (lane == 0 && *abort_flag && q_it > 0) mbar_wait_drain(bar(S::BAR_QFULL), (q_it - 1) & 1, 100000000ull);
+      __syncwarp();
+    }
+  } else if (kQuant && warp >= 12) {
     set_max_registers<S::kRegsOther, false>();
-    // ------------------------------------------------- Q staging and expansion
-    // Quantised caches: warps 12-15 fill the K ring, warps 16-19 the V ring; the last four of the
-    // CTA stage Q (with a quantised cache while the first K tile is expanded).
-    const bool is_k = kQuant && warp < 16;
-    const int lead = kQuant && !is_k ? 16 : 12;  // this warpgroup's first warp
+    // ------------------------------------------------------------- expansion
+    // Warps 12-15 fill the K ring, warps 16-19 the V ring.
+    const bool is_k = warp < 16;
+    const int lead = is_k ? 12 : 16;  // this warpgroup's first warp
     const int tid = threadIdx.x - lead * 32;
     const int nst = is_k ? kStagesK : kStagesV;
     const int bfull = is_k ? S::BAR_KFULL : S::BAR_VFULL, bempty = is_k ? S::BAR_KEMPTY : S::BAR_VEMPTY;
     const int rfull = S::BAR_RFULL + (is_k ? 0 : kRaw), rempty = S::BAR_REMPTY + (is_k ? 0 : kRaw);
     const uint32_t ring = is_k ? S::kOffK : S::kOffV;
-    uint32_t q_it = 0;  // units whose Q was staged
     uint32_t n = 0;     // ring positions filled; every position is filled by this warpgroup, in order, so each
                         // wait below is for the phase right before (a wait by parity cannot tell phases two apart)
     uint32_t raw_it = 0, land = 0;
@@ -655,44 +910,16 @@ __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
     for (int u = blockIdx.x; u < total_units && ok; u += gridDim.x) {
       const Unit t = decode_unit(u, a, false);
       if (!t.valid || t.nkv == 0) continue;
-      if (!is_k) {
-        if (q_it > 0) ok = mbar_wait_warp(bar(S::BAR_QEMPTY), (q_it - 1) & 1, abort_flag);
-        if (!ok) break;
-        ++q_it;
-#pragma unroll 1
-        for (int i0 = 0; i0 < 16; i0 += 4) {
-          uint4 val[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int p = (i0 + i) * 8 + (tid >> 4);
-            val[i] = make_uint4(0, 0, 0, 0);
-            if (p < t.rows) {
-              const int r = (t.row0 + p) / a.group, h = t.hkv * a.group + (t.row0 + p) - r * a.group;
-              val[i] = __ldg(reinterpret_cast<const uint4*>(a.q + (t.sq.q_begin + r) * a.q_stride + (int64_t)h * kD) + (tid & 15));
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int p = (i0 + i) * 8 + (tid >> 4), c = tid & 15;
-            *reinterpret_cast<uint4*>(smem + S::kOffQ + (c >> 3) * kChunkBytes + p * 128 + (((c & 7) ^ (p & 7)) << 4)) = val[i];
-          }
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(S::BAR_QFULL));
-      }
-      if constexpr (kQuant) {
-        for (int j = 0; j < t.nkv && ok; ++j, ++n) {
-          if (t.t0 + j < t.sp.cached) {
-            ok = expand();
-            ++raw_it;
-          } else {
-            ok = direct(t.hkv, kv_tile(t, j));
-          }
+      for (int j = 0; j < t.nkv && ok; ++j, ++n) {
+        if (t.t0 + j < t.sp.cached) {
+          ok = expand();
+          ++raw_it;
+        } else {
+          ok = direct(t.hkv, kv_tile(t, j));
         }
       }
     }
-    if (kQuant && warp == lead && lane == 0 && *abort_flag) {
+    if (warp == lead && lane == 0 && *abort_flag) {
       // Drain: fresh tiles' copies that may still be in flight.
       for (uint32_t i = (n > (uint32_t)nst ? n - nst : 0); i < n; ++i)
         mbar_wait_drain(bar(bfull + i % nst), (i / nst) & 1, 100000000ull);
@@ -702,6 +929,9 @@ __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
   } else {
     set_max_registers<S::kRegsSoftmax, true>();
     // ---------------------------------------------------------------- softmax
+    if constexpr (kPair) {
+      softmax_pair<S>(a, tmem, bar0, abort_flag);
+    } else {
     const int wg = warp >> 2;           // 0: keys 0-63 of a tile, 1: keys 64-127
     const int wq = warp & 3;
     const int row_in_tile = threadIdx.x & 127;
@@ -721,6 +951,7 @@ __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
       // A warp whose 32 rows lie past the unit's last one only keeps the barriers going (its rows
       // of P hold anything: rows of a product do not mix).
       const bool idle = wq * 32 >= t.rows;
+      const bool row_ok = row_in_tile < t.rows;
       float m = -INFINITY;  // running max (log2 units), -inf until a visible key
       float l = 0.f;
       for (int j = 0; j < t.nkv; ++j, ++g) {
@@ -757,7 +988,7 @@ __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
           // by at most 8 (log2 units), so P stays <= 256. A row's first visible
           // key sets it (its accumulator holds zeros or is not written yet).
           const bool first = m == -INFINITY;
-          const bool need = !first && mxs > m + 8.f;
+          const bool need = row_ok && !first && mxs > m + 8.f;  // (rows past the tile's last are another sequence's)
           if (first) m = mxs;
           if (__any_sync(0xffffffffu, need)) {
             const float mn = first ? m : fmaxf(m, mxs);
@@ -790,7 +1021,6 @@ __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
       if (!ok) break;
       // Epilogue: merge the two halves, then O / l -> bf16 (the row's only split)
       // or O, (m, l) -> fp32 partials. Warpgroup w writes output columns [64w, 64w + 64).
-      const bool row_ok = row_in_tile < t.rows;
       const bool alone = t.sp.total <= a.split_chunks;
       const int h = t.hkv * a.group + (t.row0 + row_in_tile) - qr * a.group;
       __nv_bfloat16* orow = a.o + (t.sq.q_begin + qr) * a.o_stride + (int64_t)h * kD + wg * kHalfN;
@@ -862,6 +1092,7 @@ __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
         for (int v = 0; v < kHalfN / 8; ++v) dst[v] = make_uint4(0, 0, 0, 0);
       }
     }
+    }
   }
 
   tc_fence_before();
@@ -873,30 +1104,34 @@ __global__ void __launch_bounds__(Layout<kFmt>::kThreads, 1)
   if (threadIdx.x == 0 && *abort_flag) set_error(a.err, kDevWaitTimeout);
 }
 
-template <int kFmt>
+template <int kFmt, bool kPair>
 cudaError_t launch(const ChunkMaps& m, const ChunkArgs& a, int num_sms, cudaStream_t stream) {
+  using S = Layout<kFmt, kPair>;
   static std::atomic<bool> attr_set[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-    e = cudaFuncSetAttribute(attn_chunk_mma_kernel<kFmt>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)Layout<kFmt>::kSmemBytes);
+    e = cudaFuncSetAttribute(attn_chunk_mma_kernel<kFmt, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)S::kSmemBytes);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
-  return launch_pdl(attn_chunk_mma_kernel<kFmt>, dim3(std::min(a.total_units, num_sms)), dim3(Layout<kFmt>::kThreads),
-                    Layout<kFmt>::kSmemBytes, stream, m.k, m.v, m.kc, m.vc, m.kg, m.vg, a);
+  return launch_pdl(attn_chunk_mma_kernel<kFmt, kPair>, dim3(std::min(a.total_units, num_sms)), dim3(S::kThreads),
+                    S::kSmemBytes, stream, m.q, m.k, m.v, m.kc, m.vc, m.kg, m.vg, a);
 }
 
 }  // namespace chunk128
 
 cudaError_t launch_attn_chunk_mma(const ChunkMaps& maps, const ChunkArgs& a, int format, int num_sms,
                                   cudaStream_t stream) {
+  const bool pair = a.unit_rows > a.tile_rows;
   switch (format) {
-    case kFmtBf16: return chunk128::launch<kFmtBf16>(maps, a, num_sms, stream);
-    case kFmtE4m3: return chunk128::launch<kFmtE4m3>(maps, a, num_sms, stream);
-    default: return chunk128::launch<kFmtInt8>(maps, a, num_sms, stream);
+    case kFmtBf16:
+      return pair ? chunk128::launch<kFmtBf16, true>(maps, a, num_sms, stream)
+                  : chunk128::launch<kFmtBf16, false>(maps, a, num_sms, stream);
+    case kFmtE4m3: return chunk128::launch<kFmtE4m3, false>(maps, a, num_sms, stream);
+    default: return chunk128::launch<kFmtInt8, false>(maps, a, num_sms, stream);
   }
 }
 

@@ -374,6 +374,7 @@ int check_chunk_sizes(int format, int batch, int Hq, int Hkv, int max_q, int max
     return fail(DLLM_ERR_UNSUPPORTED, "cache format %d not supported", format);
   if (Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0)
     return fail(DLLM_ERR_UNSUPPORTED, "num_heads %d must be a positive multiple of num_kv_heads %d", Hq, Hkv);
+  if (Hq / Hkv > 128) return fail(DLLM_ERR_UNSUPPORTED, "%d query heads per KV head (at most 128)", Hq / Hkv);
   if (batch < 0 || max_q < 0 || max_context < 0 || max_fresh < 0)
     return fail(DLLM_ERR_INVALID_ARG, "negative size");
   if (max_context > (1 << 30) || max_fresh > (1 << 30) || (int64_t)max_q * (Hq / Hkv) > (1 << 30))
@@ -549,6 +550,8 @@ int dllm_attn_chunk_fwd(const void* q, int64_t q_tok_stride, const void* k, int6
   a.err = err_flag;
   dllm::ChunkMaps maps = {};
   if (plan.rows == dllm::kChunkMmaRows) {
+    const int group = num_heads / num_kv_heads;
+    if ((rc = encode_rows_map(&maps.q, q, total_q, num_heads, q_tok_stride, 128 / group, group)) != DLLM_OK) return rc;
     if (k != nullptr) {
       if ((rc = encode_rows_map(&maps.k, k, total_k, num_kv_heads, k_tok_stride, 128)) != DLLM_OK) return rc;
       if ((rc = encode_rows_map(&maps.v, v, total_k, num_kv_heads, v_tok_stride, 128)) != DLLM_OK) return rc;

@@ -185,28 +185,31 @@ def test_long(dev, fmt, shape, causal, tables):
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", ["bf16", "e4m3", "int8"])
 @pytest.mark.parametrize("tables", [True, False])
-def test_many_units(dev, fmt, tables):
+@pytest.mark.parametrize("most", [60, 34])
+def test_many_units(dev, fmt, tables, most):
     """More row tiles than the GPU has SMs, of unequal lengths, so that a CTA
-    takes several one after another: each sequence's rows equal, bit for bit,
-    those of a launch of its own, and a few are held to the 64-bit bound."""
+    takes several one after another. Some sequences are held to the 64-bit
+    bound; where a launch of one sequence cuts its rows into the same units
+    (at most 34 x 3 packed rows: one tile), its bits are the batch's."""
     g = I.gen(17)
     n = 90
-    nq = torch.randint(0, 60, (n,), generator=g).tolist()
+    nq = torch.randint(0, most, (n,), generator=g).tolist()
     nc = torch.randint(0, 500, (n,), generator=g).tolist()
     nc[3], nc[40], nq[7], nq[40] = 0, 0, 0, 33
+    seqs = [3, 7, 11, 40] + list(range(0, n, 8))
     nf = [x if i % 3 else min(x, 17) for i, x in enumerate(nq)]
     c = Case(18, fmt, 12, 4, nq, nc, nf, tables, page=128, spread=False)
     args, kw = c.args(dev)
     ops = _ops()
     for causal in (False, True):
         out = ops.chunk_attention(*args, causal=causal, max_context=512, **kw)
-        c.check(out, causal, seqs=[3, 7, 11, 40])
+        c.check(out, causal, seqs=seqs)
         for _ in range(3):  # launches back to back
             again = ops.chunk_attention(*args, causal=causal, max_context=512, **kw)
         assert torch.equal(again[:sum(nq)], out[:sum(nq)])
         cu, cuk, cus = (_cu(x).tolist() for x in (nq, nf, nc))
         for b in range(0, n, 4):
-            if nq[b] == 0:
+            if nq[b] == 0 or most > 34:
                 continue
             one = dict(kw)
             one |= {"k": kw["k"][cuk[b]:cuk[b + 1]], "v": kw["v"][cuk[b]:cuk[b + 1]], "cu_seqlens_k": _cu([nf[b]]).to(dev)}
@@ -221,6 +224,35 @@ def test_many_units(dev, fmt, tables):
                                         causal=causal, max_context=512, **one)
             assert torch.equal(alone, out[cu[b]:cu[b + 1]]), b
     assert ops.read_device_status(dev) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3", "int8"])
+@pytest.mark.parametrize("heads,tables", [((4, 4), True), ((12, 4), False), ((10, 2), True)])
+def test_long_chunks_of_many_sequences(dev, fmt, heads, tables):
+    """Enough rows that a work unit takes two row tiles (and a quantised cache
+    is expanded first), of unequal lengths; 3 and 5 heads per KV head do not
+    divide a tile's 128 rows."""
+    hq, hkv = heads
+    g = I.gen(23)
+    n = 40 if hkv == 4 else 80
+    nq = torch.randint(1, 280, (n,), generator=g).tolist()
+    nc = torch.randint(0, 420, (n,), generator=g).tolist()
+    nq[5], nq[6], nc[6], nc[9] = 257, 0, 0, 0
+    nf = nq if hkv == 4 else [0] * n
+    if hkv == 2:
+        nc = [a + b if i % 5 else a for i, (a, b) in enumerate(zip(nc, nq))]
+    c = Case(24, fmt, hq, hkv, nq, nc, nf if hkv == 4 else None, tables, page=128, spread=hq == 4)
+    args, kw = c.args(dev)
+    for causal in (True, False):
+        out = torch.full(c.q.shape, 5.0, dtype=torch.bfloat16, device=dev)
+        _ops().chunk_attention(*args, causal=causal, out=out, **kw)
+        c.check(out, causal, seqs=[5, 6, 9, 10] if hq == 4 else [9, 13])
+        assert (out[sum(nq):] == 5).all()
+        for _ in range(2):
+            again = _ops().chunk_attention(*args, causal=causal, **kw)
+        assert torch.equal(again[:sum(nq)], out[:sum(nq)])
+    assert _ops().read_device_status(dev) == 0
 
 
 @pytest.mark.gpu
