@@ -457,43 +457,46 @@ int64_t dllm_attn_chunk_workspace(int format, int batch, int num_heads, int num_
       .workspace_bytes;
 }
 
-int dllm_attn_chunk_fwd(const void* q, int64_t q_tok_stride, const void* k, int64_t k_tok_stride, const void* v,
-                        int64_t v_tok_stride, const void* k_cache, const void* v_cache, const void* k_exp,
-                        const void* v_exp, int format, int64_t num_slots, const int32_t* block_tables,
-                        int64_t table_stride, int max_blocks, int block_size, const int32_t* context_lens,
-                        const int32_t* slots, const int32_t* cu_seqlens_slots, int64_t total_slots,
-                        int max_context, void* o, int64_t o_tok_stride, const int32_t* cu_seqlens_q,
-                        const int32_t* cu_seqlens_k, int batch, int max_seqlen_q, int max_fresh, int64_t total_q,
-                        int64_t total_k, int num_heads, int num_kv_heads, int head_dim, float softmax_scale,
-                        int causal, void* workspace, int64_t workspace_bytes, int32_t* err_flag, void* stream) {
+int dllm_attn_chunk_fwd(const dllm_chunk_args* args) {
+  if (args == nullptr) return fail(DLLM_ERR_INVALID_ARG, "args is null");
+  const dllm_chunk_args& p = *args;
+  const void *q = p.q, *k = p.k, *v = p.v, *k_cache = p.k_cache, *v_cache = p.v_cache, *k_exp = p.k_exp, *v_exp = p.v_exp;
+  const int64_t q_tok_stride = p.q_tok_stride, k_tok_stride = p.k_tok_stride, v_tok_stride = p.v_tok_stride;
+  const int64_t o_tok_stride = p.o_tok_stride, num_slots = p.num_slots, total_slots = p.total_slots;
+  const int64_t total_q = p.total_q, total_k = p.total_k;
+  const int32_t *block_tables = p.block_tables, *slots = p.slots;
+  const int format = p.format, batch = p.batch, num_heads = p.num_heads, num_kv_heads = p.num_kv_heads;
+  const int head_dim = p.head_dim, max_seqlen_q = p.max_seqlen_q, block_size = p.block_size, max_blocks = p.max_blocks;
+  int max_context = p.max_context, max_fresh = p.max_fresh;
+  void* workspace = p.workspace;
   if (head_dim != 128) return fail(DLLM_ERR_UNSUPPORTED, "head_dim %d not supported (only 128)", head_dim);
   int rc = check_chunk_sizes(format, batch, num_heads, num_kv_heads, max_seqlen_q, max_context, max_fresh);
   if (rc != DLLM_OK) return rc;
   if (total_q < 0 || total_k < 0 || total_slots < 0 || num_slots < 0)
     return fail(DLLM_ERR_INVALID_ARG, "negative size");
   if (num_slots >= (int64_t)1 << 31) return fail(DLLM_ERR_TOO_LARGE, "too many cache slots");
-  if (!(softmax_scale > 0.f)) return fail(DLLM_ERR_INVALID_ARG, "softmax_scale must be > 0");
+  if (!(p.softmax_scale > 0.f)) return fail(DLLM_ERR_INVALID_ARG, "softmax_scale must be > 0");
   if (block_tables != nullptr && slots != nullptr)
     return fail(DLLM_ERR_INVALID_ARG, "block tables and a slot list are both given");
   const bool cached = block_tables != nullptr || slots != nullptr;
   if (block_tables != nullptr) {
-    if (context_lens == nullptr) return fail(DLLM_ERR_INVALID_ARG, "block_tables without context_lens");
-    if (block_size <= 0 || max_blocks < 0 || table_stride < max_blocks)
+    if (p.context_lens == nullptr) return fail(DLLM_ERR_INVALID_ARG, "block_tables without context_lens");
+    if (block_size <= 0 || max_blocks < 0 || p.table_stride < max_blocks)
       return fail(DLLM_ERR_INVALID_ARG, "bad block table shape");
   }
-  if (slots != nullptr && cu_seqlens_slots == nullptr)
+  if (slots != nullptr && p.cu_seqlens_slots == nullptr)
     return fail(DLLM_ERR_INVALID_ARG, "slots without cu_seqlens_slots");
   if (cached && (k_cache == nullptr || v_cache == nullptr)) return fail(DLLM_ERR_INVALID_ARG, "cache is null");
   if (cached && format != DLLM_KV_BF16 && (k_exp == nullptr || v_exp == nullptr))
     return fail(DLLM_ERR_INVALID_ARG, "a quantised cache needs k_exp and v_exp");
   if (!aligned(k_cache, 16) || !aligned(v_cache, 16))
     return fail(DLLM_ERR_ALIGNMENT, "caches must be 16-byte aligned");
-  if ((k == nullptr) != (v == nullptr) || (k == nullptr) != (cu_seqlens_k == nullptr))
+  if ((k == nullptr) != (v == nullptr) || (k == nullptr) != (p.cu_seqlens_k == nullptr))
     return fail(DLLM_ERR_INVALID_ARG, "k, v and cu_seqlens_k are given together");
   if (batch == 0 || total_q == 0 || max_seqlen_q == 0) return DLLM_OK;
-  if (cu_seqlens_q == nullptr) return fail(DLLM_ERR_INVALID_ARG, "cu_seqlens_q is null");
+  if (p.cu_seqlens_q == nullptr) return fail(DLLM_ERR_INVALID_ARG, "cu_seqlens_q is null");
   if ((rc = check_rows("q", q, q_tok_stride, num_heads, total_q)) != DLLM_OK) return rc;
-  if ((rc = check_rows("o", o, o_tok_stride, num_heads, total_q)) != DLLM_OK) return rc;
+  if ((rc = check_rows("o", p.o, o_tok_stride, num_heads, total_q)) != DLLM_OK) return rc;
   if (k != nullptr) {
     if ((rc = check_rows("k", k, k_tok_stride, num_kv_heads, total_k)) != DLLM_OK) return rc;
     if ((rc = check_rows("v", v, v_tok_stride, num_kv_heads, total_k)) != DLLM_OK) return rc;
@@ -504,8 +507,8 @@ int dllm_attn_chunk_fwd(const void* q, int64_t q_tok_stride, const void* k, int6
       dllm::plan_attn_chunk(format, batch, num_kv_heads, num_heads / num_kv_heads, max_seqlen_q, max_context,
                             max_fresh, num_sms_of_current_device());
   if (plan.workspace_bytes > 0) {
-    if (workspace == nullptr || workspace_bytes < plan.workspace_bytes)
-      return fail(DLLM_ERR_INVALID_ARG, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
+    if (workspace == nullptr || p.workspace_bytes < plan.workspace_bytes)
+      return fail(DLLM_ERR_INVALID_ARG, "workspace of %lld bytes, %lld needed", (long long)p.workspace_bytes,
                   (long long)plan.workspace_bytes);
     if (!aligned(workspace, 16)) return fail(DLLM_ERR_ALIGNMENT, "workspace is not 16-byte aligned");
   }
@@ -522,19 +525,19 @@ int dllm_attn_chunk_fwd(const void* q, int64_t q_tok_stride, const void* k, int6
   a.v_exp = static_cast<const uint8_t*>(v_exp);
   a.num_slots = num_slots;
   a.slots = slots;
-  a.cu_s = cu_seqlens_slots;
+  a.cu_s = p.cu_seqlens_slots;
   a.total_slots = total_slots;
   a.tables = block_tables;
-  a.table_stride = table_stride;
+  a.table_stride = p.table_stride;
   a.max_blocks = max_blocks;
   a.block_size = block_tables != nullptr ? block_size : 1;
   a.block_shift = -1;
   for (int s = 0; s < 31; ++s)
     if (a.block_size == 1 << s) a.block_shift = s;
-  a.ctx = context_lens;
+  a.ctx = p.context_lens;
   a.max_context = max_context;
-  a.cu_q = cu_seqlens_q;
-  a.cu_k = cu_seqlens_k;
+  a.cu_q = p.cu_seqlens_q;
+  a.cu_k = p.cu_seqlens_k;
   a.total_q = total_q;
   a.total_k = total_k;
   a.max_q = max_seqlen_q;
@@ -543,11 +546,11 @@ int dllm_attn_chunk_fwd(const void* q, int64_t q_tok_stride, const void* k, int6
   a.Hq = num_heads;
   a.Hkv = num_kv_heads;
   a.group = num_heads / num_kv_heads;
-  a.scale_log2 = softmax_scale * 1.4426950408889634f;
-  a.causal = causal != 0;
-  a.o = static_cast<__nv_bfloat16*>(o);
+  a.scale_log2 = p.softmax_scale * 1.4426950408889634f;
+  a.causal = p.causal != 0;
+  a.o = static_cast<__nv_bfloat16*>(p.o);
   a.o_stride = o_tok_stride;
-  a.err = err_flag;
+  a.err = p.err_flag;
   dllm::ChunkMaps maps = {};
   if (plan.rows == dllm::kChunkMmaRows) {
     const int group = num_heads / num_kv_heads;
@@ -566,20 +569,20 @@ int dllm_attn_chunk_fwd(const void* q, int64_t q_tok_stride, const void* k, int6
     } else if (cached && num_slots > 0) {
       for (int i = 0; i < 2; ++i) {
         CUtensorMap* m = i == 0 ? &maps.kc : &maps.vc;
-        const void* p = i == 0 ? k_cache : v_cache;
-        rc = format == DLLM_KV_BF16 ? encode_rows_map(m, p, num_slots, num_kv_heads, row, 128)
-                                    : encode_codes_map(m, p, num_slots, num_kv_heads);
+        const void* c = i == 0 ? k_cache : v_cache;
+        rc = format == DLLM_KV_BF16 ? encode_rows_map(m, c, num_slots, num_kv_heads, row, 128)
+                                    : encode_codes_map(m, c, num_slots, num_kv_heads);
         if (rc != DLLM_OK) return rc;
         // tiles that are no run of slots: from a slot list, or from blocks smaller than a tile
         if (slots != nullptr || block_size % 128 != 0) {
-          rc = encode_gather_map(i == 0 ? &maps.kg : &maps.vg, p, num_slots, row, format == DLLM_KV_BF16);
+          rc = encode_gather_map(i == 0 ? &maps.kg : &maps.vg, c, num_slots, row, format == DLLM_KV_BF16);
           if (rc != DLLM_OK) return rc;
         }
       }
     }
   }
   cudaError_t e = dllm::launch_attn_chunk(a, format, plan, maps, workspace, num_sms_of_current_device(),
-                                          reinterpret_cast<cudaStream_t>(stream));
+                                          reinterpret_cast<cudaStream_t>(p.stream));
   if (e != cudaSuccess) return cuda_fail(e, "attn_chunk launch");
   return DLLM_OK;
 }

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libdllm_attn.so")
@@ -55,11 +56,7 @@ SIGNATURES = {
         _I,
     ),
     "dllm_attn_chunk_workspace": ([_I, _I, _I, _I, _I, _I, _I], _I64),
-    "dllm_attn_chunk_fwd": (
-        [_P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I, _I64, _P, _I64, _I, _I, _P, _P, _P, _I64, _I,
-         _P, _I64, _P, _P, _I, _I, _I, _I64, _I64, _I, _I, _I, _F, _I, _P, _I64, _P, _P],
-        _I,
-    ),
+    "dllm_attn_chunk_fwd": ([ctypes.c_char_p], _I),  # a packed dllm_chunk_args
     "dllm_attn_varlen_fwd": (
         [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I, _I, _I64, _I64, _I, _I, _I, _F, _P, _P, _P],
         _I,
@@ -102,6 +99,11 @@ SIGNATURES = {
         _I,
     ),
 }
+
+
+# dllm_chunk_args as bytes: 27 pointers and 64-bit sizes, 11 ints, the scale
+# (packing it costs a third of 39 converted arguments).
+CHUNK_ARGS = struct.Struct("=27q11if")
 
 
 class NativeLibraryMissing(RuntimeError):

@@ -185,26 +185,46 @@ def load_kvcache_quant(key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping)
     _kv_quant(False, key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping)
 
 
+def _same_device(*ts: torch.Tensor) -> int:
+    """Index of the CUDA device that holds every tensor (one integer query per
+    tensor: the quick form of ``_require_cuda``)."""
+    idx = ts[0].get_device()
+    for t in ts:
+        i = t.get_device()
+        if i != idx or i < 0:
+            _require_cuda(*ts)
+            raise ValueError("all tensors must be on one CUDA device")
+    return idx
+
+
+def _status_ptr_of(idx: int) -> int:
+    """``_status_ptr`` by device index."""
+    t = _STATUS.get(idx)
+    return t.data_ptr() if t is not None else _status_ptr(torch.device("cuda", idx))
+
+
 def _check_quant_cache(name, cache, exp, heads, head_dim) -> int:
     """Validates a quantised cache and its exponent bytes; returns its slots."""
-    if cache.dim() < 3 or cache.shape[-2] != heads or cache.shape[-1] != head_dim or not cache.is_contiguous():
+    sh = cache.shape
+    if len(sh) < 3 or sh[-2] != heads or sh[-1] != head_dim or not cache.is_contiguous():
         raise ValueError(f"{name}_cache must be contiguous [blocks, block_size, {heads}, {head_dim}]")
     slots = cache.numel() // (heads * head_dim)
-    if exp.dtype is not torch.uint8 or not exp.is_contiguous() or exp.shape[-1] != heads or exp.numel() != slots * heads:
+    if exp.dtype is not torch.uint8 or not exp.is_contiguous() or exp.numel() != slots * heads or exp.shape[-1] != heads:
         raise ValueError(f"{name}_exp must be contiguous uint8 [blocks, block_size, {heads}]")
     return slots
 
 
 def _kv_quant(store, key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping):
-    if key.dim() != 3 or value.shape != key.shape:
+    sh = key.shape
+    if len(sh) != 3 or value.shape != sh:
         raise ValueError("key and value must be [tokens, num_kv_heads, head_dim] of one shape")
-    N, H, D = key.shape
+    N, H, D = sh
     if key.dtype is not torch.bfloat16 or value.dtype is not torch.bfloat16:
         raise ValueError("key and value must be bfloat16")
     ks, vs = key.stride(), value.stride()
     if ks[2] != 1 or ks[1] != D or vs[2] != 1 or vs[1] != D:
         raise ValueError("key and value must have contiguous heads")
-    dev = _require_cuda(key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping)
+    dev = _same_device(key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping)
     fmt = _KV_FORMATS.get(k_cache.dtype, _native.KV_BF16)
     if fmt == _native.KV_BF16 or v_cache.dtype is not k_cache.dtype:
         raise ValueError("k_cache and v_cache must both be float8_e4m3fn or both int8")
@@ -217,10 +237,15 @@ def _kv_quant(store, key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping):
         return
     lib = _native.lib()
     fn = lib.dllm_store_kvcache_quant if store else lib.dllm_load_kvcache_quant
-    with _on_device(dev):
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            rc = fn(key.data_ptr(), ks[0], value.data_ptr(), vs[0], k_cache.data_ptr(), v_cache.data_ptr(),
+                    k_exp.data_ptr(), v_exp.data_ptr(), slot_mapping.data_ptr(), N, H, D, fmt, slots,
+                    _status_ptr_of(dev), _stream_ptr())
+    else:
         rc = fn(key.data_ptr(), ks[0], value.data_ptr(), vs[0], k_cache.data_ptr(), v_cache.data_ptr(),
                 k_exp.data_ptr(), v_exp.data_ptr(), slot_mapping.data_ptr(), N, H, D, fmt, slots,
-                _status_ptr(dev), _stream_ptr())
+                _status_ptr_of(dev), _stream_ptr())
     if rc:
         _native.check(rc, "store_kvcache_quant" if store else "load_kvcache_quant")
     LAUNCHES[0] += 1
@@ -618,10 +643,7 @@ def chunk_attention(
     ``causal``: the chunk's rows are the last positions of the keys, and row i
     of Lq sees the first L - Lq + i + 1 of L keys; else every row sees all. A
     row that sees no key is zero. Returns ``out`` (new by default)."""
-    if q.dim() != 3:
-        raise ValueError("q must be [tokens, num_heads, head_dim]")
-    Hq, D = q.shape[1], q.shape[2]
-    _check_rows("q", q, Hq, D)
+    Hq, D, q_str = _chunk_rows("q", q)
     if (k is None) != (v is None) or (k is None) != (cu_seqlens_k is None):
         raise ValueError("k, v and cu_seqlens_k go together")
     cached = block_tables is not None or slots is not None
@@ -629,106 +651,137 @@ def chunk_attention(
         raise ValueError("no keys: give block_tables, slots or fresh k and v")
     if cached and (k_cache is None or v_cache is None):
         raise ValueError("block_tables / slots need k_cache and v_cache")
-    dev = _require_cuda(q, cu_seqlens_q)
+    dev = _same_device(q, cu_seqlens_q)
     B = cu_seqlens_q.numel() - 1
     _check_cu("cu_seqlens_q", cu_seqlens_q, B, dev)
+    max_q = int(max_seqlen_q)
     fmt = _native.KV_BF16
-    Hkv = k.shape[1] if k is not None else k_cache.shape[-2]
-    k_ptr = v_ptr = cu_k_ptr = kx_ptr = vx_ptr = kc_ptr = vc_ptr = None
-    k_str = v_str = total_k = num_slots = max_fresh = 0
+    k_ptr = v_ptr = cu_k_ptr = kx_ptr = vx_ptr = kc_ptr = vc_ptr = k_str = v_str = total_k = num_slots = max_fresh = 0
+    bt_ptr = ctx_ptr = sl_ptr = cus_ptr = table_stride = max_blocks = block_size = total_slots = most = 0
     if k is not None:
-        _check_rows("k", k, Hkv, D)
-        _check_rows("v", v, Hkv, D)
-        if v.shape[0] != k.shape[0]:
-            raise ValueError("k and v have different row counts")
-        if k.device != dev or v.device != dev:
+        Hkv, Dk, k_str = _chunk_rows("k", k)
+        Hv, Dv, v_str = _chunk_rows("v", v)
+        total_k = k.shape[0]
+        if Dk != D or Dv != D or Hv != Hkv or v.shape[0] != total_k:
+            raise ValueError(f"k and v must be [rows, num_kv_heads, {D}] of one shape")
+        if k.get_device() != dev or v.get_device() != dev:
             raise ValueError("all tensors must be on the same device")
         _check_cu("cu_seqlens_k", cu_seqlens_k, B, dev)
-        k_ptr, k_str, v_ptr, v_str = k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0)
-        cu_k_ptr, total_k = cu_seqlens_k.data_ptr(), k.shape[0]
-        max_fresh = int(max_seqlen_q if max_seqlen_k is None else max_seqlen_k)
-    bt_ptr = ctx_ptr = sl_ptr = cus_ptr = None
-    table_stride = max_blocks = block_size = total_slots = 0
+        k_ptr, v_ptr, cu_k_ptr = k.data_ptr(), v.data_ptr(), cu_seqlens_k.data_ptr()
+        max_fresh = max_q if max_seqlen_k is None else int(max_seqlen_k)
+    else:
+        Hkv = k_cache.shape[-2]
     if cached:
         fmt = _KV_FORMATS.get(k_cache.dtype)
         if fmt is None or v_cache.dtype is not k_cache.dtype:
             raise ValueError("k_cache and v_cache must both be bfloat16, float8_e4m3fn or int8")
-        if (k_cache.dim() != 4 or k_cache.shape[2] != Hkv or k_cache.shape[3] != D or v_cache.shape != k_cache.shape
+        sh = k_cache.shape
+        if (len(sh) != 4 or sh[2] != Hkv or sh[3] != D or v_cache.shape != sh
                 or not k_cache.is_contiguous() or not v_cache.is_contiguous()):
             raise ValueError(f"caches must be contiguous [blocks, block_size, {Hkv}, {D}]")
-        if k_cache.device != dev or v_cache.device != dev:
+        if k_cache.get_device() != dev or v_cache.get_device() != dev:
             raise ValueError("all tensors must be on the same device")
-        block_size = k_cache.shape[1]
-        num_slots = k_cache.shape[0] * block_size
+        block_size = sh[1]
+        num_slots = sh[0] * block_size
         kc_ptr, vc_ptr = k_cache.data_ptr(), v_cache.data_ptr()
         if fmt != _native.KV_BF16:
             if k_exp is None or v_exp is None:
                 raise ValueError("a quantised cache needs k_exp and v_exp")
             _check_quant_cache("k", k_cache, k_exp, Hkv, D)
             _check_quant_cache("v", v_cache, v_exp, Hkv, D)
-            if k_exp.device != dev or v_exp.device != dev:
+            if k_exp.get_device() != dev or v_exp.get_device() != dev:
                 raise ValueError("all tensors must be on the same device")
             kx_ptr, vx_ptr = k_exp.data_ptr(), v_exp.data_ptr()
         if block_tables is not None:
             if slots is not None:
                 raise ValueError("give block_tables or slots, not both")
-            if (block_tables.dtype is not torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] != B
-                    or block_tables.device != dev or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1)):
+            sh, st = block_tables.shape, block_tables.stride()
+            if (block_tables.dtype is not torch.int32 or len(sh) != 2 or sh[0] != B
+                    or block_tables.get_device() != dev or (sh[1] > 1 and st[1] != 1)):
                 raise ValueError(f"block_tables must be int32 [{B}, max_blocks] with contiguous rows")
             if (context_lens is None or context_lens.dtype is not torch.int32 or context_lens.numel() != B
-                    or not context_lens.is_contiguous() or context_lens.device != dev):
+                    or not context_lens.is_contiguous() or context_lens.get_device() != dev):
                 raise ValueError(f"context_lens must be contiguous int32 [{B}]")
-            max_blocks = block_tables.shape[1]
-            table_stride = block_tables.stride(0) if B > 1 else max(max_blocks, block_tables.stride(0))
+            max_blocks = sh[1]
+            table_stride = st[0] if B > 1 else max(max_blocks, st[0])
             bt_ptr, ctx_ptr = block_tables.data_ptr(), context_lens.data_ptr()
             most = max_blocks * block_size
         else:
-            if slots.dtype is not torch.int32 or slots.dim() != 1 or not slots.is_contiguous() or slots.device != dev:
+            if slots.dtype is not torch.int32 or slots.dim() != 1 or not slots.is_contiguous() or slots.get_device() != dev:
                 raise ValueError("slots must be a contiguous 1-D int32 tensor")
             if cu_seqlens_slots is None:
                 raise ValueError("slots need cu_seqlens_slots")
             _check_cu("cu_seqlens_slots", cu_seqlens_slots, B, dev)
             most = total_slots = slots.numel()
             sl_ptr, cus_ptr = slots.data_ptr(), cu_seqlens_slots.data_ptr()
-        max_context = most if max_context is None else min(int(max_context), most)
-    else:
-        max_context = 0
-    if softmax_scale is None:
-        softmax_scale = D ** -0.5
+        if max_context is not None:
+            most = min(int(max_context), most)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = torch.empty_like(q)
+        o_str = out.stride(0)
     else:
-        _check_rows("out", out, Hq, D)
-        if out.shape[0] != q.shape[0] or out.device != dev:
-            raise ValueError("out must have as many rows as q, on its device")
-    lib = _native.lib()
-    max_q = int(max_seqlen_q)
-    with _on_device(dev):
-        key = (fmt, B, Hq, Hkv, max_q, max_context, max_fresh, dev.index)
-        ws_bytes = _CHUNK_WS.get(key)
-        if ws_bytes is None:
-            ws_bytes = lib.dllm_attn_chunk_workspace(fmt, B, Hq, Hkv, max_q, max_context, max_fresh)
-            if len(_CHUNK_WS) > 4096:
-                _CHUNK_WS.clear()
-            _CHUNK_WS[key] = ws_bytes
-        # allocated per call on the current stream, so overlapping launches never share it
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
-        rc = lib.dllm_attn_chunk_fwd(
-            q.data_ptr(), q.stride(0), k_ptr, k_str, v_ptr, v_str, kc_ptr, vc_ptr, kx_ptr, vx_ptr, fmt, num_slots,
-            bt_ptr, table_stride, max_blocks, block_size, ctx_ptr, sl_ptr, cus_ptr, total_slots, max_context,
-            out.data_ptr(), out.stride(0), cu_seqlens_q.data_ptr(), cu_k_ptr, B, max_q, max_fresh, q.shape[0], total_k,
-            Hq, Hkv, D, softmax_scale, causal, None if ws is None else ws.data_ptr(), ws_bytes, _status_ptr(dev),
-            _stream_ptr())
-    if rc:
-        _native.check(rc, "chunk_attention")
+        Ho, Do, o_str = _chunk_rows("out", out)
+        if Ho != Hq or Do != D or out.shape[0] != q.shape[0] or out.get_device() != dev:
+            raise ValueError("out must have q's shape, on its device")
+    args = (fmt, B, Hq, Hkv, max_q, most, max_fresh)
+    if min(args) < 0 or max(args) >= 1 << 31 or max_blocks >= 1 << 31 or block_size >= 1 << 31:
+        raise ValueError(f"sizes out of range: {args}")
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            launches = _chunk_launch(
+                dev, args, out, (q.data_ptr(), q_str, k_ptr, k_str, v_ptr, v_str, kc_ptr, vc_ptr, kx_ptr, vx_ptr, num_slots, bt_ptr,
+                                 table_stride, ctx_ptr, sl_ptr, cus_ptr, total_slots, out.data_ptr(), o_str,
+                                 cu_seqlens_q.data_ptr(), cu_k_ptr, q.shape[0], total_k),
+                max_blocks, block_size, D, causal, softmax_scale)
+    else:
+        launches = _chunk_launch(
+            dev, args, out, (q.data_ptr(), q_str, k_ptr, k_str, v_ptr, v_str, kc_ptr, vc_ptr, kx_ptr, vx_ptr, num_slots, bt_ptr,
+                             table_stride, ctx_ptr, sl_ptr, cus_ptr, total_slots, out.data_ptr(), o_str,
+                             cu_seqlens_q.data_ptr(), cu_k_ptr, q.shape[0], total_k),
+            max_blocks, block_size, D, causal, softmax_scale)
     if B > 0 and max_q > 0 and q.shape[0] > 0:
-        LAUNCHES[0] += 1 if ws is None else 2
+        LAUNCHES[0] += launches
     return out
 
 
+def _chunk_launch(dev, sizes, out, pointers, max_blocks, block_size, D, causal, softmax_scale) -> int:
+    """Allocates the workspace and calls dllm_attn_chunk_fwd on the current
+    device (``dev``); returns the number of kernels it launches."""
+    lib = _native.lib()
+    fmt, B, Hq, Hkv, max_q, max_context, max_fresh = sizes
+    plan = _CHUNK_WS.get((sizes, dev))
+    if plan is None:
+        need = lib.dllm_attn_chunk_workspace(*sizes)
+        if need < 0:
+            # the launch below would refuse the sizes too; this keeps the message
+            code = _native.DLLM_ERR_UNSUPPORTED if Hkv <= 0 or Hq % max(Hkv, 1) or Hq > 128 * Hkv else _native.DLLM_ERR_INVALID_ARG
+            _native.check(code, "chunk_attention")
+        if len(_CHUNK_WS) > 4096:
+            _CHUNK_WS.clear()
+        plan = _CHUNK_WS[(sizes, dev)] = need
+    # allocated per call on the current stream, so overlapping launches never share it
+    ws = torch.empty(plan, dtype=torch.uint8, device=out.device) if plan > 0 else None
+    rc = lib.dllm_attn_chunk_fwd(_native.CHUNK_ARGS.pack(
+        *pointers, 0 if ws is None else ws.data_ptr(), plan, _status_ptr_of(dev), _stream_ptr(), fmt, max_blocks,
+        block_size, max_context, B, max_q, max_fresh, Hq, Hkv, D, 1 if causal else 0,
+        D ** -0.5 if softmax_scale is None else softmax_scale))
+    if rc:
+        _native.check(rc, "chunk_attention")
+    return 1 if ws is None else 2
+
+
+def _chunk_rows(name, t):
+    """(heads, head_dim, token stride) of a bfloat16 [rows, heads, head_dim] with
+    contiguous heads."""
+    sh, st = t.shape, t.stride()
+    if len(sh) != 3 or t.dtype is not torch.bfloat16 or st[2] != 1 or st[1] != sh[2]:
+        raise ValueError(f"{name} must be bfloat16 [rows, heads, head_dim] with contiguous heads, got {t.dtype} {tuple(sh)}")
+    return sh[1], sh[2], st[0]
+
+
 def _check_cu(name, c, B, dev):
-    if c.dtype is not torch.int32 or c.numel() != B + 1 or not c.is_contiguous() or c.device != dev:
-        raise ValueError(f"{name} must be contiguous int32 [{B + 1}] on {dev}")
+    if c.dtype is not torch.int32 or c.numel() != B + 1 or not c.is_contiguous() or c.get_device() != dev:
+        raise ValueError(f"{name} must be contiguous int32 [{B + 1}] on cuda:{dev}")
 
 
 # ---------------------------------------------------------------------------

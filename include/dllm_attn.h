@@ -192,27 +192,59 @@ DLLM_API int dllm_load_kvcache_quant(void* key, int64_t key_stride, void* value,
  * rows are num_kv_heads * 128 elements, num_slots of them. Slots or blocks out of range
  * read as zero rows and flag DLLM_DEV_SLOT_OUT_OF_RANGE; lengths or offsets outside
  * their buffers or bounds are cut there and flag DLLM_DEV_BAD_SEQUENCE.
- * q, o: [total_q, num_heads, 128]; head_dim must be 128; max_seqlen_q bounds every Lq.
+ * q, o: [total_q, num_heads, 128]; head_dim must be 128; num_heads a multiple of, and at
+ * most 128 times, num_kv_heads; max_seqlen_q bounds every Lq.
  *
  * workspace: device memory of at least dllm_attn_chunk_workspace(...) bytes, 16-byte
  * aligned, whose contents need not be set; null if that is 0. Launches that may overlap
  * need distinct ones. The result does not depend on the launch's timing (splits are
  * merged in order).
  */
+typedef struct dllm_chunk_args {
+  const void* q;                    /* bf16 [total_q, num_heads, 128] */
+  int64_t q_tok_stride;
+  const void* k;                    /* fresh rows, or null */
+  int64_t k_tok_stride;
+  const void* v;
+  int64_t v_tok_stride;
+  const void* k_cache;              /* num_slots rows of num_kv_heads * 128 elements */
+  const void* v_cache;
+  const void* k_exp;
+  const void* v_exp;
+  int64_t num_slots;
+  const int32_t* block_tables;
+  int64_t table_stride;
+  const int32_t* context_lens;
+  const int32_t* slots;
+  const int32_t* cu_seqlens_slots;
+  int64_t total_slots;
+  void* o;                          /* bf16 [total_q, num_heads, 128] */
+  int64_t o_tok_stride;
+  const int32_t* cu_seqlens_q;      /* int32 [batch + 1] */
+  const int32_t* cu_seqlens_k;
+  int64_t total_q;
+  int64_t total_k;
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t* err_flag;
+  void* stream;
+  int32_t format;
+  int32_t max_blocks;
+  int32_t block_size;
+  int32_t max_context;
+  int32_t batch;
+  int32_t max_seqlen_q;
+  int32_t max_fresh;
+  int32_t num_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t causal;
+  float softmax_scale;
+} dllm_chunk_args;
+
 DLLM_API int64_t dllm_attn_chunk_workspace(int format, int batch, int num_heads, int num_kv_heads,
                                            int max_seqlen_q, int max_context, int max_fresh);
-DLLM_API int dllm_attn_chunk_fwd(const void* q, int64_t q_tok_stride, const void* k, int64_t k_tok_stride,
-                                 const void* v, int64_t v_tok_stride, const void* k_cache,
-                                 const void* v_cache, const void* k_exp, const void* v_exp, int format,
-                                 int64_t num_slots, const int32_t* block_tables, int64_t table_stride,
-                                 int max_blocks, int block_size, const int32_t* context_lens,
-                                 const int32_t* slots, const int32_t* cu_seqlens_slots, int64_t total_slots,
-                                 int max_context, void* o, int64_t o_tok_stride,
-                                 const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int batch,
-                                 int max_seqlen_q, int max_fresh, int64_t total_q, int64_t total_k,
-                                 int num_heads, int num_kv_heads, int head_dim, float softmax_scale,
-                                 int causal, void* workspace, int64_t workspace_bytes, int32_t* err_flag,
-                                 void* stream);
+DLLM_API int dllm_attn_chunk_fwd(const dllm_chunk_args* args);
 
 /*
  * Non-causal varlen attention, bf16 in/out, fp32 accumulation:

@@ -4,7 +4,6 @@ The reference reads the same cache (the values its codes stand for), so the
 only errors are those of the operator's own roundings; the bound per output
 element is derived in ``oracle.kv_quant_ref.attention_bound``.
 """
-import ctypes
 import math
 
 import pytest
@@ -486,29 +485,32 @@ def test_refusals():
     lib = _native.lib()
 
     def call(**kw):
-        a = dict(q=64, qs=512, k=None, ks=0, v=None, vs=0, kc=64, vc=64, ke=64, ve=64, fmt=1, slots_n=64, bt=64, bts=4,
-                 mb=4, bs=16, ctx=64, sl=None, cus=None, ts=0, mc=64, o=64, os=512, cuq=64, cuk=None, B=1, mq=1, mf=0,
-                 tq=1, tk=0, hq=4, hkv=4, hd=128, sc=ctypes.c_float(0.1), ca=1, ws=None, wb=0)
+        a = dict(q=64, qs=512, k=0, ks=0, v=0, vs=0, kc=64, vc=64, ke=64, ve=64, slots_n=64, bt=64, bts=4, ctx=64, sl=0,
+                 cus=0, ts=0, o=64, os=512, cuq=64, cuk=0, tq=1, tk=0, ws=0, wb=0, err=0, stream=0, fmt=1, mb=4, bs=16,
+                 mc=64, B=1, mq=1, mf=0, hq=4, hkv=4, hd=128, ca=1, sc=0.1)
         a.update(kw)
-        return lib.dllm_attn_chunk_fwd(*a.values(), None, None)
+        return lib.dllm_attn_chunk_fwd(_native.CHUNK_ARGS.pack(*a.values()))
 
     E = _native
     assert call(hd=64) == E.DLLM_ERR_UNSUPPORTED
     assert call(fmt=3) == E.DLLM_ERR_UNSUPPORTED
     assert call(hq=6) == E.DLLM_ERR_UNSUPPORTED
+    assert call(hq=4 * 129, qs=4 * 129 * 128) == E.DLLM_ERR_UNSUPPORTED
+    assert lib.dllm_attn_chunk_fwd(None) == E.DLLM_ERR_INVALID_ARG
+    assert _native.CHUNK_ARGS.size == 27 * 8 + 12 * 4
     assert call(B=-1) == E.DLLM_ERR_INVALID_ARG
-    assert call(sc=ctypes.c_float(0.0)) == E.DLLM_ERR_INVALID_ARG
-    assert call(sc=ctypes.c_float(math.nan)) == E.DLLM_ERR_INVALID_ARG
+    assert call(sc=0.0) == E.DLLM_ERR_INVALID_ARG
+    assert call(sc=math.nan) == E.DLLM_ERR_INVALID_ARG
     assert call(sl=64, cus=64) == E.DLLM_ERR_INVALID_ARG       # tables and a slot list
-    assert call(ctx=None) == E.DLLM_ERR_INVALID_ARG
+    assert call(ctx=0) == E.DLLM_ERR_INVALID_ARG
     assert call(bs=0) == E.DLLM_ERR_INVALID_ARG
     assert call(bts=3) == E.DLLM_ERR_INVALID_ARG
-    assert call(bt=None, sl=64) == E.DLLM_ERR_INVALID_ARG      # slots without offsets
-    assert call(kc=None) == E.DLLM_ERR_INVALID_ARG
-    assert call(ke=None) == E.DLLM_ERR_INVALID_ARG
+    assert call(bt=0, sl=64) == E.DLLM_ERR_INVALID_ARG      # slots without offsets
+    assert call(kc=0) == E.DLLM_ERR_INVALID_ARG
+    assert call(ke=0) == E.DLLM_ERR_INVALID_ARG
     assert call(kc=72) == E.DLLM_ERR_ALIGNMENT
     assert call(k=64) == E.DLLM_ERR_INVALID_ARG                # k without v
-    assert call(cuq=None) == E.DLLM_ERR_INVALID_ARG
+    assert call(cuq=0) == E.DLLM_ERR_INVALID_ARG
     assert call(q=72) == E.DLLM_ERR_ALIGNMENT
     assert call(qs=516) == E.DLLM_ERR_ALIGNMENT
     assert call(os=500) == E.DLLM_ERR_INVALID_ARG
