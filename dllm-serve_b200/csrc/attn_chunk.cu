@@ -27,17 +27,23 @@
 // ring of stages filled by cp.async, so the main loop has no CTA barrier. The
 // warps' partial results are merged in shared memory in a fixed order; splits
 // are merged by a second kernel, also in a fixed order. Products are
-// mma.sync m16n8k16: at one to 32 rows per KV head a launch reads
-// 256 (K) + 256 (V) bytes per bf16 key for at most 32 x 512 operations, below
-// what this instruction sustains, and its operands go straight from
-// shared memory to registers, where codes are expanded.
+// mma.sync m16n8k16: at up to 16 rows per KV head a launch reads 512 bytes per
+// bf16 key for at most 16 x 512 operations, below what this instruction
+// sustains, and its operands go straight from shared memory to registers,
+// where codes are expanded. (At 32 rows it took 62 us where the tcgen05
+// kernel takes 54: 8 sequences, 32 heads, 1,144 e4m3 rows.)
 //
-// Operand layout: the reduction order over head dimensions and over keys is
-// free as long as both operands agree, and so is the order of output columns.
-// Thread (g, t) of a warp (g = lane / 4, t = lane % 4) takes dimensions
-// 16t .. 16t+15 and 64+16t .. 64+16t+15 of key g for the scores (two 16-byte
-// reads of codes), and dimensions 16g .. 16g+15 of keys 2t, 2t+1, 2t+8, 2t+9
-// for the outputs, whose column n of tile j is then dimension 16n + j.
+// Operand layout: keys (scores) and dimensions (outputs) take the products' 16
+// rows and the packed query rows their 8 columns, so eight rows leave nothing
+// idle and need half the accumulators of the other way round. The reduction
+// order over head dimensions and over keys is free as long as both operands
+// agree, and so is the order of the outputs' dimensions. Thread (g, t) of a
+// warp (g = lane / 4, t = lane % 4) takes dimensions 16t .. 16t+15 and
+// 64+16t .. 64+16t+15 of keys g and g + 8 for the scores (two 16-byte reads of
+// codes a key), and dimensions 16g .. 16g+15 of keys 2t, 2t+1, 2t+8, 2t+9 for
+// the outputs: rows g and g + 8 of output tile j are dimensions 16g + 2j and
+// 16g + 2j + 1. Probabilities get from the scores' layout to the second
+// operand's by an 8x8 transpose across the warp.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -55,25 +61,32 @@ namespace {
 constexpr int kD = 128;
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kStages = 3;
 constexpr uint32_t kStageBytes = 8192;  // K half then V half
 constexpr int kFreshKeys = 16;          // keys of a bf16 chunk
+constexpr uint32_t kScaleBytes = 34 * 8;  // of a stage: 32 (K, V) scales, the largest exponent
+constexpr int kNoExp = -(1 << 30);        // no value exponent met
 
 template <int kFmt>
 constexpr int chunk_keys() { return kFmt == kFmtBf16 ? 16 : 32; }
 
-constexpr uint32_t kOffStages = 0;
-constexpr uint32_t kOffScales = kOffStages + kWarps * kStages * kStageBytes;
-constexpr uint32_t kScaleBytes = 34 * 8;                               // 32 (K, V) scales, the largest exponent
-constexpr uint32_t kOffRowFactor = kOffScales + kWarps * kStages * kScaleBytes;  // float per packed row
-constexpr uint32_t kOffQ = kOffRowFactor + 32 * 4;
-constexpr int kNoExp = -(1 << 30);      // no value exponent met
-
-template <int kMT>
-constexpr uint32_t smem_bytes() { return kOffQ + kMT * 16 * kD * 2; }
-static_assert(2 * (smem_bytes<2>() + 1024) <= 233472, "two CTAs do not fit an SM");
-// the merge buffers (per warp: rows x 128 floats, then rows float2) reuse the stages
-static_assert(kWarps * (32 * kD * 4 + 32 * 8) <= kWarps * kStages * kStageBytes, "merge buffers exceed the stages");
+// A quantised chunk is bound by the latency of its conversions and products
+// (issue slots 36 % used with eight warps an SM), a bf16 chunk by bytes in
+// flight. Eight e4m3 contexts of 16,384 rows, 32 heads: two CTAs of three
+// stages 253 us, three CTAs of two 197 us; bf16 contexts of 4,096 rows, 28/4
+// heads: 54 and 66 us.
+template <int kFmt>
+struct Cfg {
+  static constexpr int kStages = kFmt == kFmtBf16 ? 3 : 2;
+  static constexpr int kCtas = kFmt == kFmtBf16 ? 2 : 3;  // per SM
+  static constexpr uint32_t kOffStages = 0;
+  static constexpr uint32_t kOffScales = kOffStages + kWarps * kStages * kStageBytes;
+  static constexpr uint32_t kOffRowFactor = kOffScales + kWarps * kStages * kScaleBytes;  // float per packed row
+  static constexpr uint32_t kOffQ = kOffRowFactor + 16 * 4;
+  static constexpr uint32_t kSmemBytes = kOffQ + 16 * kD * 2;
+  static_assert(kCtas * (kSmemBytes + 1024) <= 233472, "the CTAs do not fit an SM");
+  // the merge buffers (per warp: rows x 128 floats, then rows float2) reuse the stages
+  static_assert(kWarps * (16 * kD * 4 + 16 * 8) <= kWarps * kStages * kStageBytes, "merge buffers exceed the stages");
+};
 
 DLLM_DEVICE void cp_async16(uint32_t dst, const void* src, bool live) {
   const int n = live ? 16 : 0;  // 0: the 16 bytes are filled with zeros, nothing is read
@@ -150,101 +163,78 @@ DLLM_DEVICE uint32_t v_unit(uint32_t unit, uint32_t key) {
 
 }  // namespace
 
-// Running state of a warp's rows: thread (g, t) holds rows 8 r + g of its
-// 16-row tiles, r < kR (kR = 1: the tile has at most eight rows, so the upper
-// half of every product is idle and its softmax is left out).
-template <int kMT, int kR>
+// Running state of a warp: thread (g, t) holds packed rows 8n + 2t and 8n + 2t + 1,
+// n < kN (all eight lanes of equal t hold the same m).
+template <int kN>
 struct Rows {
-  float m[kMT][kR];          // running maximum, log2 units
-  float l[kMT][kR];          // sum of this thread's columns
-  float rf[kMT][kR];         // score of a product: times this (log2 units)
-  int seen[kMT][kR];         // keys the row sees, from the sequence's first
-  float o[kMT][16][4];
-  int e;                     // O is in units of 2^(e - 15) (quantised caches)
+  float m[kN][2];        // running maximum, log2 units
+  float l[kN][2];        // sum over this thread's keys
+  float rf[kN][2];       // score of a product: times this (log2 units)
+  int seen[kN][2];       // keys the row sees, from the sequence's first
+  float o[8][kN][4];     // dimensions 16g + 2j, 16g + 2j + 1 of both rows
+  int e;                 // O is in units of 2^(e - 15) (quantised caches)
 };
+
+// The 8x8 matrix of 16-bit values whose row g the lanes 4g .. 4g+3 hold, transposed.
+DLLM_DEVICE uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 
 // Products, softmax and products of one chunk of KB keys in shared memory. A
 // row sees the chunk's first min(seen, end) - pos keys; `whole`: all of them,
-// for every row. kQuant: the kernel's cache is quantised (Q is f16, O scaled),
-// kFmt: the format of this chunk (its fresh chunks are bf16).
-template <bool kQuant, int kFmt, int kMT, int kR>
-DLLM_DEVICE void chunk_step(uint32_t ks, uint32_t vs, uint32_t scales, uint32_t qs, const uint32_t (&qf)[8][4],
-                            int lane, float sl2, bool whole, int pos, int end, Rows<kMT, kR>& w) {
+// for every row. kQuant: the kernel's cache is quantised (Q is f16 with a
+// factor `back` for row 8n + g, O scaled), kFmt: the format of this chunk (its
+// fresh chunks are bf16).
+template <bool kQuant, int kFmt, int kN>
+DLLM_DEVICE void chunk_step(uint32_t ks, uint32_t vs, uint32_t scales, const uint32_t (&qf)[kN][16],
+                            const float (&back)[kN], int lane, float sl2, bool whole, int pos, int end, Rows<kN>& w) {
   constexpr int KB = chunk_keys<kFmt>();
-  constexpr int NT = KB / 8;
+  constexpr int KT = KB / 16;  // 16-key tiles
   constexpr bool kCodes = kFmt != kFmtBf16;
   constexpr uint32_t kRow = kCodes ? 128 : 256;  // bytes of a key's row
   const int g = lane >> 2, t = lane & 3;
-  float s[kMT][NT][4];
+  float s[KT][kN][4];
 #pragma unroll
-  for (int mt = 0; mt < kMT; ++mt)
+  for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < kN; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[mt][n][e] = 0.f;
-  // what a product of this chunk is multiplied by: a fresh chunk's Q is the f16 Q brought back to bf16
-  float rf[kMT][kR], back[kMT][2] = {};
-#pragma unroll
-  for (int mt = 0; mt < kMT; ++mt)
-#pragma unroll
-    for (int r = 0; r < kR; ++r) {
-      rf[mt][r] = kQuant && !kCodes ? sl2 : w.rf[mt][r];
-      if (kQuant && !kCodes) back[mt][r] = w.rf[mt][r] / sl2;
-    }
+      for (int e = 0; e < 4; ++e) s[kt][n][e] = 0.f;
   // scores: half h covers dimensions 64h + 16t .. + 15 of this thread
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t qa[kMT][4][4];
+  for (int kt = 0; kt < KT; ++kt) {
 #pragma unroll
-    for (int mt = 0; mt < kMT; ++mt) {
-      if constexpr (kMT == 1) {
+    for (int h = 0; h < 2; ++h) {
+      uint32_t ka[2][8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) qa[mt][i][e] = qf[4 * h + i][e];
-      } else {
-#pragma unroll
-        for (int rr = 0; rr < 2; ++rr) {
-          const int row = mt * 16 + rr * 8 + g;
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const uint4 x = lds128(qs + row * 256 + (((8 * h + 2 * t + c) ^ (row & 1)) << 4));
-            qa[mt][2 * c][rr] = x.x, qa[mt][2 * c][2 + rr] = x.y;
-            qa[mt][2 * c + 1][rr] = x.z, qa[mt][2 * c + 1][2 + rr] = x.w;
-          }
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t key = 16 * kt + 8 * e + g;
+        if constexpr (!kCodes) {
+          const uint4 x = lds128(ks + key * kRow + (k_unit<kFmt>(8 * h + 2 * t, key) << 4));
+          const uint4 y = lds128(ks + key * kRow + (k_unit<kFmt>(8 * h + 2 * t + 1, key) << 4));
+          ka[e][0] = x.x, ka[e][1] = x.y, ka[e][2] = x.z, ka[e][3] = x.w;
+          ka[e][4] = y.x, ka[e][5] = y.y, ka[e][6] = y.z, ka[e][7] = y.w;
+        } else {
+          const uint4 x = lds128(ks + key * kRow + (k_unit<kFmt>(4 * h + t, key) << 4));
+          codes_to_f16<kFmt>(x.x, ka[e][0], ka[e][1]);
+          codes_to_f16<kFmt>(x.y, ka[e][2], ka[e][3]);
+          codes_to_f16<kFmt>(x.z, ka[e][4], ka[e][5]);
+          codes_to_f16<kFmt>(x.w, ka[e][6], ka[e][7]);
         }
-      }
-      if constexpr (kQuant && !kCodes) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) qa[mt][i][e] = f16_to_bf16(qa[mt][i][e], back[mt][e & 1]);
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const uint32_t key = 8 * n + g;
-      uint32_t kb[8];
-      if constexpr (!kCodes) {
-        const uint4 x = lds128(ks + key * kRow + (k_unit<kFmt>(8 * h + 2 * t, key) << 4));
-        const uint4 y = lds128(ks + key * kRow + (k_unit<kFmt>(8 * h + 2 * t + 1, key) << 4));
-        kb[0] = x.x, kb[1] = x.y, kb[2] = x.z, kb[3] = x.w;
-        kb[4] = y.x, kb[5] = y.y, kb[6] = y.z, kb[7] = y.w;
-      } else {
-        const uint4 x = lds128(ks + key * kRow + (k_unit<kFmt>(4 * h + t, key) << 4));
-        codes_to_f16<kFmt>(x.x, kb[0], kb[1]);
-        codes_to_f16<kFmt>(x.y, kb[2], kb[3]);
-        codes_to_f16<kFmt>(x.z, kb[4], kb[5]);
-        codes_to_f16<kFmt>(x.w, kb[6], kb[7]);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int mt = 0; mt < kMT; ++mt) {
-          if constexpr (kCodes)
-            mma16816_f16(s[mt][n], qa[mt][i][0], qa[mt][i][1], qa[mt][i][2], qa[mt][i][3], kb[2 * i], kb[2 * i + 1]);
-          else
-            mma16816(s[mt][n], qa[mt][i][0], qa[mt][i][1], qa[mt][i][2], qa[mt][i][3], kb[2 * i], kb[2 * i + 1]);
+        for (int n = 0; n < kN; ++n) {
+          uint32_t b0 = qf[n][8 * h + 2 * i], b1 = qf[n][8 * h + 2 * i + 1];
+          if constexpr (kCodes) {
+            mma16816_f16(s[kt][n], ka[0][2 * i], ka[1][2 * i], ka[0][2 * i + 1], ka[1][2 * i + 1], b0, b1);
+          } else {
+            if constexpr (kQuant) b0 = f16_to_bf16(b0, back[n]), b1 = f16_to_bf16(b1, back[n]);
+            mma16816(s[kt][n], ka[0][2 * i], ka[1][2 * i], ka[0][2 * i + 1], ka[1][2 * i + 1], b0, b1);
+          }
         }
     }
   }
@@ -264,136 +254,133 @@ DLLM_DEVICE void chunk_step(uint32_t ks, uint32_t vs, uint32_t scales, uint32_t 
     if (w.e == kNoExp) w.e = 0;
     ufac = pow2(15 - w.e);
   }
-  // masks and column factors
-  float vsc[NT][2];
+  // masks and key factors: keys 16kt + g, 16kt + 8 + g
+  float vsc[KT][2];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    float k0 = 1.f, k1 = 1.f;
-    vsc[n][0] = vsc[n][1] = ufac;
-    if constexpr (kCodes) {
-      const uint4 x = lds128(scales + (8 * n + 2 * t) * 8);  // (K, V) scales of two keys
-      k0 = __uint_as_float(x.x), k1 = __uint_as_float(x.z);
-      vsc[n][0] *= __uint_as_float(x.y), vsc[n][1] *= __uint_as_float(x.w);
-    }
+  for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-    for (int mt = 0; mt < kMT; ++mt)
-#pragma unroll
-      for (int r = 0; r < kR; ++r) {
-        if constexpr (kCodes) s[mt][n][2 * r] *= k0, s[mt][n][2 * r + 1] *= k1;
-        if (!whole) {
-          const int c = 8 * n + 2 * t, lim = min(w.seen[mt][r], end) - pos;
-          if (c >= lim) s[mt][n][2 * r] = -INFINITY;
-          if (c + 1 >= lim) s[mt][n][2 * r + 1] = -INFINITY;
-        }
+    for (int e = 0; e < 2; ++e) {
+      float k0 = 1.f;
+      vsc[kt][e] = ufac;
+      if constexpr (kCodes) {
+        float v0;
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(k0), "=f"(v0) : "r"(scales + (16 * kt + 8 * e + g) * 8));
+        vsc[kt][e] *= v0;
       }
-  }
-  float alpha[kMT][kR];
+#pragma unroll
+      for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          if constexpr (kCodes) s[kt][n][2 * e + r] *= k0;
+          if (!whole && 16 * kt + 8 * e + g >= min(w.seen[n][r], end) - pos) s[kt][n][2 * e + r] = -INFINITY;
+        }
+    }
+  float alpha[kN][2];
   bool moved = grow != 1.f;
 #pragma unroll
-  for (int mt = 0; mt < kMT; ++mt)
+  for (int n = 0; n < kN; ++n)
 #pragma unroll
-    for (int r = 0; r < kR; ++r) {
+    for (int r = 0; r < 2; ++r) {
+      const float rf = kQuant && !kCodes ? sl2 : w.rf[n][r];
       float mx = -INFINITY;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) mx = max3f(mx, s[mt][n][2 * r], s[mt][n][2 * r + 1]);
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float mn = fmaxf(w.m[mt][r], mx * rf[mt][r]);
+      for (int kt = 0; kt < KT; ++kt) mx = max3f(mx, s[kt][n][r], s[kt][n][2 + r]);
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+      const float mn = fmaxf(w.m[n][r], mx * rf);
       const float base = mn == -INFINITY ? 0.f : mn;  // a row that has seen no key yet
-      moved |= mn > w.m[mt][r];
-      alpha[mt][r] = ex2_approx(w.m[mt][r] - base);
-      w.m[mt][r] = mn;
+      moved |= mn > w.m[n][r];
+      alpha[n][r] = ex2_approx(w.m[n][r] - base);
+      w.m[n][r] = mn;
       float sum = 0.f;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float p = ex2_approx(fmaf(s[mt][n][2 * r + e], rf[mt][r], -base));
+          const float p = ex2_approx(fmaf(s[kt][n][2 * e + r], rf, -base));
           sum += p;
-          s[mt][n][2 * r + e] = kQuant ? p * vsc[n][e] : p;
+          s[kt][n][2 * e + r] = kQuant ? p * vsc[kt][e] : p;
         }
-      w.l[mt][r] = fmaf(w.l[mt][r], alpha[mt][r], sum);
+      w.l[n][r] = fmaf(w.l[n][r], alpha[n][r], sum);
     }
   if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-    for (int mt = 0; mt < kMT; ++mt)
+    for (int n = 0; n < kN; ++n)
 #pragma unroll
-      for (int r = 0; r < kR; ++r) {
-        const float f = alpha[mt][r] * grow;
+      for (int r = 0; r < 2; ++r) {
+        const float f = alpha[n][r] * grow;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) w.o[mt][j][2 * r] *= f, w.o[mt][j][2 * r + 1] *= f;
+        for (int j = 0; j < 8; ++j) w.o[j][n][r] *= f, w.o[j][n][2 + r] *= f;
       }
   }
   // outputs: probabilities are rounded to f16 (see above) or bf16 (2^-8 of their value)
   auto pack = [](float lo, float hi) { return kCodes ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi); };
 #pragma unroll
-    for (int u = 0; u < NT / 2; ++u) {
-      uint32_t pa[kMT][4];
+  for (int u = 0; u < KT; ++u) {
+    uint32_t pb[kN][2];
 #pragma unroll
-      for (int mt = 0; mt < kMT; ++mt)
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) pb[n][e] = transpose8(pack(s[u][n][2 * e], s[u][n][2 * e + 1]));
+    const uint32_t k0 = 16 * u + 2 * t;
+    auto product = [&](int j, const uint32_t (&x)[2], const uint32_t (&y)[2]) {
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+        if constexpr (kCodes)
+          mma16816_f16(w.o[j][n], x[0], y[0], x[1], y[1], pb[n][0], pb[n][1]);
+        else
+          mma16816(w.o[j][n], x[0], y[0], x[1], y[1], pb[n][0], pb[n][1]);
+      }
+    };
+    if constexpr (!kCodes) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {  // eight dimensions of this thread at a time
+        uint32_t vb[8][2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float* x = s[mt][2 * u + e];
-          pa[mt][2 * e] = pack(x[0], x[1]);
-          pa[mt][2 * e + 1] = kR == 2 ? pack(x[2], x[3]) : 0u;
-        }
-      const uint32_t k0 = 16 * u + 2 * t;
-      auto product = [&](int j, uint32_t b0, uint32_t b1) {
+          const uint32_t ka = k0 + 8 * e, kb = ka + 1;
+          const uint4 x = lds128(vs + ka * kRow + (v_unit<kFmt>(2 * g + c, ka) << 4));
+          const uint4 y = lds128(vs + kb * kRow + (v_unit<kFmt>(2 * g + c, kb) << 4));
+          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-        for (int mt = 0; mt < kMT; ++mt) {
-          if constexpr (kCodes)
-            mma16816_f16(w.o[mt][j], pa[mt][0], pa[mt][1], pa[mt][2], pa[mt][3], b0, b1);
-          else
-            mma16816(w.o[mt][j], pa[mt][0], pa[mt][1], pa[mt][2], pa[mt][3], b0, b1);
-        }
-      };
-      if constexpr (!kCodes) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {  // eight output columns of this thread at a time
-          uint32_t vb[8][2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t ka = k0 + 8 * e, kb = ka + 1;
-            const uint4 x = lds128(vs + ka * kRow + (v_unit<kFmt>(2 * g + c, ka) << 4));
-            const uint4 y = lds128(vs + kb * kRow + (v_unit<kFmt>(2 * g + c, kb) << 4));
-            const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              vb[2 * i][e] = __byte_perm(xs[i], ys[i], 0x5410);
-              vb[2 * i + 1][e] = __byte_perm(xs[i], ys[i], 0x7632);
-            }
+          for (int i = 0; i < 4; ++i) {
+            vb[2 * i][e] = __byte_perm(xs[i], ys[i], 0x5410);
+            vb[2 * i + 1][e] = __byte_perm(xs[i], ys[i], 0x7632);
           }
-#pragma unroll
-          for (int j = 0; j < 8; ++j) product(8 * c + j, vb[j][0], vb[j][1]);
-        }
-      } else {
-        uint32_t x[4][4];  // codes of keys 2t, 2t + 1, 2t + 8, 2t + 9: 16 dimensions each
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t key = k0 + (i >> 1) * 8 + (i & 1);
-          const uint4 y = lds128(vs + key * kRow + (v_unit<kFmt>(g, key) << 4));
-          x[i][0] = y.x, x[i][1] = y.y, x[i][2] = y.z, x[i][3] = y.w;
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t vb[4][2];
+        for (int j = 0; j < 4; ++j) product(4 * c + j, vb[2 * j], vb[2 * j + 1]);
+      }
+    } else {
+      uint32_t x[4][4];  // codes of keys 2t, 2t + 1, 2t + 8, 2t + 9: 16 dimensions each
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            codes_to_f16<kFmt>(__byte_perm(x[2 * e][i], x[2 * e + 1][i], 0x5140), vb[0][e], vb[1][e]);
-            codes_to_f16<kFmt>(__byte_perm(x[2 * e][i], x[2 * e + 1][i], 0x7362), vb[2][e], vb[3][e]);
-          }
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t key = k0 + (i >> 1) * 8 + (i & 1);
+        const uint4 y = lds128(vs + key * kRow + (v_unit<kFmt>(g, key) << 4));
+        x[i][0] = y.x, x[i][1] = y.y, x[i][2] = y.z, x[i][3] = y.w;
+      }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) product(4 * i + j, vb[j][0], vb[j][1]);
+      for (int i = 0; i < 4; ++i) {
+        uint32_t vb[4][2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          codes_to_f16<kFmt>(__byte_perm(x[2 * e][i], x[2 * e + 1][i], 0x5140), vb[0][e], vb[1][e]);
+          codes_to_f16<kFmt>(__byte_perm(x[2 * e][i], x[2 * e + 1][i], 0x7362), vb[2][e], vb[3][e]);
         }
+        product(2 * i, vb[0], vb[1]);
+        product(2 * i + 1, vb[2], vb[3]);
       }
     }
+  }
 }
 
-template <int kFmt, int kMT, int kR>
-__global__ void __launch_bounds__(kThreads, 2) attn_chunk_kernel(const __grid_constant__ ChunkArgs a) {
+template <int kFmt, int kN>
+__global__ void __launch_bounds__(kThreads, Cfg<kFmt>::kCtas) attn_chunk_kernel(const __grid_constant__ ChunkArgs a) {
   constexpr int KB = chunk_keys<kFmt>();
-  constexpr int kRows = kMT == 1 ? 8 * kR : 16 * kMT;  // packed rows of a tile
-  constexpr int kQRows = 16 * kMT;
+  using C = Cfg<kFmt>;
+  constexpr int kStages = C::kStages;
+  constexpr int kRows = 8 * kN;  // packed rows of a tile
   constexpr bool kQuant = kFmt != kFmtBf16;
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
@@ -416,8 +403,8 @@ __global__ void __launch_bounds__(kThreads, 2) attn_chunk_kernel(const __grid_co
   if (split > 0 && c_begin >= c_end) return;  // this split has no keys (split 0 writes empty rows)
 
   // ------------------------------------------------------------ key chunks
-  const uint32_t stage0 = base + kOffStages + warp * (kStages * kStageBytes);
-  const uint32_t scale0 = base + kOffScales + warp * (kStages * kScaleBytes);
+  const uint32_t stage0 = base + C::kOffStages + warp * (kStages * kStageBytes);
+  const uint32_t scale0 = base + C::kOffScales + warp * (kStages * kScaleBytes);
   const int n_mine = c_begin + warp < c_end ? (c_end - c_begin - warp + kWarps - 1) / kWarps : 0;
   const int64_t row_bytes = (int64_t)a.Hkv * (kQuant ? kD : 2 * kD);  // a cache slot
   const uint8_t* kc = a.kc + (int64_t)hkv * (kQuant ? kD : 2 * kD);
@@ -513,10 +500,10 @@ __global__ void __launch_bounds__(kThreads, 2) attn_chunk_kernel(const __grid_co
   }
 
   // Q rows, packed and swizzled (zero past the tile's rows); f16 with a row factor if the cache is quantised
-  for (int i = threadIdx.x; i < kQRows * 16; i += kThreads) {
+  for (int i = threadIdx.x; i < kRows * 16; i += kThreads) {
     const int p = i >> 4, u = i & 15;
     uint4 x = make_uint4(0, 0, 0, 0);
-    if (p < rows && p < kRows) {
+    if (p < rows) {
       const int r = (row0 + p) / a.group, h = hkv * a.group + (row0 + p) - r * a.group;
       x = __ldg(reinterpret_cast<const uint4*>(a.q + (sq.q_begin + r) * a.q_stride + (int64_t)h * kD) + u);
     }
@@ -534,47 +521,40 @@ __global__ void __launch_bounds__(kThreads, 2) attn_chunk_kernel(const __grid_co
       x = make_uint4(pack_f16x2(y[0] * f, y[1] * f), pack_f16x2(y[2] * f, y[3] * f), pack_f16x2(y[4] * f, y[5] * f),
                      pack_f16x2(y[6] * f, y[7] * f));
       if (u == 0)
-        asm volatile("st.shared.f32 [%0], %1;" ::"r"(base + kOffRowFactor + p * 4), "f"(pow2(-up)) : "memory");
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(base + C::kOffRowFactor + p * 4), "f"(pow2(-up)) : "memory");
     }
-    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(base + kOffQ + p * 256 + ((u ^ (p & 1)) << 4)),
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(base + C::kOffQ + p * 256 + ((u ^ (p & 1)) << 4)),
                  "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w)
                  : "memory");
   }
   __syncthreads();
-  uint32_t qf[8][4] = {};
-  if constexpr (kMT == 1) {
-#pragma unroll
-    for (int rr = 0; rr < kR; ++rr)
-#pragma unroll
-      for (int hc = 0; hc < 4; ++hc) {
-        const int row = rr * 8 + g, unit = 8 * (hc >> 1) + 2 * t + (hc & 1);
-        const uint4 x = lds128(base + kOffQ + row * 256 + ((unit ^ (row & 1)) << 4));
-        qf[2 * hc][rr] = x.x, qf[2 * hc][2 + rr] = x.y;
-        qf[2 * hc + 1][rr] = x.z, qf[2 * hc + 1][2 + rr] = x.w;
-      }
-  }
+  uint32_t qf[kN][16];
+  float back[kN];
   const int64_t L = (int64_t)sq.nc + sq.nk;
-  Rows<kMT, kR> w;
+  Rows<kN> w;
 #pragma unroll
-  for (int mt = 0; mt < kMT; ++mt) {
+  for (int n = 0; n < kN; ++n) {
+    const int row = 8 * n + g;
 #pragma unroll
-    for (int r = 0; r < kR; ++r) {
-      const int p = mt * 16 + r * 8 + g;
+    for (int hc = 0; hc < 4; ++hc) {
+      const uint4 x = lds128(base + C::kOffQ + row * 256 + (((8 * (hc >> 1) + 2 * t + (hc & 1)) ^ (row & 1)) << 4));
+      qf[n][4 * hc] = x.x, qf[n][4 * hc + 1] = x.y, qf[n][4 * hc + 2] = x.z, qf[n][4 * hc + 3] = x.w;
+    }
+    const float* factor = reinterpret_cast<const float*>(smem + C::kOffRowFactor);
+    back[n] = kQuant ? factor[row] : 1.f;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int p = 8 * n + 2 * t + r;
       const int i = (row0 + p) / a.group;
-      w.m[mt][r] = -INFINITY;
-      w.l[mt][r] = 0.f;
-      w.seen[mt][r] = (int)(a.causal ? min(L, max((int64_t)0, L - sq.Lq + i + 1)) : L);
-      w.rf[mt][r] = a.scale_log2;
-      if constexpr (kQuant) {
-        float f;
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(base + kOffRowFactor + p * 4));
-        w.rf[mt][r] *= f;
-      }
+      w.m[n][r] = -INFINITY;
+      w.l[n][r] = 0.f;
+      w.seen[n][r] = (int)(a.causal ? min(L, max((int64_t)0, L - sq.Lq + i + 1)) : L);
+      w.rf[n][r] = kQuant ? a.scale_log2 * factor[p] : a.scale_log2;
     }
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
+    for (int j = 0; j < 8; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w.o[mt][j][e] = 0.f;
+      for (int e = 0; e < 4; ++e) w.o[j][n][e] = 0.f;
   }
   w.e = kNoExp;
   const int seen_by_all = (int)(a.causal ? min(L, max((int64_t)0, L - sq.Lq + row0 / a.group + 1)) : L);
@@ -590,11 +570,11 @@ __global__ void __launch_bounds__(kThreads, 2) attn_chunk_kernel(const __grid_co
     const uint32_t sc = scale0 + (i % kStages) * kScaleBytes;
     if (c < sp.cached) {
       const int pos = c * KB;
-      chunk_step<kQuant, kFmt, kMT, kR>(st, st + kStageBytes / 2, sc, base + kOffQ, qf, lane, a.scale_log2,
+      chunk_step<kQuant, kFmt, kN>(st, st + kStageBytes / 2, sc, qf, back, lane, a.scale_log2,
                                         min(seen_by_all, sq.nc) - pos >= KB, pos, sq.nc, w);
     } else {
       const int pos = sq.nc + (c - sp.cached) * kFreshKeys;
-      chunk_step<kQuant, kFmtBf16, kMT, kR>(st, st + kStageBytes / 2, sc, base + kOffQ, qf, lane, a.scale_log2,
+      chunk_step<kQuant, kFmtBf16, kN>(st, st + kStageBytes / 2, sc, qf, back, lane, a.scale_log2,
                                             seen_by_all - pos >= kFreshKeys, pos, (int)L, w);
     }
   }
@@ -606,24 +586,20 @@ __global__ void __launch_bounds__(kThreads, 2) attn_chunk_kernel(const __grid_co
   float2* ml = reinterpret_cast<float2*>(smem + kWarps * kRows * kD * 4);  // [warp][row]
   const float unit = !kQuant ? 1.f : w.e == kNoExp ? 0.f : pow2(w.e - 15);
 #pragma unroll
-  for (int mt = 0; mt < kMT; ++mt)
+  for (int n = 0; n < kN; ++n)
 #pragma unroll
-    for (int r = 0; r < kR; ++r) {
-      const int row = mt * 16 + r * 8 + g;
-      float sum = w.l[mt][r];
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      if (t == 0) ml[warp * kRows + row] = make_float2(w.m[mt][r], sum);
-      // column n of tile j is dimension 16n + j: this thread's n are 2t, 2t + 1
-      float* dst = mo + ((size_t)warp * kRows + row) * kD;
+    for (int r = 0; r < 2; ++r) {
+      const int row = 8 * n + 2 * t + r;
+      float sum = w.l[n][r];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+      if (g == 0) ml[warp * kRows + row] = make_float2(w.m[n][r], sum);
+      float* dst = mo + ((size_t)warp * kRows + row) * kD + 16 * g;
 #pragma unroll
-      for (int j = 0; j < 16; j += 4)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int x = 2 * r + e;
-          *reinterpret_cast<float4*>(dst + 32 * t + 16 * e + j) =
-              make_float4(w.o[mt][j][x] * unit, w.o[mt][j + 1][x] * unit, w.o[mt][j + 2][x] * unit, w.o[mt][j + 3][x] * unit);
-        }
+      for (int j = 0; j < 8; j += 2)
+        *reinterpret_cast<float4*>(dst + 2 * j) = make_float4(w.o[j][n][r] * unit, w.o[j][n][2 + r] * unit,
+                                                              w.o[j + 1][n][r] * unit, w.o[j + 1][n][2 + r] * unit);
     }
   __syncthreads();
   const bool alone = sp.total <= a.split_chunks;  // no other split has keys of this tile
@@ -763,31 +739,30 @@ __global__ void __launch_bounds__(256) expand_rows_kernel(const __grid_constant_
   v_out[o + 1] = make_uint4(v[4], v[5], v[6], v[7]);
 }
 
-template <int kFmt, int kMT, int kR>
+template <int kFmt, int kN>
 cudaError_t launch(const ChunkArgs& a, cudaStream_t stream) {
   static std::atomic<bool> attr_set[64];
-  constexpr int kRows = kMT == 1 ? 8 * kR : 16 * kMT;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-    e = cudaFuncSetAttribute(attn_chunk_kernel<kFmt, kMT, kR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)smem_bytes<kMT>());
+    e = cudaFuncSetAttribute(attn_chunk_kernel<kFmt, kN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)Cfg<kFmt>::kSmemBytes);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
   const int64_t items = (int64_t)a.B * a.Hkv * a.mtiles;
   if (items * a.splits > 0x7fffffffLL) return cudaErrorInvalidValue;
-  e = launch_pdl(attn_chunk_kernel<kFmt, kMT, kR>, dim3((unsigned)(items * a.splits)), dim3(kThreads),
-                 smem_bytes<kMT>(), stream, a);
+  e = launch_pdl(attn_chunk_kernel<kFmt, kN>, dim3((unsigned)(items * a.splits)), dim3(kThreads),
+                 Cfg<kFmt>::kSmemBytes, stream, a);
   if (e != cudaSuccess || a.splits == 1) return e;
-  return launch_pdl(attn_chunk_merge_kernel<chunk_keys<kFmt>(), kFreshKeys, kRows>,
-                    dim3((unsigned)((items * kRows + 7) / 8)), dim3(256), 0, stream, a);
+  return launch_pdl(attn_chunk_merge_kernel<chunk_keys<kFmt>(), kFreshKeys, 8 * kN>,
+                    dim3((unsigned)(items * kN)), dim3(256), 0, stream, a);
 }
 
 template <int kFmt>
 cudaError_t launch_rows(const ChunkArgs& a, int rows, cudaStream_t stream) {
-  return rows == 8 ? launch<kFmt, 1, 1>(a, stream) : rows == 16 ? launch<kFmt, 1, 2>(a, stream) : launch<kFmt, 2, 2>(a, stream);
+  return rows == 8 ? launch<kFmt, 1>(a, stream) : launch<kFmt, 2>(a, stream);
 }
 
 }  // namespace chunk
@@ -833,16 +808,24 @@ ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int 
   const int kb = format == kFmtBf16 ? 16 : 32;
   const int64_t chunks = ((int64_t)max_context + kb - 1) / kb + ((int64_t)max_fresh + 15) / 16;
   const int64_t items = (int64_t)B * Hkv * p.mtiles;
-  // Two CTAs fit an SM. The keys are split until every SM has its two, as long
-  // as a warp keeps four chunks, and on to four times as many CTAs (batches of
-  // unequal contexts then finish together) as long as a warp keeps 16. Eight
-  // e4m3 contexts of 4,096-32,768 rows, 32 heads: 366 us with the SMs filled
-  // once, 270 us four times, 268 us eight times; one bf16 context of 65,536
-  // rows, 4 KV heads: 36 us once, 67 us four times.
-  const int64_t slots = 2 * (int64_t)num_sms;
-  const int64_t once = items > 0 ? std::min((slots + items - 1) / items, chunks / (4 * chunk::kWarps)) : 1;
-  const int64_t more = items > 0 ? std::min((4 * slots + items - 1) / items, chunks / (16 * chunk::kWarps)) : 1;
-  const int64_t splits = std::max<int64_t>(1, std::max(once, more));
+  // Splits: the count with the least estimated time, in chunks of a warp. A CTA
+  // of c chunks a warp takes c + 3; the launch takes whole waves of CTAs if all
+  // contexts are as long as the bound, and if they are 60 % of it on average
+  // its mean load and the last CTA's tail: the sum of both estimates decides.
+  // The merge costs four chunks and one for 16 splits.
+  const int64_t slots = (int64_t)(format == kFmtBf16 ? chunk::Cfg<kFmtBf16>::kCtas : chunk::Cfg<kFmtE4m3>::kCtas) * num_sms;
+  int64_t splits = 1;
+  double best = 0;
+  for (int64_t s = 1; items > 0 && s <= std::max<int64_t>(1, chunks / chunk::kWarps) && s <= 1024; s += std::max<int64_t>(1, s / 8)) {
+    const int64_t per = (chunks + s - 1) / s;
+    const double cta = (double)((per + chunk::kWarps - 1) / chunk::kWarps) + 3;
+    const double waves = (double)(items * s) / (double)slots;
+    const double cost = cta * (double)((items * s + slots - 1) / slots) + cta * (0.6 * waves + 1) + (s > 1 ? 8 + (double)s / 8 : 0);
+    if (s == 1 || cost < best) {
+      best = cost;
+      splits = s;
+    }
+  }
   p.split_chunks = (int)std::max<int64_t>(1, (chunks + splits - 1) / splits);
   p.splits = (int)std::max<int64_t>(1, (chunks + p.split_chunks - 1) / p.split_chunks);
   p.workspace_bytes = p.splits > 1 ? items * p.splits * p.rows * (chunk::kD * 4 + 8) : 0;
