@@ -48,6 +48,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "common.cuh"
 #include "kvquant.cuh"
@@ -767,8 +768,8 @@ cudaError_t launch_rows(const ChunkArgs& a, int rows, cudaStream_t stream) {
 
 }  // namespace chunk
 
-ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int max_context, int max_fresh,
-                          int num_sms) {
+ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int64_t total_q, int max_context,
+                          int max_fresh, int num_sms) {
   constexpr int kDenseTiles = 4;
   ChunkPlan p = {};
   const int64_t rows = (int64_t)max_q * group;
@@ -795,11 +796,19 @@ ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int 
       p.dense_bytes = bytes;
       p.workspace_bytes += bytes;
     }
-    // Two row tiles per unit where every SM still has one.
-    const int64_t pairs = (rows + 2 * p.tile_rows - 1) / (2 * p.tile_rows);
-    if ((format == kFmtBf16 || p.dense > 0) && p.mtiles >= 2 && (int64_t)B * Hkv * pairs >= num_sms) {
-      p.unit_rows = 2 * p.tile_rows;
-      p.mtiles = (int)pairs;
+    // One or two row tiles per unit (bf16 rows): a KV tile takes a unit of two 1.83 times as long
+    // (2 x 1,024 rows over 2,000, 32 heads: 107 us, one tile 117), but fewer, larger units fill the
+    // SMs less evenly (4 chunks of 300-512 rows, 28/4 heads: 131 us, one tile 113). The better
+    // estimate of rounds x time decides; half the sequences are taken to end inside a tile.
+    if ((format == kFmtBf16 || p.dense > 0) && p.mtiles >= 2 && p.splits == 1) {
+      auto rounds = [&](int64_t unit_rows) {
+        const double n = Hkv * ((double)total_q * group / (double)unit_rows + 0.5 * B) / num_sms;
+        return n > 3 ? n + 0.5 : std::ceil(n);
+      };
+      if (1.83 * rounds(2 * p.tile_rows) < rounds(p.tile_rows)) {
+        p.unit_rows = 2 * p.tile_rows;
+        p.mtiles = (int)((rows + p.unit_rows - 1) / p.unit_rows);
+      }
     }
     return p;
   }

@@ -74,8 +74,9 @@ struct ChunkPlan {
   int64_t workspace_bytes;
 };
 
-ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int max_context, int max_fresh,
-                          int num_sms);
+// (total_q decides only how row tiles are grouped, not the workspace)
+ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int64_t total_q, int max_context,
+                          int max_fresh, int num_sms);
 
 // Tensor maps of a 128-row launch: q (boxes of 64 dimensions, a KV head's group of heads, as
 // many rows as fit 128); fresh k / v (bf16 boxes of 64 x 1 x 128, 128-byte

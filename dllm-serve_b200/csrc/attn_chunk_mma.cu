@@ -14,7 +14,7 @@
 // One row tile ("single"): each KV tile's 128 columns are split between two
 // softmax warpgroups, each with its own running maximum, sum and accumulator,
 // merged once per unit (exact: softmax of a union). Two row tiles ("pair",
-// bf16 rows, launches with at least one such unit per SM): a warpgroup per row
+// bf16 rows, where such units fill the SMs evenly enough): a warpgroup per row
 // tile, and every key tile read from L2 serves both: the single form needs 64
 // KB per 2,290 cycles and SM, close to what L2 delivers.
 //

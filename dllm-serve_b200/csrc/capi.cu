@@ -452,7 +452,7 @@ int64_t dllm_attn_chunk_workspace(int format, int batch, int num_heads, int num_
   if (check_chunk_sizes(format, batch, num_heads, num_kv_heads, max_seqlen_q, max_context, max_fresh) != DLLM_OK)
     return -1;
   if (batch == 0 || max_seqlen_q == 0) return 0;
-  return dllm::plan_attn_chunk(format, batch, num_kv_heads, num_heads / num_kv_heads, max_seqlen_q, max_context,
+  return dllm::plan_attn_chunk(format, batch, num_kv_heads, num_heads / num_kv_heads, max_seqlen_q, 0, max_context,
                                max_fresh, num_sms_of_current_device())
       .workspace_bytes;
 }
@@ -504,7 +504,7 @@ int dllm_attn_chunk_fwd(const dllm_chunk_args* args) {
   if (!cached) max_context = 0;
   if (k == nullptr) max_fresh = 0;
   const dllm::ChunkPlan plan =
-      dllm::plan_attn_chunk(format, batch, num_kv_heads, num_heads / num_kv_heads, max_seqlen_q, max_context,
+      dllm::plan_attn_chunk(format, batch, num_kv_heads, num_heads / num_kv_heads, max_seqlen_q, total_q, max_context,
                             max_fresh, num_sms_of_current_device());
   if (plan.workspace_bytes > 0) {
     if (workspace == nullptr || p.workspace_bytes < plan.workspace_bytes)

@@ -255,6 +255,31 @@ def test_long_chunks_of_many_sequences(dev, fmt, heads, tables):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3", "int8"])
+@pytest.mark.parametrize("heads,nq,causal", [((16, 16), [1000, 1100], True), ((48, 16), [340, 345], False)])
+def test_two_row_tiles_per_unit(dev, fmt, heads, nq, causal):
+    """Sizes at which a work unit takes two row tiles (the second one partial,
+    or missing at a sequence's end), the last sequence's slots scattered."""
+    c = Case(25, fmt, *heads, nq, [200, 37], nq, False, page=128)
+    args, kw = c.args(dev)
+    out = torch.full(c.q.shape, 5.0, dtype=torch.bfloat16, device=dev)
+    _ops().chunk_attention(*args, causal=causal, out=out, **kw)
+    c.check(out, causal, seqs=[1])
+    assert (out[sum(nq):] == 5).all()
+    again = _ops().chunk_attention(*args, causal=causal, **kw)
+    assert torch.equal(again[:sum(nq)], out[:sum(nq)])
+    # the first sequence alone, one tile per unit: both forms are within the bound of each other's roundings
+    one = dict(kw)
+    one |= {"k": kw["k"][:nq[0]], "v": kw["v"][:nq[0]], "cu_seqlens_k": _cu(nq[:1]).to(dev), "max_seqlen_k": nq[0],
+            "slots": kw["slots"][:200], "cu_seqlens_slots": _cu([200]).to(dev)}
+    alone = _ops().chunk_attention(args[0][:nq[0]], *args[1:3], _cu(nq[:1]).to(dev), nq[0], causal=causal, **one)
+    # two results of bf16 roundings each: of the output (2^-8) and of every probability (2^-8 sum p |v|)
+    big = max(float(c.values[1][c.lists[0].long()].abs().max()), float(c.v[:nq[0]].abs().max()))
+    assert (alone.float() - out[:nq[0]].float()).abs().max() <= 4 * 2.0 ** -8 * big
+    assert _ops().read_device_status(dev) == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
 def test_fresh_only(dev, fmt):
     """No cache at all: causal attention among the chunk's own rows."""
