@@ -382,6 +382,58 @@ int check_chunk_sizes(int format, int batch, int Hq, int Hkv, int max_q, int max
   return DLLM_OK;
 }
 
+int select_common(const void* q, int64_t q_tok_stride, const void* k, int64_t k_tok_stride, const void* v,
+                  int64_t v_tok_stride, const int32_t* seq_desc, int n_seqs, int max_klen, int num_heads,
+                  int num_kv_heads, int head_dim, int head_select, void* k_cache, void* v_cache,
+                  int64_t cache_tok_stride, int64_t num_slots, const int32_t* slots, int64_t* top_idx,
+                  int32_t* err_flag, void* stream, int format = DLLM_KV_BF16, void* k_exp = nullptr,
+                  void* v_exp = nullptr) {
+  if (head_dim != 128)
+    return fail(DLLM_ERR_UNSUPPORTED, "head_dim %d not supported (only 128)", head_dim);
+  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0)
+    return fail(DLLM_ERR_UNSUPPORTED, "num_heads must be a positive multiple of num_kv_heads");
+  if (n_seqs < 0 || max_klen < 0) return fail(DLLM_ERR_INVALID_ARG, "negative size");
+  if (max_klen > 16384) return fail(DLLM_ERR_TOO_LARGE, "max_klen %d > 16384", max_klen);
+  if (n_seqs == 0 || max_klen == 0) return DLLM_OK;
+  if (!q || !k || !v || !seq_desc || !k_cache || !v_cache || !slots)
+    return fail(DLLM_ERR_INVALID_ARG, "null pointer");
+  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(k_cache, 16) ||
+      !aligned(v_cache, 16) || q_tok_stride % 8 || k_tok_stride % 8 || v_tok_stride % 8 ||
+      cache_tok_stride % 8)
+    return fail(DLLM_ERR_ALIGNMENT, "q/k/v/cache must be 16-byte aligned with strides %% 8 == 0");
+  if (cache_tok_stride < (int64_t)num_kv_heads * 128)
+    return fail(DLLM_ERR_INVALID_ARG, "cache_tok_stride smaller than num_kv_heads*head_dim");
+  dllm::SelectArgs a;
+  a.q = reinterpret_cast<const __nv_bfloat16*>(q);
+  a.k = reinterpret_cast<const __nv_bfloat16*>(k);
+  a.v = reinterpret_cast<const __nv_bfloat16*>(v);
+  a.q_tok_stride = q_tok_stride;
+  a.k_tok_stride = k_tok_stride;
+  a.v_tok_stride = v_tok_stride;
+  a.seq_desc = seq_desc;
+  a.max_klen = max_klen;
+  a.Hq = num_heads;
+  a.Hkv = num_kv_heads;
+  a.group = num_heads / num_kv_heads;
+  a.sqrt_d = (float)sqrt((double)head_dim);
+  a.k_cache = reinterpret_cast<__nv_bfloat16*>(k_cache);
+  a.v_cache = reinterpret_cast<__nv_bfloat16*>(v_cache);
+  a.cache_tok_stride = cache_tok_stride;
+  a.num_slots = num_slots;
+  a.slots = slots;
+  a.top_idx = top_idx;
+  a.err = err_flag;
+  a.format = format;
+  a.k_exp = static_cast<uint8_t*>(k_exp);
+  a.v_exp = static_cast<uint8_t*>(v_exp);
+  const size_t smem = dllm::select_kv_smem_bytes(head_select ? a.group : a.Hq, max_klen);
+  if (smem > 227 * 1024) return fail(DLLM_ERR_TOO_LARGE, "select_kv needs %zu B smem", smem);
+  cudaError_t e = dllm::launch_select_kv(a, head_select != 0, n_seqs,
+                                         reinterpret_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "select_kv launch");
+  return DLLM_OK;
+}
+
 // Scheduler workspace of dllm_attn_varlen_fwd_static_ws: file-scope device
 // memory (one copy per device, zero when the module loads). The attention
 // kernel uses the first DLLM_SCHED_WORKSPACE_INTS words and leaves them zero;
@@ -762,47 +814,24 @@ int dllm_select_kv_store(const void* q, int64_t q_tok_stride, const void* k, int
                          int head_select, void* k_cache, void* v_cache, int64_t cache_tok_stride,
                          int64_t num_slots, const int32_t* slots, int64_t* top_idx,
                          int32_t* err_flag, void* stream) {
-  if (head_dim != 128)
-    return fail(DLLM_ERR_UNSUPPORTED, "head_dim %d not supported (only 128)", head_dim);
-  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0)
-    return fail(DLLM_ERR_UNSUPPORTED, "num_heads must be a positive multiple of num_kv_heads");
-  if (n_seqs < 0 || max_klen < 0) return fail(DLLM_ERR_INVALID_ARG, "negative size");
-  if (max_klen > 16384) return fail(DLLM_ERR_TOO_LARGE, "max_klen %d > 16384", max_klen);
-  if (n_seqs == 0 || max_klen == 0) return DLLM_OK;
-  if (!q || !k || !v || !seq_desc || !k_cache || !v_cache || !slots)
+  return select_common(q, q_tok_stride, k, k_tok_stride, v, v_tok_stride, seq_desc, n_seqs, max_klen, num_heads,
+                       num_kv_heads, head_dim, head_select, k_cache, v_cache, cache_tok_stride, num_slots, slots,
+                       top_idx, err_flag, stream);
+}
+
+int dllm_select_kv_store_quant(const void* q, int64_t q_tok_stride, const void* k, int64_t k_tok_stride,
+                               const void* v, int64_t v_tok_stride, const int32_t* seq_desc, int n_seqs,
+                               int max_klen, int num_heads, int num_kv_heads, int head_dim, int head_select,
+                               void* k_cache, void* v_cache, void* k_exp, void* v_exp, int format,
+                               int64_t num_slots, const int32_t* slots, int64_t* top_idx, int32_t* err_flag,
+                               void* stream) {
+  if (format != DLLM_KV_E4M3 && format != DLLM_KV_INT8)
+    return fail(DLLM_ERR_UNSUPPORTED, "format %d is not a quantised cache format", format);
+  if (n_seqs > 0 && max_klen > 0 && (k_exp == nullptr || v_exp == nullptr))
     return fail(DLLM_ERR_INVALID_ARG, "null pointer");
-  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(k_cache, 16) ||
-      !aligned(v_cache, 16) || q_tok_stride % 8 || k_tok_stride % 8 || v_tok_stride % 8 ||
-      cache_tok_stride % 8)
-    return fail(DLLM_ERR_ALIGNMENT, "q/k/v/cache must be 16-byte aligned with strides %% 8 == 0");
-  if (cache_tok_stride < (int64_t)num_kv_heads * 128)
-    return fail(DLLM_ERR_INVALID_ARG, "cache_tok_stride smaller than num_kv_heads*head_dim");
-  dllm::SelectArgs a;
-  a.q = reinterpret_cast<const __nv_bfloat16*>(q);
-  a.k = reinterpret_cast<const __nv_bfloat16*>(k);
-  a.v = reinterpret_cast<const __nv_bfloat16*>(v);
-  a.q_tok_stride = q_tok_stride;
-  a.k_tok_stride = k_tok_stride;
-  a.v_tok_stride = v_tok_stride;
-  a.seq_desc = seq_desc;
-  a.max_klen = max_klen;
-  a.Hq = num_heads;
-  a.Hkv = num_kv_heads;
-  a.group = num_heads / num_kv_heads;
-  a.sqrt_d = (float)sqrt((double)head_dim);
-  a.k_cache = reinterpret_cast<__nv_bfloat16*>(k_cache);
-  a.v_cache = reinterpret_cast<__nv_bfloat16*>(v_cache);
-  a.cache_tok_stride = cache_tok_stride;
-  a.num_slots = num_slots;
-  a.slots = slots;
-  a.top_idx = top_idx;
-  a.err = err_flag;
-  const size_t smem = dllm::select_kv_smem_bytes(head_select ? a.group : a.Hq, max_klen);
-  if (smem > 227 * 1024) return fail(DLLM_ERR_TOO_LARGE, "select_kv needs %zu B smem", smem);
-  cudaError_t e = dllm::launch_select_kv(a, head_select != 0, n_seqs,
-                                         reinterpret_cast<cudaStream_t>(stream));
-  if (e != cudaSuccess) return cuda_fail(e, "select_kv launch");
-  return DLLM_OK;
+  return select_common(q, q_tok_stride, k, k_tok_stride, v, v_tok_stride, seq_desc, n_seqs, max_klen, num_heads,
+                       num_kv_heads, head_dim, head_select, k_cache, v_cache, (int64_t)num_kv_heads * 128, num_slots,
+                       slots, top_idx, err_flag, stream, format, k_exp, v_exp);
 }
 
 int dllm_build_step_plan(const int64_t* seqs, int batch, int num_kv_heads, int32_t* out,

@@ -75,23 +75,13 @@ __global__ void __launch_bounds__(kThreads) kv_quant_kernel(KvQuantArgs a) {
       load32<kWide>(value, v);
     }
     // the lanes of a group are one token's, so they are all live or all idle
-    uint32_t bad_k, bad_v;
-    uint32_t mk = finite_max16(k, bad_k), mv = finite_max16(v, bad_v);
-    uint32_t both = mk | (mv << 16);
-#pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, o));
-    uint32_t ek = exp_byte<kFmt>(both & 0xffffu), ev = exp_byte<kFmt>(both >> 16);
-    if (__any_sync(0xffffffffu, (bad_k | bad_v) != 0)) {
-      uint32_t nan = (bad_k >> 1) | (bad_v & 2);  // bit 0: a NaN in the K row, bit 1: in the V row
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) nan |= __shfl_xor_sync(0xffffffffu, nan, o);
-      if (nan & 1) ek = kNanByte;
-      if (nan & 2) ev = kNanByte;
-      if (bad_k | bad_v) set_error(a.err, kDevNonFinite);
-    }
+    uint32_t ek, ev, ck[4], cv[4];
+    group_bytes<kFmt, kLanes>(k, v, 0xffffffffu, a.err, ek, ev);
     if (!ok) return;
-    *reinterpret_cast<uint4*>(a.k_cache + code) = quantise16<kFmt>(k, ek);
-    *reinterpret_cast<uint4*>(a.v_cache + code) = quantise16<kFmt>(v, ev);
+    quantise<kFmt>(k, ek, ck);
+    quantise<kFmt>(v, ev, cv);
+    *reinterpret_cast<uint4*>(a.k_cache + code) = make_uint4(ck[0], ck[1], ck[2], ck[3]);
+    *reinterpret_cast<uint4*>(a.v_cache + code) = make_uint4(cv[0], cv[1], cv[2], cv[3]);
     if (part == 0) {
       a.k_exp[ex] = (uint8_t)ek;
       a.v_exp[ex] = (uint8_t)ev;

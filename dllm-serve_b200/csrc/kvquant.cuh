@@ -73,18 +73,19 @@ DLLM_DEVICE uint32_t encode4(float y0, float y1, float y2, float y3) {
   }
 }
 
-// Largest finite bf16 magnitude of eight words (pairs of bf16). bad: 1 if any
+// Largest finite bf16 magnitude of kWords words (pairs of bf16). bad: 1 if any
 // value is infinite, 2 if any is NaN.
-DLLM_DEVICE uint32_t finite_max16(const uint32_t (&w)[8], uint32_t& bad) {
+template <int kWords>
+DLLM_DEVICE uint32_t finite_max(const uint32_t (&w)[kWords], uint32_t& bad) {
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+  for (int i = 0; i < kWords; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
   m = max(m & 0xffffu, m >> 16);
   bad = m > 0x7f80u ? 2 : m == 0x7f80u ? 1 : 0;
   if (bad) {
     m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < kWords; ++i) {
       const uint32_t lo = w[i] & 0x7fffu, hi = (w[i] >> 16) & 0x7fffu;
       if (lo < 0x7f80u) m = max(m, lo);
       if (hi < 0x7f80u) m = max(m, hi);
@@ -93,19 +94,43 @@ DLLM_DEVICE uint32_t finite_max16(const uint32_t (&w)[8], uint32_t& bad) {
   return m;
 }
 
-// Quantises 16 bf16 values (eight words) with the group's exponent byte.
-template <int kFmt>
-DLLM_DEVICE uint4 quantise16(const uint32_t (&w)[8], uint32_t byte) {
-  if (byte == kNanByte) return make_uint4(0, 0, 0, 0);
-  const float inv = __uint_as_float((254u - byte) << 23);  // 2^-e
-  uint32_t c[4];
+// Quantises kWords words of bf16 pairs with the group's exponent byte.
+template <int kFmt, int kWords>
+DLLM_DEVICE void quantise(const uint32_t (&w)[kWords], uint32_t byte, uint32_t (&c)[kWords / 2]) {
+  if (byte == kNanByte) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kWords / 2; ++i) c[i] = 0;
+    return;
+  }
+  const float inv = __uint_as_float((254u - byte) << 23);  // 2^-e
+#pragma unroll
+  for (int i = 0; i < kWords / 2; ++i) {
     const uint32_t a = w[2 * i], b = w[2 * i + 1];
     c[i] = encode4<kFmt>(__uint_as_float(a << 16) * inv, __uint_as_float(a & 0xffff0000u) * inv,
                          __uint_as_float(b << 16) * inv, __uint_as_float(b & 0xffff0000u) * inv);
   }
-  return make_uint4(c[0], c[1], c[2], c[3]);
+}
+
+// Exponent bytes of a K and a V group spread over kLanes lanes (kWords words
+// each; every lane of `mask` takes part). Infinities and NaN set *err.
+template <int kFmt, int kLanes, int kWords>
+DLLM_DEVICE void group_bytes(const uint32_t (&k)[kWords], const uint32_t (&v)[kWords], uint32_t mask, int32_t* err,
+                             uint32_t& ek, uint32_t& ev) {
+  uint32_t bad_k, bad_v;
+  const uint32_t mk = finite_max(k, bad_k), mv = finite_max(v, bad_v);
+  uint32_t both = mk | (mv << 16);
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) both = __vmaxu2(both, __shfl_xor_sync(mask, both, o));
+  ek = exp_byte<kFmt>(both & 0xffffu);
+  ev = exp_byte<kFmt>(both >> 16);
+  if (__any_sync(mask, (bad_k | bad_v) != 0)) {
+    uint32_t nan = (bad_k >> 1) | (bad_v & 2);  // bit 0: a NaN in the K row, bit 1: in the V row
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) nan |= __shfl_xor_sync(mask, nan, o);
+    if (nan & 1) ek = kNanByte;
+    if (nan & 2) ev = kNanByte;
+    if (bad_k | bad_v) set_error(err, kDevNonFinite);
+  }
 }
 
 // Expansion of codes to bf16, exact. No conversion instruction: e4m3

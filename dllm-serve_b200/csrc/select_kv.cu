@@ -14,7 +14,9 @@
 // pooled score T, the keys above T plus the lowest-index keys equal to T are
 // compacted, and only those n_keep keys are bitonic-sorted as 64-bit
 // (order-preserving score bits << 32) | (0xffffffff - candidate), so the result
-// is "descending score, ties by ascending candidate index".
+// is "descending score, ties by ascending candidate index". Into a quantised
+// cache the selected rows go as store_kvcache_quant would write them (16 lanes
+// hold a row, so its maximum is four shuffles); the selection is the same.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -22,6 +24,7 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "kvquant.cuh"
 #include "select_kv.h"
 
 namespace cg = cooperative_groups;
@@ -141,7 +144,27 @@ DLLM_DEVICE int cand_token(int c, int blk_start, int blk_len) {
 // kGroup (head_select only): more than one query head per KV head. The two
 // cases are separate instantiations so that the grouped scoring's registers
 // do not cost the single-head scoring loop.
-template <bool kHeadSelect, bool kGroup>
+// Writes a selected head row (16 lanes x 8 bf16 each of K and V) into a slot of
+// a quantised cache. Every lane of `mask`, the row's 16 lanes, takes part;
+// dst < 0: nothing is written.
+template <int kFmt>
+DLLM_DEVICE void put_quantised(const SelectArgs& a, uint4 k, uint4 v, int64_t dst, int head, int hl, uint32_t mask) {
+  const uint32_t kw[4] = {k.x, k.y, k.z, k.w}, vw[4] = {v.x, v.y, v.z, v.w};
+  uint32_t ek, ev, ck[2], cv[2];
+  group_bytes<kFmt, 16>(kw, vw, mask, dst < 0 ? nullptr : a.err, ek, ev);
+  if (dst < 0) return;
+  quantise<kFmt>(kw, ek, ck);
+  quantise<kFmt>(vw, ev, cv);
+  const int64_t at = dst * a.cache_tok_stride + (int64_t)head * kD + hl * 8;
+  *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(a.k_cache) + at) = make_uint2(ck[0], ck[1]);
+  *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(a.v_cache) + at) = make_uint2(cv[0], cv[1]);
+  if (hl == 0) {
+    a.k_exp[dst * a.Hkv + head] = (uint8_t)ek;
+    a.v_exp[dst * a.Hkv + head] = (uint8_t)ev;
+  }
+}
+
+template <bool kHeadSelect, bool kGroup, int kFmt>
 __global__ void __launch_bounds__(kThreads, 2) select_kv_kernel(SelectArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int seq = blockIdx.y;
@@ -545,6 +568,18 @@ __global__ void __launch_bounds__(kThreads, 2) select_kv_kernel(SelectArgs a) {
           dst[r] = a.slots[slot_off + j];
         }
       }
+      if constexpr (kFmt != kFmtBf16) {
+#pragma unroll
+        for (int r = 0; r < kRowsInFlight; ++r) {
+          if (j0 + r * kHalves >= n_keep) break;  // (the same for the row's 16 lanes)
+          if (dst[r] >= a.num_slots) {
+            if (hl == 0) set_error(a.err, kDevSlotOutOfRange);
+            dst[r] = -1;
+          }
+          put_quantised<kFmt>(a, kv[r][0], kv[r][1], dst[r], h, hl, 0xffffu << (16 * (half & 1)));
+        }
+        continue;
+      }
 #pragma unroll
       for (int r = 0; r < kRowsInFlight; ++r) {
         if (dst[r] < 0) continue;  // negative slot: skipped (padding convention)
@@ -569,6 +604,12 @@ __global__ void __launch_bounds__(kThreads, 2) select_kv_kernel(SelectArgs a) {
       const int64_t tok = tok_start + cand_token(c, blk_start, blk_len);
       const uint4* ks = reinterpret_cast<const uint4*>(a.k + tok * a.k_tok_stride);
       const uint4* vs = reinterpret_cast<const uint4*>(a.v + tok * a.v_tok_stride);
+      if constexpr (kFmt != kFmtBf16) {
+        // a half warp per head row; the warp's halves may differ in whether they have one
+        for (int e = lane; e < row_vec; e += 32)
+          put_quantised<kFmt>(a, __ldg(ks + e), __ldg(vs + e), slot, e >> 4, lane & 15, 0xffffu << (lane & 16));
+        continue;
+      }
       uint4* kd = reinterpret_cast<uint4*>(a.k_cache + slot * a.cache_tok_stride);
       uint4* vd = reinterpret_cast<uint4*>(a.v_cache + slot * a.cache_tok_stride);
 #pragma unroll 8
@@ -601,12 +642,14 @@ cudaError_t launch_select_kv(const SelectArgs& a, bool head_select, int n_seqs, 
   // recorded into a CUDA graph, make no attribute calls).
   // Host threads share these caches; raising the attribute is serialised so
   // that a concurrent smaller request never lowers it under a larger one.
-  static std::atomic<size_t> smem_set[3][64];
+  static std::atomic<size_t> smem_set[9][64];
   static std::mutex raise_mu;
-  const int kind = head_select ? (a.group > 1 ? 2 : 1) : 0;
-  void (*kernel)(SelectArgs) = kind == 0   ? select_kv_kernel<false, false>
-                               : kind == 1 ? select_kv_kernel<true, false>
-                                           : select_kv_kernel<true, true>;
+  static void (*const kernels[9])(SelectArgs) = {
+      select_kv_kernel<false, false, kFmtBf16>, select_kv_kernel<true, false, kFmtBf16>, select_kv_kernel<true, true, kFmtBf16>,
+      select_kv_kernel<false, false, kFmtE4m3>, select_kv_kernel<true, false, kFmtE4m3>, select_kv_kernel<true, true, kFmtE4m3>,
+      select_kv_kernel<false, false, kFmtInt8>, select_kv_kernel<true, false, kFmtInt8>, select_kv_kernel<true, true, kFmtInt8>};
+  const int kind = 3 * a.format + (head_select ? (a.group > 1 ? 2 : 1) : 0);
+  void (*kernel)(SelectArgs) = kernels[kind];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;

@@ -22,6 +22,11 @@ struct SelectArgs {
   int64_t num_slots;
   const int32_t* slots;
   int64_t* top_idx;                                  // optional
+  // A quantised cache: format DLLM_KV_E4M3 / DLLM_KV_INT8, k_cache / v_cache hold codes (one byte
+  // an element, slots cache_tok_stride bytes apart), exponent bytes num_kv_heads a slot.
+  int format;
+  uint8_t* k_exp;
+  uint8_t* v_exp;
   int32_t* err;
 };
 

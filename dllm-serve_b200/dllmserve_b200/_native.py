@@ -94,6 +94,10 @@ SIGNATURES = {
     "dllm_ipc_export": ([_P, _P, _P], _I),
     "dllm_ipc_open": ([_P, _P], _I),
     "dllm_ipc_close": ([_P], _I),
+    "dllm_select_kv_store_quant": (
+        [_P, _I64, _P, _I64, _P, _I64, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I64, _P, _P, _P, _P],
+        _I,
+    ),
     "dllm_select_kv_store": (
         [_P, _I64, _P, _I64, _P, _I64, _P, _I, _I, _I, _I, _I, _I, _P, _P, _I64, _I64, _P, _P, _P, _P],
         _I,

@@ -17,6 +17,15 @@ with all per-sequence metadata built once per step (``StepPlan``). The
 reference stores the selection before it attends; the two launches touch
 disjoint memory (the selection writes only state-1 sequences' cache slots,
 the attention reads only state-2 ones), so the order changes no result.
+
+The regular path (attention.py:121-148) stores the step's rows and attends
+causally: prefill over the rows themselves, prefill over block tables (a chunk
+behind cached rows) and decode are one operator (``ops.chunk_attention``).
+
+The cache may be quantised: bind ``k_cache`` / ``v_cache`` of float8_e4m3fn or
+int8 and the exponent bytes ``k_exp`` / ``v_exp`` (uint8 [blocks, block_size,
+num_kv_heads]). Both paths then store 8-bit rows and read them back inside the
+attention launch; fresh rows of a diffusion step are used as they come.
 """
 from __future__ import annotations
 
@@ -63,6 +72,7 @@ class Attention(nn.Module):
         self.num_kv_heads = num_kv_heads
         self.causal = causal
         self.k_cache = self.v_cache = torch.tensor([])
+        self.k_exp = self.v_exp = None  # exponent bytes of a quantised cache
         self.layer_id = None
         # top_idx of the last "compute cache" launch per head_select flavour
         # (device int64); kept only when ``record_selection`` is set.
@@ -83,18 +93,61 @@ class Attention(nn.Module):
         if context.is_diffusion:
             return self._diffusion_attention(q, k, v, context)
         if self.k_cache.numel() and self.v_cache.numel():
-            store_kvcache(k, v, self.k_cache, self.v_cache, context.slot_mapping)
+            if self._quantised():
+                ops.store_kvcache_quant(k, v, self.k_cache, self.v_cache, self.k_exp, self.v_exp, context.slot_mapping)
+            else:
+                store_kvcache(k, v, self.k_cache, self.v_cache, context.slot_mapping)
         return self._regular_attention(q, k, v, context)
 
+    def _quantised(self) -> bool:
+        if self.k_cache.dtype in (torch.float8_e4m3fn, torch.int8):
+            if self.k_exp is None or self.v_exp is None:
+                raise ValueError("a quantised cache needs k_exp and v_exp")
+            return True
+        return False
+
     def _regular_attention(self, q, k, v, context):
-        """Non-diffusion path (attention.py:121-148). Only the non-causal,
-        non-paged prefill form exists on this path's kernels."""
-        if self.causal or not context.is_prefill or context.block_tables is not None:
-            raise NotImplementedError(
-                "dllmserve_b200 implements the diffusion (non-causal) attention path only")
-        o = ops.varlen_attention(q, k, v, context.cu_seqlens_q, context.cu_seqlens_k,
-                                 int(context.max_seqlen_q), self.scale)
-        return o.view(-1, self.num_heads * self.head_dim)
+        """Non-diffusion path (attention.py:121-148). Prefill without block
+        tables attends to the step's own rows; with block tables, and in
+        decode steps (one row per sequence), to the cache, which the rows were
+        stored into, the last ``max_seqlen_q`` positions being the step's own."""
+        H, Hk = self.num_heads, self.num_kv_heads
+        tables = context.block_tables
+        if context.is_prefill and tables is None:
+            if not self.causal:
+                o = ops.varlen_attention(q, k, v, context.cu_seqlens_q, context.cu_seqlens_k,
+                                         int(context.max_seqlen_q), self.scale)
+            else:
+                o = ops.chunk_attention(q, None, None, context.cu_seqlens_q, int(context.max_seqlen_q), self.scale,
+                                        causal=True, k=k, v=v, cu_seqlens_k=context.cu_seqlens_k,
+                                        max_seqlen_k=int(context.max_seqlen_k) or int(context.max_seqlen_q))
+            return o.view(-1, H * self.head_dim)
+        if tables is None:
+            raise ValueError("a decode step needs context.block_tables")
+        if context.is_prefill:
+            cu_q, max_q = context.cu_seqlens_q, int(context.max_seqlen_q)
+            lens, most = self._per_step(context, "lens", lambda: torch.diff(context.cu_seqlens_k)), int(context.max_seqlen_k)
+        else:
+            cu_q = self._per_step(context, "ones", lambda: torch.arange(q.shape[0] + 1, dtype=torch.int32, device=q.device))
+            max_q, lens, most = 1, context.context_lens, 0
+        o = ops.chunk_attention(q, self.k_cache, self.v_cache, cu_q, max_q, self.scale, causal=self.causal,
+                                block_tables=tables, context_lens=lens, max_context=most or None,
+                                k_exp=self.k_exp, v_exp=self.v_exp)
+        return o.view(-1, H * self.head_dim)
+
+    @staticmethod
+    def _per_step(context, name, make):
+        """A device array derived from the step's context, made by its first layer."""
+        cache = getattr(context, _PLAN_ATTR + "_regular", None)
+        if cache is None:
+            cache = {}
+            try:
+                setattr(context, _PLAN_ATTR + "_regular", cache)
+            except AttributeError:  # a frozen context: rebuild per layer
+                pass
+        if name not in cache:
+            cache[name] = make()
+        return cache[name]
 
     def _diffusion_attention(self, q, k, v, context):
         """q [N, num_heads*D] or [N, num_heads, D]; k, v likewise with
@@ -104,16 +157,24 @@ class Attention(nn.Module):
         if self.record_selection:
             self.last_selection = {}
         out = q.new_empty((q.shape[0], H * D))
-        launch = plan.scratch.get(self._launch_key)
-        if launch is None:
-            dev = q.device
-            # step-level arguments validated once per plan, shared by the layers of this shape
-            launch = ops.prepare_attention(
-                plan.cu, plan.cu, plan.max_rows, plan.total_rows, H, Hk, D, self.scale, dev,
-                slots=plan.slots_c, cu_seqlens_slots=plan.cu_c)
-            plan.scratch[self._launch_key] = launch
-        # out was made here with the launch's layout (q's dtype and device, [rows, H*D])
-        res = launch(q, k, v, out, self._paged_cache_args() if plan.total_c > 0 else None, out_checked=True)
+        quant = self._quantised()
+        if quant and plan.total_c > 0:
+            res = ops.chunk_attention(
+                q.view(-1, H, D), self.k_cache, self.v_cache, plan.cu, plan.max_rows, self.scale, causal=False,
+                slots=plan.slots_c, cu_seqlens_slots=plan.cu_c, max_context=max(f.n_cached for f in plan.infos),
+                k=k.view(-1, Hk, D), v=v.view(-1, Hk, D), cu_seqlens_k=plan.cu, max_seqlen_k=plan.max_rows,
+                k_exp=self.k_exp, v_exp=self.v_exp, out=out.view(-1, H, D)).view(-1, H * D)
+        else:
+            launch = plan.scratch.get(self._launch_key)
+            if launch is None:
+                dev = q.device
+                # step-level arguments validated once per plan, shared by the layers of this shape
+                launch = ops.prepare_attention(
+                    plan.cu, plan.cu, plan.max_rows, plan.total_rows, H, Hk, D, self.scale, dev,
+                    slots=plan.slots_c, cu_seqlens_slots=plan.cu_c)
+                plan.scratch[self._launch_key] = launch
+            # out was made here with the launch's layout (q's dtype and device, [rows, H*D])
+            res = launch(q, k, v, out, self._paged_cache_args() if plan.total_c > 0 else None, out_checked=True)
         # The selection runs after the attention: it writes only the cache slots
         # of compute-cache sequences, which no launch of this step reads, and
         # finds this layer's K/V still partly in L2.
@@ -129,8 +190,8 @@ class Attention(nn.Module):
                 if self.record_selection:
                     top_idx = torch.empty(idx_total, dtype=torch.int64, device=dev)
                     self.last_selection[head_select] = top_idx
-                ops.select_kv_store(qv, kv_, vv, desc, max_klen, head_select,
-                                    self.k_cache, self.v_cache, slots, top_idx)
+                ops.select_kv_store(qv, kv_, vv, desc, max_klen, head_select, self.k_cache, self.v_cache, slots, top_idx,
+                                    k_exp=self.k_exp, v_exp=self.v_exp)
         return res
 
     def _paged_cache_args(self):

@@ -844,10 +844,15 @@ def select_kv_store(
     v_cache: torch.Tensor,
     slots: torch.Tensor,
     top_idx: torch.Tensor | None = None,
+    *,
+    k_exp: torch.Tensor | None = None,
+    v_exp: torch.Tensor | None = None,
 ) -> None:
     """Score candidates, pick the top n_keep per sequence (per KV head with
     ``head_select``), write their K/V rows into ``slots`` of the cache and,
-    if given, the chosen candidate indices into ``top_idx`` (int64)."""
+    if given, the chosen candidate indices into ``top_idx`` (int64). A
+    quantised cache (float8_e4m3fn or int8, with ``k_exp`` / ``v_exp``) receives
+    the rows as ``store_kvcache_quant`` writes them."""
     Hq, D = q.shape[1], q.shape[2]
     Hkv = k.shape[1]
     _check_rows("q", q, Hq, D)
@@ -858,23 +863,38 @@ def select_kv_store(
         raise ValueError("seq_desc must be int32 [n_seqs, 8]")
     if not seq_desc.is_contiguous() or slots.dtype != torch.int32 or not slots.is_contiguous():
         raise ValueError("seq_desc and slots must be contiguous int32")
-    if k_cache.dtype != torch.bfloat16 or v_cache.dtype != torch.bfloat16:
-        raise ValueError("caches must be bfloat16")
+    fmt = _KV_FORMATS.get(k_cache.dtype)
+    if fmt is None or v_cache.dtype != k_cache.dtype:
+        raise ValueError("caches must be bfloat16, or both float8_e4m3fn or int8")
     row = Hkv * D
     if k_cache.stride(-1) != 1 or k_cache.numel() % row != 0 or v_cache.numel() != k_cache.numel():
         raise ValueError("caches must be contiguous rows of num_kv_heads*head_dim")
+    if fmt != _native.KV_BF16:
+        if k_exp is None or v_exp is None:
+            raise ValueError("a quantised cache needs k_exp and v_exp")
+        _require_cuda(q, k_exp, v_exp)
+        _check_quant_cache("k", k_cache, k_exp, Hkv, D)
+        _check_quant_cache("v", v_cache, v_exp, Hkv, D)
     if top_idx is not None:
         _require_cuda(q, top_idx)
         if top_idx.dtype != torch.int64 or not top_idx.is_contiguous():
             raise ValueError("top_idx must be contiguous int64")
     lib = _native.lib()
     with _on_device(dev):
-        rc = lib.dllm_select_kv_store(
-            q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
-            seq_desc.data_ptr(), seq_desc.shape[0], int(max_klen), Hq, Hkv, D, int(bool(head_select)),
-            k_cache.data_ptr(), v_cache.data_ptr(), row, k_cache.numel() // row, slots.data_ptr(),
-            _ptr(top_idx), _status_ptr(dev), _stream_ptr(),
-        )
+        if fmt != _native.KV_BF16:
+            rc = lib.dllm_select_kv_store_quant(
+                q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
+                seq_desc.data_ptr(), seq_desc.shape[0], int(max_klen), Hq, Hkv, D, int(bool(head_select)),
+                k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), fmt, k_cache.numel() // row,
+                slots.data_ptr(), _ptr(top_idx), _status_ptr(dev), _stream_ptr(),
+            )
+        else:
+            rc = lib.dllm_select_kv_store(
+                q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
+                seq_desc.data_ptr(), seq_desc.shape[0], int(max_klen), Hq, Hkv, D, int(bool(head_select)),
+                k_cache.data_ptr(), v_cache.data_ptr(), row, k_cache.numel() // row, slots.data_ptr(),
+                _ptr(top_idx), _status_ptr(dev), _stream_ptr(),
+            )
     _native.check(rc, "select_kv_store")
     if seq_desc.shape[0] > 0 and max_klen > 0:
         LAUNCHES[0] += 1

@@ -31,9 +31,9 @@
  *                                (linear.py:186-190), one kernel over NVLink peer memory
  *   dllm_build_step_plan      <- the per-sequence metadata of attention.py:168-304 /
  *                                model_runner.py:240-321, on the device
- *   dllm_store_kvcache_quant, dllm_load_kvcache_quant
- *                             (no reference counterpart) the two copies above for a cache
- *                                held in 8 bits per element
+ *   dllm_store_kvcache_quant, dllm_load_kvcache_quant, dllm_select_kv_store_quant
+ *                             (no reference counterpart) the two copies above, and the
+ *                                selection below, for a cache held in 8 bits per element
  *   dllm_attn_chunk_fwd       <- the regular (non-diffusion) branches of Attention.forward
  *                                (attention.py:121-148): causal prefill, prefill over block
  *                                tables, decode; also over a quantised cache, and for the
@@ -420,6 +420,19 @@ DLLM_API int dllm_select_kv_store(const void* q, int64_t q_tok_stride, const voi
                          int head_select, void* k_cache, void* v_cache, int64_t cache_tok_stride,
                          int64_t num_slots, const int32_t* slots, int64_t* top_idx,
                          int32_t* err_flag, void* stream);
+
+/*
+ * dllm_select_kv_store into a quantised cache: the selection is the same, the chosen rows
+ * are written as dllm_store_kvcache_quant writes them. k_cache, v_cache, k_exp, v_exp,
+ * format and num_slots as there (head_dim 128).
+ */
+DLLM_API int dllm_select_kv_store_quant(const void* q, int64_t q_tok_stride, const void* k, int64_t k_tok_stride,
+                                        const void* v, int64_t v_tok_stride, const int32_t* seq_desc,
+                                        int n_seqs, int max_klen, int num_heads, int num_kv_heads,
+                                        int head_dim, int head_select, void* k_cache, void* v_cache,
+                                        void* k_exp, void* v_exp, int format, int64_t num_slots,
+                                        const int32_t* slots, int64_t* top_idx, int32_t* err_flag,
+                                        void* stream);
 
 /*
  * Head-compacted attention: dllm_attn_varlen_fwd (or, with k_cache/v_cache/slots/

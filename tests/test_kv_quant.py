@@ -263,3 +263,19 @@ def test_refusals_on_device_tensors(dev):
     y = torch.zeros(2, 2, 96, dtype=torch.bfloat16, device=dev)
     with pytest.raises(NotImplementedError):
         ops.store_kvcache_quant(y, y, c.new_zeros(1, 16, 2, 96), c.new_zeros(1, 16, 2, 96), e, e, s)
+
+
+def test_selection_refusals():
+    from dllmserve_b200 import _native
+
+    fn = _native.lib().dllm_select_kv_store_quant
+
+    def call(fmt=1, ke=64, ve=64, n=1, klen=32, hd=128, h=2):
+        return fn(64, 256, 64, 256, 64, 256, 64, n, klen, h, 2, hd, 1, 64, 64, ke, ve, fmt, 64, 64, None, None, None)
+
+    assert call(fmt=0) == _native.DLLM_ERR_UNSUPPORTED
+    assert call(ke=None) == _native.DLLM_ERR_INVALID_ARG
+    assert call(hd=64) == _native.DLLM_ERR_UNSUPPORTED
+    assert call(h=3) == _native.DLLM_ERR_UNSUPPORTED
+    assert call(klen=20000) == _native.DLLM_ERR_TOO_LARGE
+    assert call(n=0, ke=None) == _native.DLLM_OK
