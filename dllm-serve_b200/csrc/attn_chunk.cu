@@ -27,11 +27,11 @@
 // ring of stages filled by cp.async, so the main loop has no CTA barrier. The
 // warps' partial results are merged in shared memory in a fixed order; splits
 // are merged by a second kernel, also in a fixed order. Products are
-// mma.sync m16n8k16: at up to 16 rows per KV head a launch reads 512 bytes per
-// bf16 key for at most 16 x 512 operations, below what this instruction
-// sustains, and its operands go straight from shared memory to registers,
-// where codes are expanded. (At 32 rows it took 62 us where the tcgen05
-// kernel takes 54: 8 sequences, 32 heads, 1,144 e4m3 rows.)
+// mma.sync m16n8k16: at up to 16 rows per KV head (32 with a quantised cache) a
+// launch reads 512 (256) bytes per key for at most 16 x 512 (32 x 512)
+// operations, below what this instruction sustains, and its operands go
+// straight from shared memory to registers, where codes are expanded; the
+// tcgen05 kernel writes them to shared memory first.
 //
 // Operand layout: keys (scores) and dimensions (outputs) take the products' 16
 // rows and the packed query rows their 8 columns, so eight rows leave nothing
@@ -73,20 +73,20 @@ constexpr int chunk_keys() { return kFmt == kFmtBf16 ? 16 : 32; }
 // A quantised chunk is bound by the latency of its conversions and products
 // (issue slots 36 % used with eight warps an SM), a bf16 chunk by bytes in
 // flight. Eight e4m3 contexts of 16,384 rows, 32 heads: two CTAs of three
-// stages 253 us, three CTAs of two 197 us; bf16 contexts of 4,096 rows, 28/4
-// heads: 54 and 66 us.
-template <int kFmt>
+// stages 195 us, three CTAs of two 184 us; bf16 contexts of 4,096 rows, 28/4
+// heads: 54 and 66 us. Four 8-row groups take the registers of two CTAs.
+template <int kFmt, int kN>
 struct Cfg {
-  static constexpr int kStages = kFmt == kFmtBf16 ? 3 : 2;
-  static constexpr int kCtas = kFmt == kFmtBf16 ? 2 : 3;  // per SM
+  static constexpr int kCtas = kFmt == kFmtBf16 || kN > 2 ? 2 : 3;  // per SM
+  static constexpr int kStages = kCtas == 2 ? 3 : 2;
   static constexpr uint32_t kOffStages = 0;
   static constexpr uint32_t kOffScales = kOffStages + kWarps * kStages * kStageBytes;
   static constexpr uint32_t kOffRowFactor = kOffScales + kWarps * kStages * kScaleBytes;  // float per packed row
-  static constexpr uint32_t kOffQ = kOffRowFactor + 16 * 4;
-  static constexpr uint32_t kSmemBytes = kOffQ + 16 * kD * 2;
+  static constexpr uint32_t kOffQ = kOffRowFactor + kN * 8 * 4;
+  static constexpr uint32_t kSmemBytes = kOffQ + kN * 8 * kD * 2;
   static_assert(kCtas * (kSmemBytes + 1024) <= 233472, "the CTAs do not fit an SM");
   // the merge buffers (per warp: rows x 128 floats, then rows float2) reuse the stages
-  static_assert(kWarps * (16 * kD * 4 + 16 * 8) <= kWarps * kStages * kStageBytes, "merge buffers exceed the stages");
+  static_assert(kWarps * kN * 8 * (kD * 4 + 8) <= kWarps * kStages * kStageBytes, "merge buffers exceed the stages");
 };
 
 DLLM_DEVICE void cp_async16(uint32_t dst, const void* src, bool live) {
@@ -176,6 +176,10 @@ struct Rows {
   int e;                 // O is in units of 2^(e - 15) (quantised caches)
 };
 
+// Q stays in registers for up to 16 rows, else it is read from shared memory chunk by chunk.
+template <int kN>
+constexpr bool kQInRegs = kN <= 2;
+
 // The 8x8 matrix of 16-bit values whose row g the lanes 4g .. 4g+3 hold, transposed.
 DLLM_DEVICE uint32_t transpose8(uint32_t x) {
   uint32_t y;
@@ -189,7 +193,7 @@ DLLM_DEVICE uint32_t transpose8(uint32_t x) {
 // factor `back` for row 8n + g, O scaled), kFmt: the format of this chunk (its
 // fresh chunks are bf16).
 template <bool kQuant, int kFmt, int kN>
-DLLM_DEVICE void chunk_step(uint32_t ks, uint32_t vs, uint32_t scales, const uint32_t (&qf)[kN][16],
+DLLM_DEVICE void chunk_step(uint32_t ks, uint32_t vs, uint32_t scales, uint32_t qs, const uint32_t (&qf)[kN][16],
                             const float (&back)[kN], int lane, float sl2, bool whole, int pos, int end, Rows<kN>& w) {
   constexpr int KB = chunk_keys<kFmt>();
   constexpr int KT = KB / 16;  // 16-key tiles
@@ -205,39 +209,57 @@ DLLM_DEVICE void chunk_step(uint32_t ks, uint32_t vs, uint32_t scales, const uin
       for (int e = 0; e < 4; ++e) s[kt][n][e] = 0.f;
   // scores: half h covers dimensions 64h + 16t .. + 15 of this thread
 #pragma unroll
-  for (int kt = 0; kt < KT; ++kt) {
+  for (int h = 0; h < 2; ++h) {
+    uint32_t ka[KT][2][8];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t ka[2][8];
+    for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const uint32_t key = 16 * kt + 8 * e + g;
+        uint32_t(&k)[8] = ka[kt][e];
         if constexpr (!kCodes) {
           const uint4 x = lds128(ks + key * kRow + (k_unit<kFmt>(8 * h + 2 * t, key) << 4));
           const uint4 y = lds128(ks + key * kRow + (k_unit<kFmt>(8 * h + 2 * t + 1, key) << 4));
-          ka[e][0] = x.x, ka[e][1] = x.y, ka[e][2] = x.z, ka[e][3] = x.w;
-          ka[e][4] = y.x, ka[e][5] = y.y, ka[e][6] = y.z, ka[e][7] = y.w;
+          k[0] = x.x, k[1] = x.y, k[2] = x.z, k[3] = x.w;
+          k[4] = y.x, k[5] = y.y, k[6] = y.z, k[7] = y.w;
         } else {
           const uint4 x = lds128(ks + key * kRow + (k_unit<kFmt>(4 * h + t, key) << 4));
-          codes_to_f16<kFmt>(x.x, ka[e][0], ka[e][1]);
-          codes_to_f16<kFmt>(x.y, ka[e][2], ka[e][3]);
-          codes_to_f16<kFmt>(x.z, ka[e][4], ka[e][5]);
-          codes_to_f16<kFmt>(x.w, ka[e][6], ka[e][7]);
+          codes_to_f16<kFmt>(x.x, k[0], k[1]);
+          codes_to_f16<kFmt>(x.y, k[2], k[3]);
+          codes_to_f16<kFmt>(x.z, k[4], k[5]);
+          codes_to_f16<kFmt>(x.w, k[6], k[7]);
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+    for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int n = 0; n < kN; ++n) {
-          uint32_t b0 = qf[n][8 * h + 2 * i], b1 = qf[n][8 * h + 2 * i + 1];
-          if constexpr (kCodes) {
-            mma16816_f16(s[kt][n], ka[0][2 * i], ka[1][2 * i], ka[0][2 * i + 1], ka[1][2 * i + 1], b0, b1);
-          } else {
-            if constexpr (kQuant) b0 = f16_to_bf16(b0, back[n]), b1 = f16_to_bf16(b1, back[n]);
-            mma16816(s[kt][n], ka[0][2 * i], ka[1][2 * i], ka[0][2 * i + 1], ka[1][2 * i + 1], b0, b1);
-          }
+      for (int n = 0; n < kN; ++n) {
+        uint32_t q[4];
+        if constexpr (kQInRegs<kN>) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) q[i] = qf[n][8 * h + 4 * c + i];
+        } else {
+          const int row = 8 * n + g;
+          const uint4 x = lds128(qs + row * 256 + (((8 * h + 2 * t + c) ^ (row & 1)) << 4));
+          q[0] = x.x, q[1] = x.y, q[2] = x.z, q[3] = x.w;
         }
-    }
+        if constexpr (kQuant && !kCodes) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) q[i] = f16_to_bf16(q[i], back[n]);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt) {
+            const uint32_t(&k0)[8] = ka[kt][0];
+            const uint32_t(&k1)[8] = ka[kt][1];
+            const int x = 4 * c + 2 * i;
+            if constexpr (kCodes)
+              mma16816_f16(s[kt][n], k0[x], k1[x], k0[x + 1], k1[x + 1], q[2 * i], q[2 * i + 1]);
+            else
+              mma16816(s[kt][n], k0[x], k1[x], k0[x + 1], k1[x + 1], q[2 * i], q[2 * i + 1]);
+          }
+      }
   }
   // the value exponents of the chunk against the unit of O
   float ufac = 1.f, grow = 1.f;  // P times this; O times this
@@ -377,9 +399,9 @@ DLLM_DEVICE void chunk_step(uint32_t ks, uint32_t vs, uint32_t scales, const uin
 }
 
 template <int kFmt, int kN>
-__global__ void __launch_bounds__(kThreads, Cfg<kFmt>::kCtas) attn_chunk_kernel(const __grid_constant__ ChunkArgs a) {
+__global__ void __launch_bounds__(kThreads, Cfg<kFmt, kN>::kCtas) attn_chunk_kernel(const __grid_constant__ ChunkArgs a) {
   constexpr int KB = chunk_keys<kFmt>();
-  using C = Cfg<kFmt>;
+  using C = Cfg<kFmt, kN>;
   constexpr int kStages = C::kStages;
   constexpr int kRows = 8 * kN;  // packed rows of a tile
   constexpr bool kQuant = kFmt != kFmtBf16;
@@ -529,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kFmt>::kCtas) attn_chunk_kernel(
                  : "memory");
   }
   __syncthreads();
-  uint32_t qf[kN][16];
+  uint32_t qf[kN][16] = {};
   float back[kN];
   const int64_t L = (int64_t)sq.nc + sq.nk;
   Rows<kN> w;
@@ -537,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kFmt>::kCtas) attn_chunk_kernel(
   for (int n = 0; n < kN; ++n) {
     const int row = 8 * n + g;
 #pragma unroll
-    for (int hc = 0; hc < 4; ++hc) {
+    for (int hc = 0; hc < 4 && kQInRegs<kN>; ++hc) {
       const uint4 x = lds128(base + C::kOffQ + row * 256 + (((8 * (hc >> 1) + 2 * t + (hc & 1)) ^ (row & 1)) << 4));
       qf[n][4 * hc] = x.x, qf[n][4 * hc + 1] = x.y, qf[n][4 * hc + 2] = x.z, qf[n][4 * hc + 3] = x.w;
     }
@@ -571,11 +593,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<kFmt>::kCtas) attn_chunk_kernel(
     const uint32_t sc = scale0 + (i % kStages) * kScaleBytes;
     if (c < sp.cached) {
       const int pos = c * KB;
-      chunk_step<kQuant, kFmt, kN>(st, st + kStageBytes / 2, sc, qf, back, lane, a.scale_log2,
+      chunk_step<kQuant, kFmt, kN>(st, st + kStageBytes / 2, sc, base + C::kOffQ, qf, back, lane, a.scale_log2,
                                         min(seen_by_all, sq.nc) - pos >= KB, pos, sq.nc, w);
     } else {
       const int pos = sq.nc + (c - sp.cached) * kFreshKeys;
-      chunk_step<kQuant, kFmtBf16, kN>(st, st + kStageBytes / 2, sc, qf, back, lane, a.scale_log2,
+      chunk_step<kQuant, kFmtBf16, kN>(st, st + kStageBytes / 2, sc, base + C::kOffQ, qf, back, lane, a.scale_log2,
                                             seen_by_all - pos >= kFreshKeys, pos, (int)L, w);
     }
   }
@@ -748,14 +770,14 @@ cudaError_t launch(const ChunkArgs& a, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64 || !attr_set[dev]) {
     e = cudaFuncSetAttribute(attn_chunk_kernel<kFmt, kN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)Cfg<kFmt>::kSmemBytes);
+                             (int)Cfg<kFmt, kN>::kSmemBytes);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
   const int64_t items = (int64_t)a.B * a.Hkv * a.mtiles;
   if (items * a.splits > 0x7fffffffLL) return cudaErrorInvalidValue;
   e = launch_pdl(attn_chunk_kernel<kFmt, kN>, dim3((unsigned)(items * a.splits)), dim3(kThreads),
-                 Cfg<kFmt>::kSmemBytes, stream, a);
+                 Cfg<kFmt, kN>::kSmemBytes, stream, a);
   if (e != cudaSuccess || a.splits == 1) return e;
   return launch_pdl(attn_chunk_merge_kernel<chunk_keys<kFmt>(), kFreshKeys, 8 * kN>,
                     dim3((unsigned)(items * kN)), dim3(256), 0, stream, a);
@@ -763,7 +785,10 @@ cudaError_t launch(const ChunkArgs& a, cudaStream_t stream) {
 
 template <int kFmt>
 cudaError_t launch_rows(const ChunkArgs& a, int rows, cudaStream_t stream) {
-  return rows == 8 ? launch<kFmt, 1>(a, stream) : launch<kFmt, 2>(a, stream);
+  if (rows == 8) return launch<kFmt, 1>(a, stream);
+  if (rows == 16) return launch<kFmt, 2>(a, stream);
+  if constexpr (kFmt != kFmtBf16) return launch<kFmt, 4>(a, stream);
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace chunk
@@ -773,7 +798,9 @@ ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int6
   constexpr int kDenseTiles = 4;
   ChunkPlan p = {};
   const int64_t rows = (int64_t)max_q * group;
-  p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : kChunkMmaRows;
+  // Which kernel (8 sequences of 32 heads, 32 rows over 1,144 cached ones): e4m3 41 us in attn_chunk.cu, 45 in
+  // the 128-row kernel, which expands every key for 96 idle rows; bf16 47 and 34; 64 rows, e4m3: 79 and 55.
+  p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 && format != kFmtBf16 ? 32 : kChunkMmaRows;
   if (p.rows == kChunkMmaRows) {
     // One CTA per SM. Splits only while SMs would have nothing to do, and four
     // tiles of keys at least for each.
@@ -822,7 +849,7 @@ ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int6
   // contexts are as long as the bound, and if they are 60 % of it on average
   // its mean load and the last CTA's tail: the sum of both estimates decides.
   // The merge costs four chunks and one for 16 splits.
-  const int64_t slots = (int64_t)(format == kFmtBf16 ? chunk::Cfg<kFmtBf16>::kCtas : chunk::Cfg<kFmtE4m3>::kCtas) * num_sms;
+  const int64_t slots = (int64_t)(format == kFmtBf16 || p.rows > 16 ? 2 : 3) * num_sms;  // Cfg::kCtas
   int64_t splits = 1;
   double best = 0;
   for (int64_t s = 1; items > 0 && s <= std::max<int64_t>(1, chunks / chunk::kWarps) && s <= 1024; s += std::max<int64_t>(1, s / 8)) {

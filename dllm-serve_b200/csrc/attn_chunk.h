@@ -64,7 +64,7 @@ constexpr int kChunkMmaRows = 128;  // packed rows of a tile of the tcgen05 kern
 
 // How a launch is laid out, from sizes the host knows.
 struct ChunkPlan {
-  int rows;                // packed rows of a tile: 8 or 16 (attn_chunk.cu), 128 (attn_chunk_mma.cu)
+  int rows;                // packed rows of a tile: 8, 16 or 32 (attn_chunk.cu), 128 (attn_chunk_mma.cu)
   int tile_rows, unit_rows;
   int mtiles;
   int splits;
