@@ -19,7 +19,7 @@
 //      nothing overflows; down to 2^-14 these keep 11 bits, and below that the
 //      rounding is at most 2^-25, i.e. 2^-39 of the largest |v| met once
 //      multiplied by the code and the unit. bf16 probabilities (2^-8 of p)
-//      would be further off for every value above 2^-31 of the largest.
+//      would be further off wherever p |v| is above 2^-31 of the largest |v|.
 //
 // A CTA takes one tile of packed rows (row r of the chunk for query head g of
 // the KV head's group is packed row r * group + g) and one split of the keys;
@@ -66,6 +66,9 @@ constexpr uint32_t kStageBytes = 8192;  // K half then V half
 constexpr int kFreshKeys = 16;          // keys of a bf16 chunk
 constexpr uint32_t kScaleBytes = 34 * 8;  // of a stage: 32 (K, V) scales, the largest exponent
 constexpr int kNoExp = -(1 << 30);        // no value exponent met
+// A scaled Q (below 2^15) times codes (at most 448) over 128 dimensions is below 2^31; with keys'
+// 2^e (e <= 121) lowered by this the scores stay finite, whatever the cache holds.
+constexpr float kKeyDown = 0x1p-24f;
 
 template <int kFmt>
 constexpr int chunk_keys() { return kFmt == kFmtBf16 ? 16 : 32; }
@@ -274,7 +277,11 @@ DLLM_DEVICE void chunk_step(uint32_t ks, uint32_t vs, uint32_t scales, uint32_t 
       ufac = pow2(ev - w.e);
     }
   } else if constexpr (kQuant) {
-    if (w.e == kNoExp) w.e = 0;
+    // fresh values may be of any size: their P must not exceed 1
+    if (w.e < 15) {
+      grow = w.e == kNoExp ? 1.f : pow2(w.e - 15);
+      w.e = 15;
+    }
     ufac = pow2(15 - w.e);
   }
   // masks and key factors: keys 16kt + g, 16kt + 8 + g
@@ -497,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kFmt, kN>::kCtas) attn_chunk_ker
     }
     cp_async_commit();
   };
-  // Scales of chunk i, issued by the last issue(): 2^e of each key, 2^(e - e_max + 15) of
+  // Scales of chunk i, issued by the last issue(): 2^(e - 24) of each key, 2^(e - e_max + 15) of
   // each value, then the values' largest exponent.
   auto put_scales = [&](int i) {
     if constexpr (kQuant) {
@@ -506,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kFmt, kN>::kCtas) attn_chunk_ker
         const int ev = (int)pend_v - 127;
         const bool live = pend_v != 0 && pend_v != kNanByte;
         const int hi = __reduce_max_sync(0xffffffffu, live ? ev : kNoExp);
-        const float2 x = make_float2(exp_scale(pend_k), live ? pow2(ev - hi + 15) : exp_scale(pend_v));
+        const float2 x = make_float2(exp_scale(pend_k) * kKeyDown, live ? pow2(ev - hi + 15) : exp_scale(pend_v));
         asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at + lane * 8), "f"(x.x), "f"(x.y) : "memory");
         if (lane == 0) asm volatile("st.shared.s32 [%0], %1;" ::"r"(at + 32 * 8), "r"(hi) : "memory");
       }
@@ -572,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kFmt, kN>::kCtas) attn_chunk_ker
       w.m[n][r] = -INFINITY;
       w.l[n][r] = 0.f;
       w.seen[n][r] = (int)(a.causal ? min(L, max((int64_t)0, L - sq.Lq + i + 1)) : L);
-      w.rf[n][r] = kQuant ? a.scale_log2 * factor[p] : a.scale_log2;
+      w.rf[n][r] = kQuant ? a.scale_log2 / kKeyDown * factor[p] : a.scale_log2;
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j)

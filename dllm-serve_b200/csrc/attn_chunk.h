@@ -29,7 +29,9 @@ struct ChunkArgs {
   int max_blocks;          // entries of a table row
   int block_size;          // slots of a block
   int block_shift;         // log2(block_size), or -1
-  const int32_t* ctx;      // cached rows per sequence (with tables)
+  const int32_t* ctx;      // with tables: sequence b has ctx[b] - (ctx_base[b] & ctx_mask) cached rows
+  const int32_t* ctx_base;
+  int ctx_mask;            // 0 (lengths) or -1 (running sums)
   int max_context;         // no sequence has more cached rows
   const int32_t* cu_q;
   const int32_t* cu_k;     // fresh rows per sequence, or null

@@ -377,7 +377,7 @@ int check_chunk_sizes(int format, int batch, int Hq, int Hkv, int max_q, int max
   if (Hq / Hkv > 128) return fail(DLLM_ERR_UNSUPPORTED, "%d query heads per KV head (at most 128)", Hq / Hkv);
   if (batch < 0 || max_q < 0 || max_context < 0 || max_fresh < 0)
     return fail(DLLM_ERR_INVALID_ARG, "negative size");
-  if (max_context > (1 << 30) || max_fresh > (1 << 30) || (int64_t)max_q * (Hq / Hkv) > (1 << 30))
+  if ((int64_t)max_context + max_fresh > (1 << 30) || (int64_t)max_q * (Hq / Hkv) > (1 << 30))
     return fail(DLLM_ERR_TOO_LARGE, "more than 2^30 rows of a sequence");
   return DLLM_OK;
 }
@@ -509,6 +509,16 @@ int64_t dllm_attn_chunk_workspace(int format, int batch, int num_heads, int num_
       .workspace_bytes;
 }
 
+int dllm_attn_chunk_launches(int format, int batch, int num_heads, int num_kv_heads, int max_seqlen_q,
+                             int max_context, int max_fresh) {
+  if (check_chunk_sizes(format, batch, num_heads, num_kv_heads, max_seqlen_q, max_context, max_fresh) != DLLM_OK)
+    return -1;
+  if (batch == 0 || max_seqlen_q == 0) return 0;
+  const dllm::ChunkPlan p = dllm::plan_attn_chunk(format, batch, num_kv_heads, num_heads / num_kv_heads, max_seqlen_q, 0,
+                                                  max_context, max_fresh, num_sms_of_current_device());
+  return 1 + (p.dense > 0) + (p.splits > 1);
+}
+
 int dllm_attn_chunk_fwd(const dllm_chunk_args* args) {
   if (args == nullptr) return fail(DLLM_ERR_INVALID_ARG, "args is null");
   const dllm_chunk_args& p = *args;
@@ -532,21 +542,24 @@ int dllm_attn_chunk_fwd(const dllm_chunk_args* args) {
     return fail(DLLM_ERR_INVALID_ARG, "block tables and a slot list are both given");
   const bool cached = block_tables != nullptr || slots != nullptr;
   if (block_tables != nullptr) {
-    if (p.context_lens == nullptr) return fail(DLLM_ERR_INVALID_ARG, "block_tables without context_lens");
+    if ((p.context_lens == nullptr) == (p.cu_seqlens_slots == nullptr))
+      return fail(DLLM_ERR_INVALID_ARG, "block_tables need context_lens or cu_seqlens_slots");
     if (block_size <= 0 || max_blocks < 0 || p.table_stride < max_blocks)
       return fail(DLLM_ERR_INVALID_ARG, "bad block table shape");
   }
   if (slots != nullptr && p.cu_seqlens_slots == nullptr)
     return fail(DLLM_ERR_INVALID_ARG, "slots without cu_seqlens_slots");
   if (cached && (k_cache == nullptr || v_cache == nullptr)) return fail(DLLM_ERR_INVALID_ARG, "cache is null");
+  if (cached && num_slots == 0) return fail(DLLM_ERR_INVALID_ARG, "the cache has no slots");
   if (cached && format != DLLM_KV_BF16 && (k_exp == nullptr || v_exp == nullptr))
     return fail(DLLM_ERR_INVALID_ARG, "a quantised cache needs k_exp and v_exp");
   if (!aligned(k_cache, 16) || !aligned(v_cache, 16))
     return fail(DLLM_ERR_ALIGNMENT, "caches must be 16-byte aligned");
   if ((k == nullptr) != (v == nullptr) || (k == nullptr) != (p.cu_seqlens_k == nullptr))
     return fail(DLLM_ERR_INVALID_ARG, "k, v and cu_seqlens_k are given together");
+  if (p.cu_seqlens_q == nullptr && max_seqlen_q != 1)
+    return fail(DLLM_ERR_INVALID_ARG, "cu_seqlens_q is null: every sequence has one row, max_seqlen_q must be 1");
   if (batch == 0 || total_q == 0 || max_seqlen_q == 0) return DLLM_OK;
-  if (p.cu_seqlens_q == nullptr) return fail(DLLM_ERR_INVALID_ARG, "cu_seqlens_q is null");
   if ((rc = check_rows("q", q, q_tok_stride, num_heads, total_q)) != DLLM_OK) return rc;
   if ((rc = check_rows("o", p.o, o_tok_stride, num_heads, total_q)) != DLLM_OK) return rc;
   if (k != nullptr) {
@@ -586,7 +599,9 @@ int dllm_attn_chunk_fwd(const dllm_chunk_args* args) {
   a.block_shift = -1;
   for (int s = 0; s < 31; ++s)
     if (a.block_size == 1 << s) a.block_shift = s;
-  a.ctx = p.context_lens;
+  a.ctx = p.context_lens != nullptr ? p.context_lens : p.cu_seqlens_slots + 1;
+  a.ctx_base = p.context_lens != nullptr ? p.context_lens : p.cu_seqlens_slots;
+  a.ctx_mask = p.context_lens != nullptr ? 0 : -1;
   a.max_context = max_context;
   a.cu_q = p.cu_seqlens_q;
   a.cu_k = p.cu_seqlens_k;
@@ -607,7 +622,7 @@ int dllm_attn_chunk_fwd(const dllm_chunk_args* args) {
   if (plan.rows == dllm::kChunkMmaRows) {
     const int group = num_heads / num_kv_heads;
     if ((rc = encode_rows_map(&maps.q, q, total_q, num_heads, q_tok_stride, 128 / group, group)) != DLLM_OK) return rc;
-    if (k != nullptr) {
+    if (k != nullptr && total_k > 0) {
       if ((rc = encode_rows_map(&maps.k, k, total_k, num_kv_heads, k_tok_stride, 128)) != DLLM_OK) return rc;
       if ((rc = encode_rows_map(&maps.v, v, total_k, num_kv_heads, v_tok_stride, 128)) != DLLM_OK) return rc;
     }

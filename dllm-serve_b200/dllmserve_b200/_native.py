@@ -56,6 +56,7 @@ SIGNATURES = {
         _I,
     ),
     "dllm_attn_chunk_workspace": ([_I, _I, _I, _I, _I, _I, _I], _I64),
+    "dllm_attn_chunk_launches": ([_I, _I, _I, _I, _I, _I, _I], _I),
     "dllm_attn_chunk_fwd": ([ctypes.c_char_p], _I),  # a packed dllm_chunk_args
     "dllm_attn_varlen_fwd": (
         [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I, _I, _I64, _I64, _I, _I, _I, _F, _P, _P, _P],

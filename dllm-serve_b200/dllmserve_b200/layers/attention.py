@@ -124,30 +124,15 @@ class Attention(nn.Module):
             return o.view(-1, H * self.head_dim)
         if tables is None:
             raise ValueError("a decode step needs context.block_tables")
+        # (max_context None: what the tables hold)
         if context.is_prefill:
-            cu_q, max_q = context.cu_seqlens_q, int(context.max_seqlen_q)
-            lens, most = self._per_step(context, "lens", lambda: torch.diff(context.cu_seqlens_k)), int(context.max_seqlen_k)
+            o = ops.chunk_attention(q, self.k_cache, self.v_cache, context.cu_seqlens_q, int(context.max_seqlen_q), self.scale,
+                                    causal=self.causal, block_tables=tables, cu_seqlens_slots=context.cu_seqlens_k,
+                                    max_context=int(context.max_seqlen_k) or None, k_exp=self.k_exp, v_exp=self.v_exp)
         else:
-            cu_q = self._per_step(context, "ones", lambda: torch.arange(q.shape[0] + 1, dtype=torch.int32, device=q.device))
-            max_q, lens, most = 1, context.context_lens, 0
-        o = ops.chunk_attention(q, self.k_cache, self.v_cache, cu_q, max_q, self.scale, causal=self.causal,
-                                block_tables=tables, context_lens=lens, max_context=most or None,
-                                k_exp=self.k_exp, v_exp=self.v_exp)
+            o = ops.chunk_attention(q, self.k_cache, self.v_cache, None, 1, self.scale, causal=self.causal,
+                                    block_tables=tables, context_lens=context.context_lens, k_exp=self.k_exp, v_exp=self.v_exp)
         return o.view(-1, H * self.head_dim)
-
-    @staticmethod
-    def _per_step(context, name, make):
-        """A device array derived from the step's context, made by its first layer."""
-        cache = getattr(context, _PLAN_ATTR + "_regular", None)
-        if cache is None:
-            cache = {}
-            try:
-                setattr(context, _PLAN_ATTR + "_regular", cache)
-            except AttributeError:  # a frozen context: rebuild per layer
-                pass
-        if name not in cache:
-            cache[name] = make()
-        return cache[name]
 
     def _diffusion_attention(self, q, k, v, context):
         """q [N, num_heads*D] or [N, num_heads, D]; k, v likewise with

@@ -222,8 +222,9 @@ def _kv_quant(store, key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping):
     if key.dtype is not torch.bfloat16 or value.dtype is not torch.bfloat16:
         raise ValueError("key and value must be bfloat16")
     ks, vs = key.stride(), value.stride()
-    if ks[2] != 1 or ks[1] != D or vs[2] != 1 or vs[1] != D:
+    if ks[2] != 1 or vs[2] != 1 or ((ks[1] != D or vs[1] != D) and H != 1):
         raise ValueError("key and value must have contiguous heads")
+    k_str, v_str = (ks[0], vs[0]) if N > 1 else (H * D, H * D)  # (one row: any stride will do)
     dev = _same_device(key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping)
     fmt = _KV_FORMATS.get(k_cache.dtype, _native.KV_BF16)
     if fmt == _native.KV_BF16 or v_cache.dtype is not k_cache.dtype:
@@ -239,11 +240,11 @@ def _kv_quant(store, key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping):
     fn = lib.dllm_store_kvcache_quant if store else lib.dllm_load_kvcache_quant
     if dev != _current_device():
         with torch.cuda.device(dev):
-            rc = fn(key.data_ptr(), ks[0], value.data_ptr(), vs[0], k_cache.data_ptr(), v_cache.data_ptr(),
+            rc = fn(key.data_ptr(), k_str, value.data_ptr(), v_str, k_cache.data_ptr(), v_cache.data_ptr(),
                     k_exp.data_ptr(), v_exp.data_ptr(), slot_mapping.data_ptr(), N, H, D, fmt, slots,
                     _status_ptr_of(dev), _stream_ptr())
     else:
-        rc = fn(key.data_ptr(), ks[0], value.data_ptr(), vs[0], k_cache.data_ptr(), v_cache.data_ptr(),
+        rc = fn(key.data_ptr(), k_str, value.data_ptr(), v_str, k_cache.data_ptr(), v_cache.data_ptr(),
                 k_exp.data_ptr(), v_exp.data_ptr(), slot_mapping.data_ptr(), N, H, D, fmt, slots,
                 _status_ptr_of(dev), _stream_ptr())
     if rc:
@@ -597,14 +598,14 @@ def _varlen_attention_rope(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, so
 # ---------------------------------------------------------------------------
 # Attention of a chunk over a paged cache (attention.py:121-148)
 # ---------------------------------------------------------------------------
-_CHUNK_WS: dict = {}  # workspace bytes by launch sizes
+_CHUNK_WS: dict = {}  # (workspace bytes, kernels) by launch sizes
 
 
 def chunk_attention(
     q: torch.Tensor,
     k_cache: torch.Tensor | None,
     v_cache: torch.Tensor | None,
-    cu_seqlens_q: torch.Tensor,
+    cu_seqlens_q: torch.Tensor | None,
     max_seqlen_q: int,
     softmax_scale: float | None = None,
     *,
@@ -625,13 +626,15 @@ def chunk_attention(
     """Attention of a chunk of new tokens over a paged KV cache.
 
     q: bfloat16 [total_q, num_heads, 128], the sequences' chunks one after
-    another (``cu_seqlens_q`` int32 [B+1], none longer than ``max_seqlen_q``).
+    another (``cu_seqlens_q`` int32 [B+1], none longer than ``max_seqlen_q``;
+    None: one row per sequence).
     The keys of a sequence are its cached rows followed by its fresh rows:
 
     * cached rows, from k_cache / v_cache [blocks, block_size, num_kv_heads,
       128]: either ``block_tables`` (int32 [B, max_blocks]) with
-      ``context_lens`` (int32 [B]), or ``slots`` (int32) with
-      ``cu_seqlens_slots`` (int32 [B+1]), or neither (no cached rows).
+      ``context_lens`` (int32 [B]) or the lengths' sums ``cu_seqlens_slots``
+      (int32 [B+1]), or ``slots`` (int32) with ``cu_seqlens_slots``, or
+      neither (no cached rows).
       ``max_context`` bounds the cached rows of a sequence (default: what the
       table, or the slot list, can hold); the closer it is, the better the
       work is spread. The cache is bfloat16, or float8_e4m3fn / int8 with the
@@ -651,10 +654,14 @@ def chunk_attention(
         raise ValueError("no keys: give block_tables, slots or fresh k and v")
     if cached and (k_cache is None or v_cache is None):
         raise ValueError("block_tables / slots need k_cache and v_cache")
-    dev = _same_device(q, cu_seqlens_q)
-    B = cu_seqlens_q.numel() - 1
-    _check_cu("cu_seqlens_q", cu_seqlens_q, B, dev)
     max_q = int(max_seqlen_q)
+    if cu_seqlens_q is None:
+        if max_q != 1:
+            raise ValueError("without cu_seqlens_q every sequence has one row: max_seqlen_q must be 1")
+        dev, B, cu_q_ptr = _same_device(q), q.shape[0], 0
+    else:
+        dev, B, cu_q_ptr = _same_device(q, cu_seqlens_q), cu_seqlens_q.numel() - 1, cu_seqlens_q.data_ptr()
+        _check_cu("cu_seqlens_q", cu_seqlens_q, B, dev)
     fmt = _native.KV_BF16
     k_ptr = v_ptr = cu_k_ptr = kx_ptr = vx_ptr = kc_ptr = vc_ptr = k_str = v_str = total_k = num_slots = max_fresh = 0
     bt_ptr = ctx_ptr = sl_ptr = cus_ptr = table_stride = max_blocks = block_size = total_slots = most = 0
@@ -667,10 +674,13 @@ def chunk_attention(
         if k.get_device() != dev or v.get_device() != dev:
             raise ValueError("all tensors must be on the same device")
         _check_cu("cu_seqlens_k", cu_seqlens_k, B, dev)
-        k_ptr, v_ptr, cu_k_ptr = k.data_ptr(), v.data_ptr(), cu_seqlens_k.data_ptr()
-        max_fresh = max_q if max_seqlen_k is None else int(max_seqlen_k)
+        if total_k > 0:
+            k_ptr, v_ptr, cu_k_ptr = k.data_ptr(), v.data_ptr(), cu_seqlens_k.data_ptr()
+            max_fresh = max_q if max_seqlen_k is None else int(max_seqlen_k)
+    elif k_cache.dim() != 4:
+        raise ValueError(f"caches must be contiguous [blocks, block_size, num_kv_heads, {D}]")
     else:
-        Hkv = k_cache.shape[-2]
+        Hkv = k_cache.shape[2]
     if cached:
         fmt = _KV_FORMATS.get(k_cache.dtype)
         if fmt is None or v_cache.dtype is not k_cache.dtype:
@@ -699,12 +709,19 @@ def chunk_attention(
             if (block_tables.dtype is not torch.int32 or len(sh) != 2 or sh[0] != B
                     or block_tables.get_device() != dev or (sh[1] > 1 and st[1] != 1)):
                 raise ValueError(f"block_tables must be int32 [{B}, max_blocks] with contiguous rows")
-            if (context_lens is None or context_lens.dtype is not torch.int32 or context_lens.numel() != B
-                    or not context_lens.is_contiguous() or context_lens.get_device() != dev):
-                raise ValueError(f"context_lens must be contiguous int32 [{B}]")
+            if (context_lens is None) == (cu_seqlens_slots is None):
+                raise ValueError("block_tables need either context_lens or cu_seqlens_slots")
+            if context_lens is None:
+                _check_cu("cu_seqlens_slots", cu_seqlens_slots, B, dev)
+                cus_ptr = cu_seqlens_slots.data_ptr()
+            else:
+                if (context_lens.dtype is not torch.int32 or context_lens.numel() != B
+                        or not context_lens.is_contiguous() or context_lens.get_device() != dev):
+                    raise ValueError(f"context_lens must be contiguous int32 [{B}]")
+                ctx_ptr = context_lens.data_ptr()
             max_blocks = sh[1]
             table_stride = st[0] if B > 1 else max(max_blocks, st[0])
-            bt_ptr, ctx_ptr = block_tables.data_ptr(), context_lens.data_ptr()
+            bt_ptr = block_tables.data_ptr()
             most = max_blocks * block_size
         else:
             if slots.dtype is not torch.int32 or slots.dim() != 1 or not slots.is_contiguous() or slots.get_device() != dev:
@@ -718,7 +735,7 @@ def chunk_attention(
             most = min(int(max_context), most)
     if out is None:
         out = torch.empty_like(q)
-        o_str = out.stride(0)
+        o_str = out.stride(0) if q.shape[0] > 1 else Hq * D
     else:
         Ho, Do, o_str = _chunk_rows("out", out)
         if Ho != Hq or Do != D or out.shape[0] != q.shape[0] or out.get_device() != dev:
@@ -731,13 +748,13 @@ def chunk_attention(
             launches = _chunk_launch(
                 dev, args, out, (q.data_ptr(), q_str, k_ptr, k_str, v_ptr, v_str, kc_ptr, vc_ptr, kx_ptr, vx_ptr, num_slots, bt_ptr,
                                  table_stride, ctx_ptr, sl_ptr, cus_ptr, total_slots, out.data_ptr(), o_str,
-                                 cu_seqlens_q.data_ptr(), cu_k_ptr, q.shape[0], total_k),
+                                 cu_q_ptr, cu_k_ptr, q.shape[0], total_k),
                 max_blocks, block_size, D, causal, softmax_scale)
     else:
         launches = _chunk_launch(
             dev, args, out, (q.data_ptr(), q_str, k_ptr, k_str, v_ptr, v_str, kc_ptr, vc_ptr, kx_ptr, vx_ptr, num_slots, bt_ptr,
                              table_stride, ctx_ptr, sl_ptr, cus_ptr, total_slots, out.data_ptr(), o_str,
-                             cu_seqlens_q.data_ptr(), cu_k_ptr, q.shape[0], total_k),
+                             cu_q_ptr, cu_k_ptr, q.shape[0], total_k),
             max_blocks, block_size, D, causal, softmax_scale)
     if B > 0 and max_q > 0 and q.shape[0] > 0:
         LAUNCHES[0] += launches
@@ -758,25 +775,26 @@ def _chunk_launch(dev, sizes, out, pointers, max_blocks, block_size, D, causal, 
             _native.check(code, "chunk_attention")
         if len(_CHUNK_WS) > 4096:
             _CHUNK_WS.clear()
-        plan = _CHUNK_WS[(sizes, dev)] = need
+        plan = _CHUNK_WS[(sizes, dev)] = (need, lib.dllm_attn_chunk_launches(*sizes))
+    need, launches = plan
     # allocated per call on the current stream, so overlapping launches never share it
-    ws = torch.empty(plan, dtype=torch.uint8, device=out.device) if plan > 0 else None
+    ws = torch.empty(need, dtype=torch.uint8, device=out.device) if need > 0 else None
     rc = lib.dllm_attn_chunk_fwd(_native.CHUNK_ARGS.pack(
-        *pointers, 0 if ws is None else ws.data_ptr(), plan, _status_ptr_of(dev), _stream_ptr(), fmt, max_blocks,
+        *pointers, 0 if ws is None else ws.data_ptr(), need, _status_ptr_of(dev), _stream_ptr(), fmt, max_blocks,
         block_size, max_context, B, max_q, max_fresh, Hq, Hkv, D, 1 if causal else 0,
         D ** -0.5 if softmax_scale is None else softmax_scale))
     if rc:
         _native.check(rc, "chunk_attention")
-    return 1 if ws is None else 2
+    return launches
 
 
 def _chunk_rows(name, t):
     """(heads, head_dim, token stride) of a bfloat16 [rows, heads, head_dim] with
     contiguous heads."""
     sh, st = t.shape, t.stride()
-    if len(sh) != 3 or t.dtype is not torch.bfloat16 or st[2] != 1 or st[1] != sh[2]:
+    if len(sh) != 3 or t.dtype is not torch.bfloat16 or st[2] != 1 or (st[1] != sh[2] and sh[1] != 1):
         raise ValueError(f"{name} must be bfloat16 [rows, heads, head_dim] with contiguous heads, got {t.dtype} {tuple(sh)}")
-    return sh[1], sh[2], st[0]
+    return sh[1], sh[2], st[0] if sh[0] > 1 else sh[1] * sh[2]  # (one row: any stride will do)
 
 
 def _check_cu(name, c, B, dev):

@@ -174,9 +174,11 @@ DLLM_API int dllm_load_kvcache_quant(void* key, int64_t key_stride, void* value,
  * Attention.forward (attention.py:121-148), flash_attn_varlen_func(causal=True,
  * block_table=...) and flash_attn_with_kvcache(...).
  *
- * The keys of sequence b are [its C_b cached rows ; its F_b fresh rows]:
+ * The chunk of sequence b is rows cu_seqlens_q[b] .. cu_seqlens_q[b+1] of q, or row b
+ * (cu_seqlens_q null: decode). Its keys are [its C_b cached rows ; its F_b fresh rows]:
  *   cached, by block table: row p is slot block_tables[b * table_stride + p / block_size]
- *     * block_size + p % block_size, C_b = context_lens[b] <= max_context; table rows
+ *     * block_size + p % block_size, C_b = context_lens[b], or (context_lens null)
+ *     cu_seqlens_slots[b+1] - cu_seqlens_slots[b], at most max_context; table rows
  *     have max_blocks entries, of which only the first ceil(C_b / block_size) are read;
  *   cached, by slot list: row p is slots[cu_seqlens_slots[b] + p] (total_slots entries),
  *     C_b <= max_context;
@@ -186,7 +188,7 @@ DLLM_API int dllm_load_kvcache_quant(void* key, int64_t key_stride, void* value,
  * With causal != 0 query row i of the chunk's Lq rows sees the first C_b + F_b - Lq + i + 1
  * keys (the chunk's rows are the last Lq positions), else all of them. A row that sees no
  * key is zero. Values at positions that a row does not see must be finite within the
- * sequence's own keys; slots of no key of the sequence are not read.
+ * sequence's own keys; what other slots hold does not matter.
  *
  * format: DLLM_KV_*; k_exp / v_exp as in dllm_store_kvcache_quant (null for bf16). Cache
  * rows are num_kv_heads * 128 elements, num_slots of them. Slots or blocks out of range
@@ -195,8 +197,9 @@ DLLM_API int dllm_load_kvcache_quant(void* key, int64_t key_stride, void* value,
  * q, o: [total_q, num_heads, 128]; head_dim must be 128; num_heads a multiple of, and at
  * most 128 times, num_kv_heads; max_seqlen_q bounds every Lq.
  *
- * workspace: device memory of at least dllm_attn_chunk_workspace(...) bytes, 16-byte
- * aligned, whose contents need not be set; null if that is 0. Launches that may overlap
+ * workspace: device memory of at least dllm_attn_chunk_workspace(...) bytes (max_context,
+ * max_fresh: 0 where the launch has no such keys), 16-byte aligned, whose contents need
+ * not be set; null if that is 0. Launches that may overlap
  * need distinct ones. The result does not depend on the launch's timing (splits are
  * merged in order).
  */
@@ -244,6 +247,9 @@ typedef struct dllm_chunk_args {
 
 DLLM_API int64_t dllm_attn_chunk_workspace(int format, int batch, int num_heads, int num_kv_heads,
                                            int max_seqlen_q, int max_context, int max_fresh);
+/* the number of kernels that a launch of these sizes consists of */
+DLLM_API int dllm_attn_chunk_launches(int format, int batch, int num_heads, int num_kv_heads, int max_seqlen_q,
+                                      int max_context, int max_fresh);
 DLLM_API int dllm_attn_chunk_fwd(const dllm_chunk_args* args);
 
 /*

@@ -535,7 +535,12 @@ def test_refusals():
     assert call(ke=0) == E.DLLM_ERR_INVALID_ARG
     assert call(kc=72) == E.DLLM_ERR_ALIGNMENT
     assert call(k=64) == E.DLLM_ERR_INVALID_ARG                # k without v
-    assert call(cuq=0) == E.DLLM_ERR_INVALID_ARG
+    assert call(cuq=0, mq=2, wb=1 << 40, ws=64) == E.DLLM_ERR_INVALID_ARG  # without offsets: one row per sequence
+    assert "max_seqlen_q" in lib.dllm_last_error().decode()
+    assert call(slots_n=0) == E.DLLM_ERR_INVALID_ARG
+    assert call(ctx=0, cus=0) == E.DLLM_ERR_INVALID_ARG
+    assert call(ctx=64, cus=64) == E.DLLM_ERR_INVALID_ARG
+    assert call(mc=2 ** 29 + 1, mf=2 ** 29) == E.DLLM_ERR_TOO_LARGE
     assert call(q=72) == E.DLLM_ERR_ALIGNMENT
     assert call(qs=516) == E.DLLM_ERR_ALIGNMENT
     assert call(os=500) == E.DLLM_ERR_INVALID_ARG
@@ -548,6 +553,11 @@ def test_refusals():
     assert ws(1, 1, 4, 4, 1, 100000, 0) > 0
     assert ws(1, 64, 32, 32, 1, 64, 0) == 0
     assert ws(9, 1, 4, 4, 1, 64, 0) == -1
+    kernels = lib.dllm_attn_chunk_launches
+    assert kernels(1, 1, 4, 4, 1, 100000, 0) == 2                # splits and their merge
+    assert kernels(1, 64, 32, 32, 1, 64, 0) == 1
+    assert kernels(1, 1, 4, 4, 512, 100000, 0) == 3              # the expanded copy, splits, merge
+    assert kernels(9, 1, 4, 4, 1, 64, 0) == -1
     q = torch.zeros(1, 4, 128, dtype=torch.bfloat16)
     cu = torch.tensor([0, 1], dtype=torch.int32)
     with pytest.raises(ValueError, match="no keys"):
@@ -588,3 +598,99 @@ def test_refusals_on_device_tensors(dev):
     y = torch.zeros(3, 4, 64, dtype=torch.bfloat16, device=dev)
     with pytest.raises(NotImplementedError):
         ops.chunk_attention(y, None, None, cu, 2, k=y, v=y, cu_seqlens_k=cu)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3", "int8"])
+def test_one_row_per_sequence_and_summed_lengths(dev, fmt):
+    """cu_seqlens_q None: row b is sequence b's; lengths as running sums. Both
+    give the bits of the arrays they stand for."""
+    ops = _ops()
+    c = Case(82, fmt, 12, 4, [1] * 5, [70, 0, 300, 16, 31], None, True)
+    args, kw = c.args(dev)
+    q = args[0][:5]
+    want = ops.chunk_attention(q, *args[1:], **kw)
+    c.check(want, True)
+    assert torch.equal(ops.chunk_attention(q, *args[1:3], None, 1, **kw), want)
+    sums = {k: v for k, v in kw.items() if k != "context_lens"} | {"cu_seqlens_slots": _cu(c.nc).to(dev)}
+    assert torch.equal(ops.chunk_attention(q, *args[1:], **sums), want)
+    assert torch.equal(ops.chunk_attention(q, *args[1:3], None, 1, **sums), want)
+    assert ops.read_device_status(dev) == 0
+    with pytest.raises(ValueError, match="max_seqlen_q"):
+        ops.chunk_attention(q, *args[1:3], None, 2, **kw)
+    with pytest.raises(ValueError, match="either"):
+        ops.chunk_attention(q, *args[1:3], None, 1, **kw, cu_seqlens_slots=sums["cu_seqlens_slots"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("nq", [2, 40])
+def test_nothing_to_read(dev, fmt, nq):
+    """Fresh rows, slot list or table of length zero: the other keys, or zero rows."""
+    ops = _ops()
+    c = Case(83, fmt, 8, 2, [nq, nq], [50, 9], [nq, nq], False)
+    args, kw = c.args(dev)
+    zero = torch.zeros(3, dtype=torch.int32, device=dev)
+    none = {"k": kw["k"][:0], "v": kw["v"][:0], "cu_seqlens_k": zero}
+    full, c.nf, c.k = c.k, [0, 0], None
+    out = ops.chunk_attention(*args, causal=False, **{**kw, **none})
+    c.check(out, False)
+    c.k, c.nf = full, [nq, nq]
+    out = ops.chunk_attention(*args, causal=False, **{**kw, "slots": kw["slots"][:0], "cu_seqlens_slots": zero})
+    c.lists = [x[:0] for x in c.lists]
+    c.check(out, False)
+    table = torch.zeros(2, 0, dtype=torch.int32, device=dev)
+    rest = {k: kw[k] for k in ("k_exp", "v_exp")}
+    for keys in ({**kw, **none, "slots": kw["slots"][:0], "cu_seqlens_slots": zero},
+                 {**rest, "block_tables": table, "context_lens": zero[:2]}):
+        out = torch.full(c.q.shape, 5.0, dtype=torch.bfloat16, device=dev)
+        ops.chunk_attention(*args, causal=False, out=out, **keys)
+        assert (out[:2 * nq] == 0).all() and (out[2 * nq:] == 5).all()
+    empty = torch.zeros(3, 8, D, dtype=torch.bfloat16, device=dev)[:0]
+    assert ops.chunk_attention(empty, *args[1:3], zero, 1, **kw).shape == empty.shape
+    assert ops.read_device_status(dev) == 0
+
+
+@pytest.mark.gpu
+def test_layouts_of_a_single_row_or_head(dev):
+    """A length-one dimension may have any stride."""
+    ops = _ops()
+    c = Case(84, "int8", 6, 1, [1], [40], [1], True)
+    args, kw = c.args(dev)
+    q = args[0][:1].clone().as_strided((1, 6, D), (D, D, 1))
+    k, v = (x.clone().as_strided((1, 1, D), (3, 5, 1)) for x in (kw["k"], kw["v"]))
+    want = ops.chunk_attention(args[0][:1], *args[1:], **kw)
+    c.check(want, True)
+    assert torch.equal(ops.chunk_attention(q, *args[1:], **{**kw, "k": k, "v": v}), want)
+    more = torch.randn(1, 5, D, generator=I.gen(3)).to(torch.bfloat16).to(dev).transpose(0, 1)  # [5, 1, D], stride 5 D
+    assert more.stride(1) == 5 * D
+    kc, ke = kw["k_exp"].clone().zero_(), kw["k_exp"]
+    slots = torch.arange(5, dtype=torch.int32, device=dev)
+    caches = [torch.zeros_like(args[1]) for _ in range(4)]
+    ops.store_kvcache_quant(more, more, *caches[:2], kc, ke.clone(), slots)
+    ke2, ve2 = torch.zeros_like(ke), torch.zeros_like(ke)
+    ops.store_kvcache_quant(more.contiguous(), more.contiguous(), *caches[2:], ke2, ve2, slots)
+    assert torch.equal(caches[0].flatten()[:5 * D], caches[2].flatten()[:5 * D])
+    assert torch.equal(kc.flatten()[:5], ke2.flatten()[:5])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("nq", [1, 20, 60])
+def test_sizes_at_the_ends_of_the_range(dev, fmt, nq):
+    """Cached values of 2^-88 with fresh ones of 2^20 and 2^100 (the outputs'
+    unit), and keys of 2^115 against queries of 2^-115 (the scores)."""
+    for dv, df, dk in ((-88, 20, 0), (-88, 100, 0), (0, 100, 0), (100, -90, 0), (0, 0, 115)):
+        c = Case(85, fmt, 4, 2, [nq, 1], [200, 33], [nq, 1], False)
+        up = lambda t, e: (t.double() * 2.0 ** e).to(torch.bfloat16)  # noqa: E731
+        c.v = up(c.v, df)
+        c.q, c.k = up(c.q, -dk), up(c.k, dk)
+        for i, e in ((0, dk), (1, dv)):
+            used = c.slots.long()
+            byte = c.exps[i].view(-1, 2)[used].int() + e
+            assert byte.min() >= 27 and byte.max() <= 246
+            c.exps[i].view(-1, 2)[used] = byte.to(torch.uint8)
+            c.values[i][used] *= 2.0 ** e
+        args, kw = c.args(dev)
+        for causal in (True, False):
+            c.check(_ops().chunk_attention(*args, causal=causal, **kw), causal)

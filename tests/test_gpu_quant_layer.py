@@ -197,3 +197,83 @@ def test_selection_into_a_quantised_cache_edges(dev):
     with pytest.raises(ValueError):
         ops.select_kv_store(q, k, v, desc, 32, True, layer.k_cache, layer.v_cache.view(torch.uint8), slots,
                             k_exp=layer.k_exp, v_exp=layer.v_exp)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("chunk", [True, False])
+@pytest.mark.parametrize("warm", [True, False])
+def test_captured_step_follows_its_buffers(dev, fmt, chunk, warm):
+    """A step captured into a graph, replayed after its lengths, tables, slots
+    and rows were changed in place, gives what an eager step on them gives;
+    ``warm``: the same context ran eagerly first. An eager step on the captured
+    context afterwards gives it too."""
+    from dllmserve_b200 import ops
+    from dllmserve_b200.utils.context import get_context, reset_context, set_context, use_context
+
+    g = I.gen(9)
+    hq, hk, page, pages = 8, 2, 16, 12
+    layers = [_layer(fmt, hq, hk, pages, page, dev, causal=True) for _ in range(2)]
+    rows = [[5, 3], [2, 6]] if chunk else [[1, 1], [1, 1]]
+    total = [[37, 20], [50, 44]]
+    tables = torch.randperm(pages, generator=g).view(2, 6).int()
+    data = []
+    for step, tot in zip(rows, total):
+        slots = torch.cat([tables[b][torch.arange(t - s, t) // page] * page + torch.arange(t - s, t) % page
+                           for b, (s, t) in enumerate(zip(step, tot))]).int()
+        x = [I.normal(g, (sum(step), h * D)).to(torch.bfloat16).to(dev) for h in (hq, hk, hk)]
+        data.append((x, slots.to(dev), _cu(step, dev), _cu(tot, dev), torch.tensor(tot, dtype=torch.int32, device=dev)))
+    fill = [I.normal(g, (pages * page, hk, D)).to(torch.bfloat16).to(dev) for _ in range(2)]
+    every = torch.arange(pages * page, dtype=torch.int32, device=dev)
+    for layer in layers:
+        if fmt == "bf16":
+            layer.k_cache.view(-1, hk, D).copy_(fill[0])
+            layer.v_cache.view(-1, hk, D).copy_(fill[1])
+        else:
+            ops.store_kvcache_quant(*fill, layer.k_cache, layer.v_cache, layer.k_exp, layer.v_exp, every)
+
+    def enter(slots, cu_q, cu_k, ctx):
+        if chunk:
+            set_context(True, cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, max_seqlen_q=8, max_seqlen_k=64, slot_mapping=slots,
+                        block_tables=tables.to(dev))
+        else:
+            set_context(False, slot_mapping=slots, context_lens=ctx, block_tables=tables.to(dev))
+
+    want = []
+    for x, *meta in data:
+        enter(*meta)
+        want.append(layers[0](*x))
+        reset_context()
+    x, *meta = [[t.clone() for t in data[0][0]]] + [t.clone() for t in data[0][1:]]
+    enter(*meta)
+    ctx = get_context()
+    if warm:
+        assert torch.equal(layers[1](*x), want[0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layers[1](*x)
+    graph.replay()
+    assert torch.equal(out, want[0])
+    for have, new in zip(x + meta, data[1][0] + list(data[1][1:])):
+        have.copy_(new)
+    graph.replay()
+    assert torch.equal(out, want[1])
+    reset_context()
+    use_context(ctx)
+    assert torch.equal(layers[1](*x), want[1])
+    reset_context()
+    assert ops.read_device_status(dev) == 0
+
+
+def test_decode_without_a_cache_is_refused(dev):
+    from dllmserve_b200.layers.attention import Attention
+    from dllmserve_b200.utils.context import reset_context, set_context
+
+    layer = Attention(4, D, D ** -0.5, 4)
+    x = torch.zeros(1, 4 * D, dtype=torch.bfloat16, device=dev)
+    one = torch.ones(1, dtype=torch.int32, device=dev)
+    for tables in (None, torch.zeros(1, 1, dtype=torch.int32, device=dev)):
+        set_context(False, slot_mapping=one, context_lens=one, block_tables=tables)
+        with pytest.raises(ValueError):
+            layer(x, x, x)
+        reset_context()
