@@ -830,16 +830,20 @@ ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int6
       p.dense_bytes = bytes;
       p.workspace_bytes += bytes;
     }
-    // One or two row tiles per unit (bf16 rows): a KV tile takes a unit of two 1.83 times as long
-    // (2 x 1,024 rows over 2,000, 32 heads: 107 us, one tile 117), but fewer, larger units fill the
-    // SMs less evenly (4 chunks of 300-512 rows, 28/4 heads: 131 us, one tile 113). The better
-    // estimate of rounds x time decides; half the sequences are taken to end inside a tile.
-    if ((format == kFmtBf16 || p.dense > 0) && p.mtiles >= 2 && p.splits == 1) {
+    // One or two row tiles per unit: a KV tile takes a unit of two 1.83 times as long (bf16, 2 x 1,024
+    // rows over 2,000, 32 heads: 107 us, one tile 117) or 1.5 times (quantised, where expanding it is
+    // what takes longest; 8 x 256 rows over 2,000: 122 us, one tile 164; 8 x 384: 253 and 232), but
+    // fewer, larger units fill the SMs less evenly (bf16, 4 chunks of 300-512 rows, 28/4 heads: 131 us,
+    // one tile 113). The better estimate of rounds x time decides; half the sequences are taken to end
+    // inside a tile, none to be longer than max_q.
+    if (p.mtiles >= 2 && p.splits == 1) {
       auto rounds = [&](int64_t unit_rows) {
-        const double n = Hkv * ((double)total_q * group / (double)unit_rows + 0.5 * B) / num_sms;
+        const double most = (double)((rows + unit_rows - 1) / unit_rows) * B;
+        const double n = Hkv * std::min(most, (double)total_q * group / (double)unit_rows + 0.5 * B) / num_sms;
         return n > 3 ? n + 0.5 : std::ceil(n);
       };
-      if (1.83 * rounds(2 * p.tile_rows) < rounds(p.tile_rows)) {
+      const double pair = format == kFmtBf16 || p.dense > 0 ? 1.83 : 1.5;
+      if (pair * rounds(2 * p.tile_rows) < rounds(p.tile_rows)) {
         p.unit_rows = 2 * p.tile_rows;
         p.mtiles = (int)((rows + p.unit_rows - 1) / p.unit_rows);
       }

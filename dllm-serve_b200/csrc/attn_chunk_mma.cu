@@ -14,9 +14,10 @@
 // One row tile ("single"): each KV tile's 128 columns are split between two
 // softmax warpgroups, each with its own running maximum, sum and accumulator,
 // merged once per unit (exact: softmax of a union). Two row tiles ("pair",
-// bf16 rows, where such units fill the SMs evenly enough): a warpgroup per row
-// tile, and every key tile read from L2 serves both: the single form needs 64
-// KB per 2,290 cycles and SM, close to what L2 delivers.
+// where such units fill the SMs evenly enough): a warpgroup per row tile, and
+// every key tile that is read, and expanded, serves both: the single form
+// needs 64 KB per 2,290 cycles and SM, close to what L2 delivers, and expands a
+// quantised tile in about as long.
 //
 // Quantised caches: 8-bit rows are brought into shared memory as they are
 // (TMA boxes, or four rows at a time where the slots are scattered) and two more
@@ -33,7 +34,7 @@
 //   warp 11         loader of Q
 //   warps 12-15     quantised: fill the K ring (expand cached tiles, load fresh ones)
 //   warps 16-19     quantised: fill the V ring
-// One warpgroup for both rings was the bottleneck: 1,560 cycles to expand a
+// (Single, e4m3:) one warpgroup for both rings was the bottleneck: 1,560 cycles to expand a
 // tile of K or V, 4,270 per KV tile against 2,290 of the bf16 kernel.
 // TMEM (512 columns): S buffers [0,128) [128,256), accumulators at 256 and 384;
 // P (bf16) over the first columns of S (pair) or of each half of it (single).
@@ -62,7 +63,6 @@ constexpr int kTileN = 128;
 constexpr int kHalfN = 64;
 constexpr uint32_t kTileBytes = 128 * kD * 2;  // bf16 tile
 constexpr uint32_t kChunkBytes = 128 * 128;    // its 64-column half; also an 8-bit tile
-constexpr int kRaw = 2;                        // stages of each raw ring
 
 template <int kFmt, bool kPair>
 struct Layout {
@@ -73,6 +73,7 @@ struct Layout {
   static constexpr int kRegsSoftmax = kQuant ? 144 : 208;
   static constexpr int kRegsOther = kQuant ? 64 : 88;
   static constexpr int kTilesQ = kPair ? 2 : 1;
+  static constexpr int kRaw = kPair ? 1 : 2;  // stages of each raw ring (the second Q tile takes one's place)
   static constexpr int kStagesK = kQuant ? 2 : 3;
   static constexpr int kStagesV = kQuant || kPair ? 2 : 3;
   // arrivals that complete a bf16 stage: the four expanding warps, or the loader's
@@ -223,13 +224,14 @@ DLLM_DEVICE void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t ide
       : "memory");
 }
 
-// P = 2^(S*scale_log2 - m) for one row of a 64-column half tile, packed to
-// bf16 pairs and stored to TMEM at tP; returns the row sum of P (fp32).
-DLLM_DEVICE float exp_store_half(const uint32_t (&s)[2][32], float sl2, float m, uint32_t tP) {
+// P = 2^(S*scale_log2 - m) for 32 kChunks columns of one row, packed to bf16
+// pairs and stored to TMEM at tP; returns the row sum of P (fp32).
+template <int kChunks>
+DLLM_DEVICE float exp_store(const uint32_t (&s)[kChunks][32], float sl2, float m, uint32_t tP) {
   const float neg_m = -m;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
+  for (int c = 0; c < kChunks; ++c) {
     uint32_t pk[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
@@ -240,26 +242,6 @@ DLLM_DEVICE float exp_store_half(const uint32_t (&s)[2][32], float sl2, float m,
       pk[e] = pack_bf16x2(p0, p1);
     }
     tmem_st16(tP + c * 16, pk);
-  }
-  return (acc[0] + acc[1]) + (acc[2] + acc[3]);
-}
-
-// The same for a whole tile's 128 columns, over the S buffer's first 64.
-DLLM_DEVICE float exp_store_tile(const uint32_t (&s)[4][32], float sl2, float m, uint32_t tS) {
-  const float neg_m = -m;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    uint32_t pk[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float p0 = ex2_approx(fmaf(__uint_as_float(s[c][2 * e]), sl2, neg_m));
-      const float p1 = ex2_approx(fmaf(__uint_as_float(s[c][2 * e + 1]), sl2, neg_m));
-      acc[(2 * e) & 3] += p0;
-      acc[(2 * e + 1) & 3] += p1;
-      pk[e] = pack_bf16x2(p0, p1);
-    }
-    tmem_st16(tS + c * 16, pk);
   }
   return (acc[0] + acc[1]) + (acc[2] + acc[3]);
 }
@@ -293,27 +275,41 @@ DLLM_DEVICE void softmax_pair(const ChunkArgs& a, uint32_t tmem, uint32_t bar0, 
       if (!mbar_wait_warp(bar(S::BAR_SFULL + wg), s_it & 1, abort_flag)) return;
       ++s_it;
       tc_fence_after();
-      uint32_t s[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, s[c]);
-      tmem_wait_ld();
       const int nv = min(kt.valid, seen - kt.pos);  // this row's visible columns
-      if (__any_sync(0xffffffffu, nv < kTileN)) {
+      // bf16 caches: the row's 128 scores at once. Quantised ones leave registers for 64: the upper
+      // half is read for its maximum, and again once the lower half's P is written.
+      constexpr int kChunks = S::kQuant ? 2 : 4;
+      uint32_t s[kChunks][32];
+      auto load = [&](int col) {  // from column `col` on, hidden ones as -inf
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < kChunks; ++c) tmem_ld32(tS + col + c * 32, s[c]);
+        tmem_wait_ld();
+        if (__any_sync(0xffffffffu, nv < col + kChunks * 32)) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (c * 32 + e >= nv) s[c][e] = __float_as_uint(-INFINITY);
+          for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (col + c * 32 + e >= nv) s[c][e] = __float_as_uint(-INFINITY);
+        }
+      };
+      auto largest = [&]() -> float {
+        float mq[kChunks];
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          float x = __uint_as_float(s[c][0]);
+#pragma unroll
+          for (int e = 1; e < 31; e += 2) x = max3f(x, __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+          mq[c] = fmaxf(x, __uint_as_float(s[c][31]));
+        }
+        return kChunks == 4 ? max3f(mq[0], mq[1], fmaxf(mq[kChunks - 2], mq[kChunks - 1])) : fmaxf(mq[0], mq[1]);
+      };
+      float mxs = -INFINITY;
+      if (S::kQuant && kt.valid > kHalfN) {
+        load(kHalfN);
+        mxs = largest();
       }
-      float mq[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float x = __uint_as_float(s[c][0]);
-#pragma unroll
-        for (int e = 1; e < 31; e += 2) x = max3f(x, __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
-        mq[c] = fmaxf(x, __uint_as_float(s[c][31]));
-      }
-      const float mxs = max3f(mq[0], mq[1], fmaxf(mq[2], mq[3])) * sl2;
+      load(0);
+      mxs = fmaxf(mxs, largest()) * sl2;
       // Lazy rescaling: a stale maximum stays while the new one exceeds it by at most 8 (log2
       // units), so P stays <= 256; a row's first visible key sets it (its accumulator holds zeros).
       const bool first = m == -INFINITY;
@@ -328,7 +324,12 @@ DLLM_DEVICE void softmax_pair(const ChunkArgs& a, uint32_t tmem, uint32_t bar0, 
         m = mn;
         l *= alpha;
       }
-      l += exp_store_tile(s, sl2, m == -INFINITY ? 0.f : m, tS);  // hidden columns give exact zeros
+      const float base = m == -INFINITY ? 0.f : m;
+      l += exp_store<kChunks>(s, sl2, base, tS);  // hidden columns give exact zeros
+      if (S::kQuant && kt.valid > kHalfN) {
+        load(kHalfN);
+        l += exp_store<kChunks>(s, sl2, base, tS + kHalfN / 2);
+      }
       if (rescale) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -393,12 +394,12 @@ DLLM_DEVICE void softmax_pair(const ChunkArgs& a, uint32_t tmem, uint32_t bar0, 
 template <int kFmt, bool kPair>
 __global__ void __launch_bounds__(Layout<kFmt, kPair>::kThreads, 1)
     attn_chunk_mma_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                          const __grid_constant__ CUtensorMap tmV,                          const __grid_constant__ CUtensorMap tmKc, const __grid_constant__ CUtensorMap tmVc,
+                          const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmKc, const __grid_constant__ CUtensorMap tmVc,
                           const __grid_constant__ CUtensorMap tmKg, const __grid_constant__ CUtensorMap tmVg,
                           const __grid_constant__ ChunkArgs a) {
   using S = Layout<kFmt, kPair>;
   constexpr bool kQuant = S::kQuant;
-  constexpr int kStagesK = S::kStagesK, kStagesV = S::kStagesV;
+  constexpr int kStagesK = S::kStagesK, kStagesV = S::kStagesV, kRaw = S::kRaw;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_base = smem_u32(smem_raw);
   const uint32_t base = (raw_base + 1023u) & ~1023u;
@@ -1011,7 +1012,7 @@ __global__ void __launch_bounds__(Layout<kFmt, kPair>::kThreads, 1)
               tmem_st32(tOwn + c * 32, o);
             }
           }
-          l += exp_store_half(s, sl2, m == -INFINITY ? 0.f : m, tS);  // hidden columns give exact zeros
+          l += exp_store<2>(s, sl2, m == -INFINITY ? 0.f : m, tS);  // hidden columns give exact zeros
           tmem_wait_st();
         }
         tc_fence_before();
@@ -1130,8 +1131,12 @@ cudaError_t launch_attn_chunk_mma(const ChunkMaps& maps, const ChunkArgs& a, int
     case kFmtBf16:
       return pair ? chunk128::launch<kFmtBf16, true>(maps, a, num_sms, stream)
                   : chunk128::launch<kFmtBf16, false>(maps, a, num_sms, stream);
-    case kFmtE4m3: return chunk128::launch<kFmtE4m3, false>(maps, a, num_sms, stream);
-    default: return chunk128::launch<kFmtInt8, false>(maps, a, num_sms, stream);
+    case kFmtE4m3:
+      return pair ? chunk128::launch<kFmtE4m3, true>(maps, a, num_sms, stream)
+                  : chunk128::launch<kFmtE4m3, false>(maps, a, num_sms, stream);
+    default:
+      return pair ? chunk128::launch<kFmtInt8, true>(maps, a, num_sms, stream)
+                  : chunk128::launch<kFmtInt8, false>(maps, a, num_sms, stream);
   }
 }
 
