@@ -278,7 +278,7 @@ DLLM_DEVICE void softmax_pair(const ChunkArgs& a, uint32_t tmem, uint32_t bar0, 
       const int nv = min(kt.valid, seen - kt.pos);  // this row's visible columns
       // bf16 caches: the row's 128 scores at once. Quantised ones leave registers for 64: the upper
       // half is read for its maximum, and again once the lower half's P is written.
-      constexpr int kChunks = S::kQuant ? 2 : 4;
+      constexpr int kHalves = S::kQuant ? 2 : 1, kChunks = 4 / kHalves;
       uint32_t s[kChunks][32];
       auto load = [&](int col) {  // from column `col` on, hidden ones as -inf
 #pragma unroll
@@ -304,12 +304,13 @@ DLLM_DEVICE void softmax_pair(const ChunkArgs& a, uint32_t tmem, uint32_t bar0, 
         return kChunks == 4 ? max3f(mq[0], mq[1], fmaxf(mq[kChunks - 2], mq[kChunks - 1])) : fmaxf(mq[0], mq[1]);
       };
       float mxs = -INFINITY;
-      if (S::kQuant && kt.valid > kHalfN) {
-        load(kHalfN);
-        mxs = largest();
+      const int last = kHalves > 1 && kt.valid > kHalfN ? 1 : 0;
+#pragma unroll 1
+      for (int h = last; h >= 0; --h) {
+        load(h * kHalfN);
+        mxs = fmaxf(mxs, largest());
       }
-      load(0);
-      mxs = fmaxf(mxs, largest()) * sl2;
+      mxs *= sl2;
       // Lazy rescaling: a stale maximum stays while the new one exceeds it by at most 8 (log2
       // units), so P stays <= 256; a row's first visible key sets it (its accumulator holds zeros).
       const bool first = m == -INFINITY;
@@ -325,13 +326,13 @@ DLLM_DEVICE void softmax_pair(const ChunkArgs& a, uint32_t tmem, uint32_t bar0, 
         l *= alpha;
       }
       const float base = m == -INFINITY ? 0.f : m;
-      l += exp_store<kChunks>(s, sl2, base, tS);  // hidden columns give exact zeros
-      if (S::kQuant && kt.valid > kHalfN) {
-        load(kHalfN);
-        l += exp_store<kChunks>(s, sl2, base, tS + kHalfN / 2);
+#pragma unroll 1
+      for (int h = 0; h <= last; ++h) {
+        if (h > 0) load(h * kHalfN);
+        l += exp_store<kChunks>(s, sl2, base, tS + h * (kHalfN / 2));  // hidden columns give exact zeros
       }
       if (rescale) {
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t o[32];
           tmem_ld32(tO + c * 32, o);
@@ -365,7 +366,7 @@ DLLM_DEVICE void softmax_pair(const ChunkArgs& a, uint32_t tmem, uint32_t bar0, 
             __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(orow), (lane & ~3) + r));
         live[r] = __shfl_sync(0xffffffffu, row_ok ? 1 : 0, (lane & ~3) + r) != 0;
       }
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t o[32];
         tmem_ld32(tO + c * 32, o);
@@ -837,13 +838,6 @@ __global__ void __launch_bounds__(Layout<kFmt, kPair>::kThreads, 1)
       // upper units: eight lanes then read eight different units and write eight different banks.
       const int un = tid & 7;
       const int r0 = (tid >> 3) ^ (un >> 2);
-      uint32_t e[8];
-      bool big = false;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        e[i] = ex[i * 16 + r0];
-        big |= exp_is_big<kFmt>(e[i]);
-      }
       const int x = (2 * un) & 7;
       uint8_t* d0 = dst + (un >> 2) * kChunkBytes + r0 * 128 + ((x ^ (r0 & 7)) << 4);
       uint8_t* d1 = dst + (un >> 2) * kChunkBytes + r0 * 128 + (((x + 1) ^ (r0 & 7)) << 4);
@@ -852,25 +846,31 @@ __global__ void __launch_bounds__(Layout<kFmt, kPair>::kThreads, 1)
         *reinterpret_cast<uint4*>(d1 + i * 2048) = make_uint4(w[4], w[5], w[6], w[7]);
       };
       src += r0 * kD + un * 16;
-      if (!__any_sync(0xffffffffu, big)) {
+#pragma unroll 1
+      for (int i0 = 0; i0 < 8; i0 += 4) {  // (unrolled, the loop costs every role instruction fetches)
+        uint4 c[4];
+        uint32_t e[4];
+        bool big = false;
 #pragma unroll
-        for (int i0 = 0; i0 < 8; i0 += 4) {
-          uint4 c[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) c[i] = *reinterpret_cast<const uint4*>(src + (i0 + i) * 16 * kD);
+        for (int i = 0; i < 4; ++i) {
+          c[i] = *reinterpret_cast<const uint4*>(src + (i0 + i) * 16 * kD);
+          e[i] = ex[(i0 + i) * 16 + r0];
+          big |= exp_is_big<kFmt>(e[i]);
+        }
+        if (!__any_sync(0xffffffffu, big)) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint32_t w[8];
-            expand16<kFmt>(c[i], code_scale<kFmt>(e[i0 + i]), w);
+            expand16<kFmt>(c[i], code_scale<kFmt>(e[i]), w);
             put(i0 + i, w);
           }
-        }
-      } else {
+        } else {
 #pragma unroll 1
-        for (int i = 0; i < 8; ++i) {
-          uint32_t w[8];
-          dequantise16<kFmt>(*reinterpret_cast<const uint4*>(src + i * 16 * kD), ex[i * 16 + r0], w);
-          put(i, w);
+          for (int i = i0; i < i0 + 4; ++i) {
+            uint32_t w[8];
+            dequantise16<kFmt>(*reinterpret_cast<const uint4*>(src + i * 16 * kD), ex[i * 16 + r0], w);
+            put(i, w);
+          }
         }
       }
       fence_proxy_async_smem();  // generic-proxy writes -> tensor-core reads
@@ -1002,7 +1002,7 @@ __global__ void __launch_bounds__(Layout<kFmt, kPair>::kThreads, 1)
             ok = mbar_wait_warp(bar(S::BAR_OREADY), (g - 1) & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < 4; ++c) {
               uint32_t o[32];
               tmem_ld32(tOwn + c * 32, o);
@@ -1057,7 +1057,7 @@ __global__ void __launch_bounds__(Layout<kFmt, kPair>::kThreads, 1)
           if (!alone && row_ok) a.part_ml[prow] = make_float2(mm, sum);
         }
         ++o_it;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 2; ++c) {
           if (idle) break;
           uint32_t oa[32], ob[32];
