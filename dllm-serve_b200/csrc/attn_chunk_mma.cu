@@ -847,26 +847,26 @@ __global__ void __launch_bounds__(Layout<kFmt, kPair>::kThreads, 1)
       };
       src += r0 * kD + un * 16;
 #pragma unroll 1
-      for (int i0 = 0; i0 < 8; i0 += 4) {  // (unrolled, the loop costs every role instruction fetches)
-        uint4 c[4];
-        uint32_t e[4];
+      for (int i0 = 0; i0 < 8; i0 += 2) {  // (unrolled, the loop costs every role instruction fetches)
+        uint4 c[2];
+        uint32_t e[2];
         bool big = false;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
           c[i] = *reinterpret_cast<const uint4*>(src + (i0 + i) * 16 * kD);
           e[i] = ex[(i0 + i) * 16 + r0];
           big |= exp_is_big<kFmt>(e[i]);
         }
         if (!__any_sync(0xffffffffu, big)) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < 2; ++i) {
             uint32_t w[8];
             expand16<kFmt>(c[i], code_scale<kFmt>(e[i]), w);
             put(i0 + i, w);
           }
         } else {
 #pragma unroll 1
-          for (int i = i0; i < i0 + 4; ++i) {
+          for (int i = i0; i < i0 + 2; ++i) {
             uint32_t w[8];
             dequantise16<kFmt>(*reinterpret_cast<const uint4*>(src + i * 16 * kD), ex[i * 16 + r0], w);
             put(i, w);
