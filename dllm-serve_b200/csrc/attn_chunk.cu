@@ -26,7 +26,7 @@
 // its four warps take the split's key chunks in turn, each with a private
 // ring of stages filled by cp.async, so the main loop has no CTA barrier. The
 // warps' partial results are merged in shared memory in a fixed order; splits
-// are merged by a second kernel, also in a fixed order. Products are
+// are merged by their cluster, or by a second kernel, also in a fixed order. Products are
 // mma.sync m16n8k16: at up to 16 rows per KV head (32 with a quantised cache) a
 // launch reads 512 (256) bytes per key for at most 16 x 512 (32 x 512)
 // operations, below what this instruction sustains, and its operands go
@@ -66,6 +66,7 @@ constexpr uint32_t kStageBytes = 8192;  // K half then V half
 constexpr int kFreshKeys = 16;          // keys of a bf16 chunk
 constexpr uint32_t kScaleBytes = 34 * 8;  // of a stage: 32 (K, V) scales, the largest exponent
 constexpr int kNoExp = -(1 << 30);        // no value exponent met
+constexpr int kClusterSplits = 8;         // splits that merge within a cluster
 // A scaled Q (below 2^15) times codes (at most 448) over 128 dimensions is below 2^31; with keys'
 // 2^e (e <= 121) lowered by this the scores stay finite, whatever the cache holds.
 constexpr float kKeyDown = 0x1p-24f;
@@ -89,7 +90,8 @@ struct Cfg {
   static constexpr uint32_t kSmemBytes = kOffQ + kN * 8 * kD * 2;
   static_assert(kCtas * (kSmemBytes + 1024) <= 233472, "the CTAs do not fit an SM");
   // the merge buffers (per warp: rows x 128 floats, then rows float2) reuse the stages
-  static_assert(kWarps * kN * 8 * (kD * 4 + 8) <= kWarps * kStages * kStageBytes, "merge buffers exceed the stages");
+  // (and one more float2 per row)
+  static_assert(kN * 8 * (kWarps * (kD * 4 + 8) + 8) <= kWarps * kStages * kStageBytes, "merge buffers exceed the stages");
 };
 
 DLLM_DEVICE void cp_async16(uint32_t dst, const void* src, bool live) {
@@ -121,6 +123,29 @@ DLLM_DEVICE void mma16816_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t 
       "{%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Every thread of the cluster's CTAs that have not ended.
+DLLM_DEVICE void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Shared memory of the cluster's CTA `rank`, at this CTA's address `a`.
+DLLM_DEVICE uint32_t cluster_addr(uint32_t a, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+  return r;
+}
+DLLM_DEVICE float2 cluster_ld2(uint32_t a, int rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(cluster_addr(a, rank)));
+  return v;
+}
+DLLM_DEVICE float4 cluster_ld4(uint32_t a, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(cluster_addr(a, rank)));
+  return v;
 }
 
 // Four codes -> two words of f16 pairs, unscaled (exact).
@@ -659,12 +684,50 @@ __global__ void __launch_bounds__(kThreads, Cfg<kFmt, kN>::kCtas) attn_chunk_ker
       x.x = pack_bf16x2(acc.x * inv, acc.y * inv);
       x.y = pack_bf16x2(acc.z * inv, acc.w * inv);
       *reinterpret_cast<uint2*>(a.o + (sq.q_begin + r) * a.o_stride + (int64_t)h * kD + d) = x;
+    } else if (a.cluster) {  // over warp 0's partial, which only this thread reads
+      *reinterpret_cast<float4*>(mo + (size_t)row * kD + d) = acc;
+      if (d == 0) ml[kWarps * kRows + row] = make_float2(mm, sum);
     } else {
       const int64_t at = ((int64_t)item * a.splits + split) * kRows + row;
       *reinterpret_cast<float4*>(a.part_o + at * kD + d) = acc;
       if (d == 0) a.part_ml[at] = make_float2(mm, sum);
     }
   }
+  if (alone || !a.cluster) return;
+  // ----------------------------- merge of the cluster's splits, in split order
+  const int n = (sp.total + a.split_chunks - 1) / a.split_chunks;  // splits with keys (the others have left)
+  cluster_barrier();
+  for (int i = split * kThreads + threadIdx.x; i < min(rows, kRows) * (kD / 4); i += n * kThreads) {
+    const int row = i / (kD / 4), d = (i % (kD / 4)) * 4;
+    const uint32_t from = base + (row * kD + d) * 4, from_ml = base + kWarps * kRows * (kD * 4 + 8) + row * 8;
+    float2 x[kClusterSplits];
+    float mm = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < kClusterSplits; ++s) {
+      x[s] = make_float2(-INFINITY, 0.f);
+      if (s < n) x[s] = cluster_ld2(from_ml, s);
+      mm = fmaxf(mm, x[s].x);
+    }
+    const float least = mm == -INFINITY ? 0.f : mm;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+#pragma unroll
+    for (int s = 0; s < kClusterSplits; ++s) {
+      if (s >= n) break;
+      const float f = ex2_approx(x[s].x - least);
+      const float4 y = cluster_ld4(from, s);
+      sum = fmaf(x[s].y, f, sum);
+      acc.x = fmaf(y.x, f, acc.x), acc.y = fmaf(y.y, f, acc.y);
+      acc.z = fmaf(y.z, f, acc.z), acc.w = fmaf(y.w, f, acc.w);
+    }
+    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    const int r = (row0 + row) / a.group, h = hkv * a.group + (row0 + row) - r * a.group;
+    uint2 out;
+    out.x = pack_bf16x2(acc.x * inv, acc.y * inv);
+    out.y = pack_bf16x2(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>(a.o + (sq.q_begin + r) * a.o_stride + (int64_t)h * kD + d) = out;
+  }
+  cluster_barrier();  // no CTA leaves while another reads its shared memory
 }
 
 // Merges the splits of each row in split order; one warp per packed row, each
@@ -783,9 +846,9 @@ cudaError_t launch(const ChunkArgs& a, cudaStream_t stream) {
   }
   const int64_t items = (int64_t)a.B * a.Hkv * a.mtiles;
   if (items * a.splits > 0x7fffffffLL) return cudaErrorInvalidValue;
-  e = launch_pdl(attn_chunk_kernel<kFmt, kN>, dim3((unsigned)(items * a.splits)), dim3(kThreads),
-                 Cfg<kFmt, kN>::kSmemBytes, stream, a);
-  if (e != cudaSuccess || a.splits == 1) return e;
+  e = launch_pdl_cluster(attn_chunk_kernel<kFmt, kN>, dim3((unsigned)(items * a.splits)), dim3(kThreads),
+                         Cfg<kFmt, kN>::kSmemBytes, stream, a.cluster ? a.splits : 1, a);
+  if (e != cudaSuccess || a.splits == 1 || a.cluster) return e;
   return launch_pdl(attn_chunk_merge_kernel<chunk_keys<kFmt>(), kFreshKeys, 8 * kN>,
                     dim3((unsigned)(items * kN)), dim3(256), 0, stream, a);
 }
@@ -859,15 +922,20 @@ ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int6
   // of c chunks a warp takes c + 3; the launch takes whole waves of CTAs if all
   // contexts are as long as the bound, and if they are 60 % of it on average
   // its mean load and the last CTA's tail: the sum of both estimates decides.
-  // The merge costs four chunks and one for 16 splits.
+  // A second kernel that merges costs eight chunks and one for 8 splits. Up to 8 splits of a launch that
+  // fits the SMs at once are clusters that merge their own (32 contexts of 128-1,024 bf16 rows, 28/4
+  // heads, two splits: 15.1 us with the second kernel, 13.5 as clusters; 16 x 2 rows over 8,192 e4m3
+  // rows, 32/4 heads: 53 and 44). In larger launches a cluster waits for as many free places (8 contexts
+  // of 16,384 e4m3 rows, 32 heads, five splits: 170 us and 200).
   const int64_t slots = (int64_t)(format == kFmtBf16 || p.rows > 16 ? 2 : 3) * num_sms;  // Cfg::kCtas
+  auto in_cluster = [&](int64_t s) { return s > 1 && s <= chunk::kClusterSplits && items * s <= slots; };
   int64_t splits = 1;
   double best = 0;
   for (int64_t s = 1; items > 0 && s <= std::max<int64_t>(1, chunks / chunk::kWarps) && s <= 1024; s += std::max<int64_t>(1, s / 8)) {
     const int64_t per = (chunks + s - 1) / s;
     const double cta = (double)((per + chunk::kWarps - 1) / chunk::kWarps) + 3;
     const double waves = (double)(items * s) / (double)slots;
-    const double cost = cta * (double)((items * s + slots - 1) / slots) + cta * (0.6 * waves + 1) + (s > 1 ? 8 + (double)s / 8 : 0);
+    const double cost = cta * (double)((items * s + slots - 1) / slots) + cta * (0.6 * waves + 1) + (in_cluster(s) ? 4 : s > 1 ? 8 + (double)s / 8 : 0);
     if (s == 1 || cost < best) {
       best = cost;
       splits = s;
@@ -875,7 +943,8 @@ ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int6
   }
   p.split_chunks = (int)std::max<int64_t>(1, (chunks + splits - 1) / splits);
   p.splits = (int)std::max<int64_t>(1, (chunks + p.split_chunks - 1) / p.split_chunks);
-  p.workspace_bytes = p.splits > 1 ? items * p.splits * p.rows * (chunk::kD * 4 + 8) : 0;
+  p.cluster = in_cluster(p.splits);
+  p.workspace_bytes = p.splits > 1 && !p.cluster ? items * p.splits * p.rows * (chunk::kD * 4 + 8) : 0;
   return p;
 }
 
@@ -894,6 +963,7 @@ cudaError_t launch_attn_chunk(ChunkArgs a, int format, const ChunkPlan& plan, co
   a.mtiles = plan.mtiles;
   a.splits = plan.splits;
   a.split_chunks = plan.split_chunks;
+  a.cluster = plan.cluster;
   const int64_t rows = (int64_t)a.B * a.Hkv * a.mtiles * a.splits * plan.rows;
   a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.dense_bytes);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * chunk::kD);

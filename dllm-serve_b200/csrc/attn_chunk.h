@@ -57,6 +57,7 @@ struct ChunkArgs {
   int mtiles;              // work units per (sequence, KV head)
   int splits;              // key splits per row tile
   int split_chunks;        // key chunks of a split
+  bool cluster;            // the splits of a row tile are a cluster, which merges them (kernel for few rows)
   int total_units;         // items * splits
   float* part_o;           // [items * splits, rows, 128] partial outputs (splits > 1)
   float2* part_ml;         // [items * splits, rows] (maximum, sum)
@@ -71,6 +72,7 @@ struct ChunkPlan {
   int mtiles;
   int splits;
   int split_chunks;
+  bool cluster;            // the splits merge within a cluster (no workspace)
   int dense;               // rows per sequence of the expanded copy of a quantised cache's rows, 0: none
   int64_t dense_bytes;     // its bytes (K, then V), at the workspace's start
   int64_t workspace_bytes;

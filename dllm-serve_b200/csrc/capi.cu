@@ -516,7 +516,7 @@ int dllm_attn_chunk_launches(int format, int batch, int num_heads, int num_kv_he
   if (batch == 0 || max_seqlen_q == 0) return 0;
   const dllm::ChunkPlan p = dllm::plan_attn_chunk(format, batch, num_kv_heads, num_heads / num_kv_heads, max_seqlen_q, 0,
                                                   max_context, max_fresh, num_sms_of_current_device());
-  return 1 + (p.dense > 0) + (p.splits > 1);
+  return 1 + (p.dense > 0) + (p.splits > 1 && !p.cluster);
 }
 
 int dllm_attn_chunk_fwd(const dllm_chunk_args* args) {
