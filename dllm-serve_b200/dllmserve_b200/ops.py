@@ -185,16 +185,15 @@ def load_kvcache_quant(key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping)
     _kv_quant(False, key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping)
 
 
-def _same_device(*ts: torch.Tensor) -> int:
-    """Index of the CUDA device that holds every tensor (one integer query per
-    tensor: the quick form of ``_require_cuda``)."""
-    idx = ts[0].get_device()
-    for t in ts:
-        i = t.get_device()
-        if i != idx or i < 0:
-            _require_cuda(*ts)
-            raise ValueError("all tensors must be on one CUDA device")
-    return idx
+def _one_device(*ts: torch.Tensor):
+    """Raises for tensors that are not all on one CUDA device."""
+    _require_cuda(*ts)
+    raise ValueError("all tensors must be on one CUDA device")
+
+
+def _stream_of(idx: int) -> int:
+    """``_stream_ptr`` of the current device, whose index is known."""
+    return _raw_stream(idx) if _raw_stream is not None else _stream_ptr()
 
 
 def _status_ptr_of(idx: int) -> int:
@@ -209,9 +208,13 @@ def _check_quant_cache(name, cache, exp, heads, head_dim) -> int:
     if len(sh) < 3 or sh[-2] != heads or sh[-1] != head_dim or not cache.is_contiguous():
         raise ValueError(f"{name}_cache must be contiguous [blocks, block_size, {heads}, {head_dim}]")
     slots = cache.numel() // (heads * head_dim)
+    _check_exponents(name, exp, slots, heads)
+    return slots
+
+
+def _check_exponents(name, exp, slots, heads) -> None:
     if exp.dtype is not torch.uint8 or not exp.is_contiguous() or exp.numel() != slots * heads or exp.shape[-1] != heads:
         raise ValueError(f"{name}_exp must be contiguous uint8 [blocks, block_size, {heads}]")
-    return slots
 
 
 def _kv_quant(store, key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping):
@@ -225,7 +228,10 @@ def _kv_quant(store, key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping):
     if ks[2] != 1 or vs[2] != 1 or ((ks[1] != D or vs[1] != D) and H != 1):
         raise ValueError("key and value must have contiguous heads")
     k_str, v_str = (ks[0], vs[0]) if N > 1 else (H * D, H * D)  # (one row: any stride will do)
-    dev = _same_device(key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping)
+    dev = key.get_device()
+    if (dev < 0 or value.get_device() != dev or k_cache.get_device() != dev or v_cache.get_device() != dev
+            or k_exp.get_device() != dev or v_exp.get_device() != dev or slot_mapping.get_device() != dev):
+        _one_device(key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping)
     fmt = _KV_FORMATS.get(k_cache.dtype, _native.KV_BF16)
     if fmt == _native.KV_BF16 or v_cache.dtype is not k_cache.dtype:
         raise ValueError("k_cache and v_cache must both be float8_e4m3fn or both int8")
@@ -242,11 +248,11 @@ def _kv_quant(store, key, value, k_cache, v_cache, k_exp, v_exp, slot_mapping):
         with torch.cuda.device(dev):
             rc = fn(key.data_ptr(), k_str, value.data_ptr(), v_str, k_cache.data_ptr(), v_cache.data_ptr(),
                     k_exp.data_ptr(), v_exp.data_ptr(), slot_mapping.data_ptr(), N, H, D, fmt, slots,
-                    _status_ptr_of(dev), _stream_ptr())
+                    _status_ptr_of(dev), _stream_of(dev))
     else:
         rc = fn(key.data_ptr(), k_str, value.data_ptr(), v_str, k_cache.data_ptr(), v_cache.data_ptr(),
                 k_exp.data_ptr(), v_exp.data_ptr(), slot_mapping.data_ptr(), N, H, D, fmt, slots,
-                _status_ptr_of(dev), _stream_ptr())
+                _status_ptr_of(dev), _stream_of(dev))
     if rc:
         _native.check(rc, "store_kvcache_quant" if store else "load_kvcache_quant")
     LAUNCHES[0] += 1
@@ -654,13 +660,16 @@ def chunk_attention(
         raise ValueError("no keys: give block_tables, slots or fresh k and v")
     if cached and (k_cache is None or v_cache is None):
         raise ValueError("block_tables / slots need k_cache and v_cache")
+    dev = q.get_device()
+    if dev < 0:
+        _one_device(q)
     max_q = int(max_seqlen_q)
     if cu_seqlens_q is None:
         if max_q != 1:
             raise ValueError("without cu_seqlens_q every sequence has one row: max_seqlen_q must be 1")
-        dev, B, cu_q_ptr = _same_device(q), q.shape[0], 0
+        B, cu_q_ptr = q.shape[0], 0
     else:
-        dev, B, cu_q_ptr = _same_device(q, cu_seqlens_q), cu_seqlens_q.numel() - 1, cu_seqlens_q.data_ptr()
+        B, cu_q_ptr = cu_seqlens_q.numel() - 1, cu_seqlens_q.data_ptr()
         _check_cu("cu_seqlens_q", cu_seqlens_q, B, dev)
     fmt = _native.KV_BF16
     k_ptr = v_ptr = cu_k_ptr = kx_ptr = vx_ptr = kc_ptr = vc_ptr = k_str = v_str = total_k = num_slots = max_fresh = 0
@@ -697,8 +706,8 @@ def chunk_attention(
         if fmt != _native.KV_BF16:
             if k_exp is None or v_exp is None:
                 raise ValueError("a quantised cache needs k_exp and v_exp")
-            _check_quant_cache("k", k_cache, k_exp, Hkv, D)
-            _check_quant_cache("v", v_cache, v_exp, Hkv, D)
+            _check_exponents("k", k_exp, num_slots, Hkv)
+            _check_exponents("v", v_exp, num_slots, Hkv)
             if k_exp.get_device() != dev or v_exp.get_device() != dev:
                 raise ValueError("all tensors must be on the same device")
             kx_ptr, vx_ptr = k_exp.data_ptr(), v_exp.data_ptr()
@@ -780,7 +789,7 @@ def _chunk_launch(dev, sizes, out, pointers, max_blocks, block_size, D, causal, 
     # allocated per call on the current stream, so overlapping launches never share it
     ws = torch.empty(need, dtype=torch.uint8, device=out.device) if need > 0 else None
     rc = lib.dllm_attn_chunk_fwd(_native.CHUNK_ARGS.pack(
-        *pointers, 0 if ws is None else ws.data_ptr(), need, _status_ptr_of(dev), _stream_ptr(), fmt, max_blocks,
+        *pointers, 0 if ws is None else ws.data_ptr(), need, _status_ptr_of(dev), _stream_of(dev), fmt, max_blocks,
         block_size, max_context, B, max_q, max_fresh, Hq, Hkv, D, 1 if causal else 0,
         D ** -0.5 if softmax_scale is None else softmax_scale))
     if rc:
