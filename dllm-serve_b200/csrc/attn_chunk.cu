@@ -26,12 +26,21 @@
 // its four warps take the split's key chunks in turn, each with a private
 // ring of stages filled by cp.async, so the main loop has no CTA barrier. The
 // warps' partial results are merged in shared memory in a fixed order; splits
-// are merged by their cluster, or by a second kernel, also in a fixed order. Products are
+// are merged by their cluster, or by a second kernel, also in a fixed order.
+// Products are
 // mma.sync m16n8k16: at up to 16 rows per KV head (32 with a quantised cache) a
 // launch reads 512 (256) bytes per key for at most 16 x 512 (32 x 512)
 // operations, below what this instruction sustains, and its operands go
 // straight from shared memory to registers, where codes are expanded; the
 // tcgen05 kernel writes them to shared memory first.
+//
+// Measured, decode (one row, 32 heads): 8 contexts of 4,096-32,768 rows bf16 350
+// us, 6.6 TB/s, e4m3 199 us, 5.9 TB/s (of 16,384 rows each 170 us, 6.4 TB/s):
+// the cache's bytes, where lengths are even. 32 contexts of 128-1,024 bf16 rows,
+// 28/4 heads: 13.5 us, 2.8 TB/s: a launch, one split's chunks and the merge one
+// after another. 8 x 32 rows over 1,144 e4m3 rows: 42.5 us: with eight warps an SM
+// the latencies of conversions and products, one launch not filling the last
+// seventh of the SMs' places.
 //
 // Operand layout: keys (scores) and dimensions (outputs) take the products' 16
 // rows and the packed query rows their 8 columns, so eight rows leave nothing
@@ -865,11 +874,12 @@ cudaError_t launch_rows(const ChunkArgs& a, int rows, cudaStream_t stream) {
 
 ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int64_t total_q, int max_context,
                           int max_fresh, int num_sms) {
-  constexpr int kDenseTiles = 4;
+  constexpr int kDenseTiles = 8;
   ChunkPlan p = {};
   const int64_t rows = (int64_t)max_q * group;
-  // Which kernel (8 sequences of 32 heads, 32 rows over 1,144 cached ones): e4m3 41 us in attn_chunk.cu, 45 in
-  // the 128-row kernel, which expands every key for 96 idle rows; bf16 47 and 34; 64 rows, e4m3: 79 and 55.
+  // Which kernel (8 sequences of 32 heads over 1,144 rows in slot lists): 32 rows, e4m3, 42.5 us in
+  // attn_chunk.cu, 36 rows 52.6 in the 128-row kernel (from block tables 41.4 and 41.1); 64 rows, e4m3,
+  // 79 and 52.7; 32 rows, bf16, 47 in attn_chunk.cu, 34 in the 128-row kernel (block tables).
   p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 && format != kFmtBf16 ? 32 : kChunkMmaRows;
   if (p.rows == kChunkMmaRows) {
     // One CTA per SM. Splits only while SMs would have nothing to do, and four
@@ -882,9 +892,10 @@ ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int6
     p.split_chunks = (int)std::max<int64_t>(1, (tiles + splits - 1) / splits);
     p.splits = (int)std::max<int64_t>(1, (tiles + p.split_chunks - 1) / p.split_chunks);
     p.workspace_bytes = p.splits > 1 ? units * p.splits * p.rows * (chunk::kD * 4 + 8) : 0;
-    // Every row tile of a (sequence, KV head) expands the quantised rows it reads. From four row
-    // tiles on they are expanded once instead, into bf16 rows that all tiles read, unless that
-    // copy would be larger than 1 GiB.
+    // Every work unit expands the quantised rows it reads. From eight row tiles on they are expanded
+    // once instead, into bf16 rows that all units read, unless that copy would be larger than 1 GiB
+    // (e4m3, 32 heads, 8 sequences over 2,000 rows, in the units, two tiles each, and once: 4 tiles 230
+    // and 256 us, 6 tiles 337 and 344, 8 tiles 452 and 435, 16 tiles 1,004 and 896).
     const int64_t cap = ((int64_t)max_context + 127) / 128 * 128;
     const int64_t bytes = 2 * (int64_t)B * cap * Hkv * chunk::kD * 2;
     if (format != kFmtBf16 && p.mtiles >= kDenseTiles && bytes > 0 && bytes <= ((int64_t)1 << 30) &&
@@ -894,18 +905,19 @@ ChunkPlan plan_attn_chunk(int format, int B, int Hkv, int group, int max_q, int6
       p.workspace_bytes += bytes;
     }
     // One or two row tiles per unit: a KV tile takes a unit of two 1.83 times as long (bf16, 2 x 1,024
-    // rows over 2,000, 32 heads: 107 us, one tile 117) or 1.5 times (quantised, where expanding it is
-    // what takes longest; 8 x 256 rows over 2,000: 122 us, one tile 164; 8 x 384: 253 and 232), but
-    // fewer, larger units fill the SMs less evenly (bf16, 4 chunks of 300-512 rows, 28/4 heads: 131 us,
-    // one tile 113). The better estimate of rounds x time decides; half the sequences are taken to end
-    // inside a tile, none to be longer than max_q.
+    // rows over 2,000, 32 heads: 107 us, one tile 117) or 1.45 to 1.8 times (quantised, where one
+    // expansion serves both; the less, the more units have one tile only: 32 x 48 rows, 28/4 heads,
+    // int8: 41 us, one tile 47; 8 x 256 rows over 2,000 e4m3 rows, 32 heads: 109 and 135; 8 x 384: 212
+    // and 194), but fewer, larger units fill the SMs less evenly (bf16, 4 chunks of 300-512 rows, 28/4
+    // heads: 131 us, one tile 113). The better estimate of rounds x time decides; half the sequences are
+    // taken to end inside a tile, none to be longer than max_q.
     if (p.mtiles >= 2 && p.splits == 1) {
       auto rounds = [&](int64_t unit_rows) {
         const double most = (double)((rows + unit_rows - 1) / unit_rows) * B;
         const double n = Hkv * std::min(most, (double)total_q * group / (double)unit_rows + 0.5 * B) / num_sms;
         return n > 3 ? n + 0.5 : std::ceil(n);
       };
-      const double pair = format == kFmtBf16 || p.dense > 0 ? 1.83 : 1.5;
+      const double pair = format == kFmtBf16 || p.dense > 0 ? 1.83 : 1.45;
       if (pair * rounds(2 * p.tile_rows) < rounds(p.tile_rows)) {
         p.unit_rows = 2 * p.tile_rows;
         p.mtiles = (int)((rows + p.unit_rows - 1) / p.unit_rows);

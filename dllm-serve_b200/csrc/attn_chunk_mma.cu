@@ -1,6 +1,6 @@
 // Attention of a chunk of new tokens over a paged KV cache, for launches with
-// more than 16 query rows per KV head (diffusion blocks, prefill chunks):
-// tcgen05 + TMEM + TMA, sm_100a.
+// more query rows per KV head than attn_chunk.cu takes (diffusion blocks,
+// prefill chunks): tcgen05 + TMEM + TMA, sm_100a.
 //
 // A work unit is (sequence b, KV head, one or two tiles of packed rows, split
 // of the keys); packed row p of a (sequence, KV head) is row p / group of the
@@ -8,8 +8,9 @@
 // key tile they read. A row tile holds as many whole chunk rows as fit 128
 // packed rows (all 128 where the group divides them). Keys come in tiles of
 // 128: the sequence's cached rows, then its fresh rows, cut at the last key
-// that a row of the unit sees. Probabilities are rounded to bf16 (2^-8 of
-// their value).
+// that a row of the unit sees. Softmax is online (a running maximum and sum per
+// row, the accumulator rescaled when the maximum has grown by 2^8).
+// Probabilities are rounded to bf16 (2^-8 of their value, up to 256).
 //
 // One row tile ("single"): each KV tile's 128 columns are split between two
 // softmax warpgroups, each with its own running maximum, sum and accumulator,
@@ -26,6 +27,15 @@
 // nothing, and the rest of the kernel is the same for every format. HBM and
 // L2 carry one byte per element.
 //
+// Measured: 4 chunks of 300-512 rows over 2,000-4,600 bf16 rows, 28/4 heads: 116
+// us, 785 TFLOP/s; 4 prefill chunks of 1,024-2,048 rows over 1,024-6,144, 32
+// heads: 544 us, 882 TFLOP/s (bf16), 609 us (e4m3, expanded once by a kernel of
+// its own). Between a tile's first product and its second stands one
+// warpgroup's softmax, about 1,500 cycles in which that row tile's products
+// wait; the tensor pipe is busy half of the time, the exponentials' half. 32
+// blocks of 32 rows over 176-496 int8 rows, 28/4 heads: 21 us, where a unit's
+// first loads and its epilogue are as long as its four tiles.
+//
 // Roles (12 warps, 20 with a quantised cache):
 //   warps 0-3, 4-7  softmax warpgroups
 //   warp 8          loader of K: bf16 stages, or the raw K ring of a quantised cache
@@ -34,8 +44,10 @@
 //   warp 11         loader of Q
 //   warps 12-15     quantised: fill the K ring (expand cached tiles, load fresh ones)
 //   warps 16-19     quantised: fill the V ring
-// (Single, e4m3:) one warpgroup for both rings was the bottleneck: 1,560 cycles to expand a
-// tile of K or V, 4,270 per KV tile against 2,290 of the bf16 kernel.
+// (Single, e4m3:) one warpgroup for both rings was the bottleneck: 1,560 cycles
+// to expand a tile of K or V, 4,270 per KV tile against 2,290 of the bf16
+// kernel. With this many roles instruction fetches count: loops that are not
+// unrolled took 126 us to 114 (8 x 128 rows over 4,000 e4m3 rows, 32 heads).
 // TMEM (512 columns): S buffers [0,128) [128,256), accumulators at 256 and 384;
 // P (bf16) over the first columns of S (pair) or of each half of it (single).
 // MMA order per KV tile j: single PV(j) of both halves, then QK(j+2); pair, for
@@ -458,329 +470,329 @@ __global__ void __launch_bounds__(Layout<kFmt, kPair>::kThreads, 1)
   if (warp >= 8 && warp < 12) {
     set_max_registers<S::kRegsOther, false>();
     if (warp == 8 || warp == 10) {
-    // ---------------------------------------------------------------- loaders
-    const bool is_k = warp == 8;
-    const uint64_t pol = policy_evict_last();
-    const int nst = is_k ? kStagesK : kStagesV;
-    const int bfull = is_k ? S::BAR_KFULL : S::BAR_VFULL;
-    const int bempty = is_k ? S::BAR_KEMPTY : S::BAR_VEMPTY;
-    const uint32_t ring = base + (is_k ? S::kOffK : S::kOffV);
-    const int rfull = S::BAR_RFULL + (is_k ? 0 : kRaw), rempty = S::BAR_REMPTY + (is_k ? 0 : kRaw);
-    const uint32_t raw_ring = base + S::kOffRaw + (is_k ? 0 : kRaw * kChunkBytes);
-    const uint32_t exp_ring = base + S::kOffExp + (is_k ? 0 : kRaw * 128);
-    const uint8_t* exps = is_k ? a.k_exp : a.v_exp;
-    const CUtensorMap* mfresh = is_k ? &tmK : &tmV;
-    const CUtensorMap* mcache = is_k ? &tmKc : &tmVc;
-    const CUtensorMap* mgather = is_k ? &tmKg : &tmVg;
-    uint32_t done = 0;                           // tiles passed in the bf16 ring
-    uint32_t raw_done = 0;                       // tiles issued into the raw ring
-    uint32_t land = 0;                           // partial V tiles landed
-    bool ok = true;
-    for (int u = blockIdx.x; u < total_units && ok; u += gridDim.x) {
-      const Unit t = decode_unit(u, a, is_k && lane == 0);
-      if (!t.valid) continue;
-      const int32_t* table = a.tables != nullptr ? a.tables + (int64_t)t.b * a.table_stride : nullptr;
-      for (int j = 0; j < t.nkv && ok; ++j, ++done) {
-        const KvTile kt = kv_tile(t, j);
-        if (kQuant && kt.fresh) break;  // the expanding warps load fresh tiles, which come last
-        const int st = done % nst;
-        // cached tiles: this lane's four rows 4 * lane + i, and whether the tile is one run of slots
-        int sl[4], s0 = 0;
-        bool contig = true;
-        if (!kt.fresh) {
-          if (!kQuant && a.dense > 0) {
-            s0 = t.b * a.dense + kt.pos;
+      // ---------------------------------------------------------------- loaders
+      const bool is_k = warp == 8;
+      const uint64_t pol = policy_evict_last();
+      const int nst = is_k ? kStagesK : kStagesV;
+      const int bfull = is_k ? S::BAR_KFULL : S::BAR_VFULL;
+      const int bempty = is_k ? S::BAR_KEMPTY : S::BAR_VEMPTY;
+      const uint32_t ring = base + (is_k ? S::kOffK : S::kOffV);
+      const int rfull = S::BAR_RFULL + (is_k ? 0 : kRaw), rempty = S::BAR_REMPTY + (is_k ? 0 : kRaw);
+      const uint32_t raw_ring = base + S::kOffRaw + (is_k ? 0 : kRaw * kChunkBytes);
+      const uint32_t exp_ring = base + S::kOffExp + (is_k ? 0 : kRaw * 128);
+      const uint8_t* exps = is_k ? a.k_exp : a.v_exp;
+      const CUtensorMap* mfresh = is_k ? &tmK : &tmV;
+      const CUtensorMap* mcache = is_k ? &tmKc : &tmVc;
+      const CUtensorMap* mgather = is_k ? &tmKg : &tmVg;
+      uint32_t done = 0;                           // tiles passed in the bf16 ring
+      uint32_t raw_done = 0;                       // tiles issued into the raw ring
+      uint32_t land = 0;                           // partial V tiles landed
+      bool ok = true;
+      for (int u = blockIdx.x; u < total_units && ok; u += gridDim.x) {
+        const Unit t = decode_unit(u, a, is_k && lane == 0);
+        if (!t.valid) continue;
+        const int32_t* table = a.tables != nullptr ? a.tables + (int64_t)t.b * a.table_stride : nullptr;
+        for (int j = 0; j < t.nkv && ok; ++j, ++done) {
+          const KvTile kt = kv_tile(t, j);
+          if (kQuant && kt.fresh) break;  // the expanding warps load fresh tiles, which come last
+          const int st = done % nst;
+          // cached tiles: this lane's four rows 4 * lane + i, and whether the tile is one run of slots
+          int sl[4], s0 = 0;
+          bool contig = true;
+          if (!kt.fresh) {
+            if (!kQuant && a.dense > 0) {
+              s0 = t.b * a.dense + kt.pos;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sl[i] = s0 + 4 * lane + i;
-          } else if (table != nullptr && a.block_size % kTileN == 0) {
-            // the tile lies inside one block
-            const int blk = kt.pos / a.block_size;
-            const int e = blk < a.max_blocks ? table[blk] : -1;
-            const int64_t at = e < 0 ? -1 : (int64_t)e * a.block_size + kt.pos % a.block_size;
-            const bool in = at >= 0 && at < a.num_slots;
-            s0 = in ? (int)at : (int)a.num_slots;  // past the cache: the copy brings zeros
+              for (int i = 0; i < 4; ++i) sl[i] = s0 + 4 * lane + i;
+            } else if (table != nullptr && a.block_size % kTileN == 0) {
+              // the tile lies inside one block
+              const int blk = kt.pos / a.block_size;
+              const int e = blk < a.max_blocks ? table[blk] : -1;
+              const int64_t at = e < 0 ? -1 : (int64_t)e * a.block_size + kt.pos % a.block_size;
+              const bool in = at >= 0 && at < a.num_slots;
+              s0 = in ? (int)at : (int)a.num_slots;  // past the cache: the copy brings zeros
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sl[i] = in ? s0 + 4 * lane + i : -1;
-          } else {
+              for (int i = 0; i < 4; ++i) sl[i] = in ? s0 + 4 * lane + i : -1;
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int r = 4 * lane + i, pos = kt.pos + r;
-              sl[i] = -1;
-              if (r < kt.valid) {
-                if (table != nullptr) {
-                  const int blk = pos / a.block_size;
-                  const int e = blk < a.max_blocks ? table[blk] : -1;
-                  const int64_t at = e < 0 ? -1 : (int64_t)e * a.block_size + pos % a.block_size;
-                  sl[i] = at < a.num_slots ? (int)at : -1;
-                } else {
-                  sl[i] = a.slots[t.sq.s_begin + pos];
+              for (int i = 0; i < 4; ++i) {
+                const int r = 4 * lane + i, pos = kt.pos + r;
+                sl[i] = -1;
+                if (r < kt.valid) {
+                  if (table != nullptr) {
+                    const int blk = pos / a.block_size;
+                    const int e = blk < a.max_blocks ? table[blk] : -1;
+                    const int64_t at = e < 0 ? -1 : (int64_t)e * a.block_size + pos % a.block_size;
+                    sl[i] = at < a.num_slots ? (int)at : -1;
+                  } else {
+                    sl[i] = a.slots[t.sq.s_begin + pos];
+                  }
                 }
               }
+              s0 = __shfl_sync(0xffffffffu, sl[0], 0);
+              contig = s0 >= 0 && (int64_t)s0 + kt.valid <= a.num_slots;
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (4 * lane + i < kt.valid && sl[i] != s0 + 4 * lane + i) contig = false;
+              contig = __all_sync(0xffffffffu, contig);
             }
-            s0 = __shfl_sync(0xffffffffu, sl[0], 0);
-            contig = s0 >= 0 && (int64_t)s0 + kt.valid <= a.num_slots;
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const bool live = 4 * lane + i < kt.valid;
+              if (live && (sl[i] < 0 || sl[i] >= a.num_slots)) bad = true;
+              if (!live || sl[i] >= a.num_slots) sl[i] = -1;  // -1: reads as a zero row
+            }
+            if (bad) set_error(a.err, kDevSlotOutOfRange);
+          }
+          if constexpr (kQuant) {
+            // ---- raw ring
+            const int rs = raw_done % kRaw;
+            if (raw_done >= (uint32_t)kRaw)
+              ok = mbar_wait_warp(bar(rempty + rs), (raw_done / kRaw - 1) & 1, abort_flag);
+            if (!ok) break;
+            const uint32_t dst = raw_ring + rs * kChunkBytes, fb = bar(rfull + rs);
+            if (contig) {
+              if (lane == 0) {
+                mbar_arrive_expect_tx(fb, kChunkBytes);
+                tma_load_3d(dst, mcache, fb, 0, t.hkv, s0, pol);
+              }
+            } else {
+              if (lane == 0) mbar_arrive_expect_tx(fb, kChunkBytes);
+              __syncwarp();
+              int r[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) r[i] = sl[i] >= 0 ? sl[i] : (int)a.num_slots;
+              tma_gather4(dst + 4 * lane * kD, mgather, fb, t.hkv * kD, r);
+            }
+            uint32_t e4 = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (4 * lane + i < kt.valid && sl[i] != s0 + 4 * lane + i) contig = false;
-            contig = __all_sync(0xffffffffu, contig);
-          }
-          bool bad = false;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool live = 4 * lane + i < kt.valid;
-            if (live && (sl[i] < 0 || sl[i] >= a.num_slots)) bad = true;
-            if (!live || sl[i] >= a.num_slots) sl[i] = -1;  // -1: reads as a zero row
-          }
-          if (bad) set_error(a.err, kDevSlotOutOfRange);
-        }
-        if constexpr (kQuant) {
-          // ---- raw ring
-          const int rs = raw_done % kRaw;
-          if (raw_done >= (uint32_t)kRaw)
-            ok = mbar_wait_warp(bar(rempty + rs), (raw_done / kRaw - 1) & 1, abort_flag);
-          if (!ok) break;
-          const uint32_t dst = raw_ring + rs * kChunkBytes, fb = bar(rfull + rs);
-          if (contig) {
-            if (lane == 0) {
-              mbar_arrive_expect_tx(fb, kChunkBytes);
-              tma_load_3d(dst, mcache, fb, 0, t.hkv, s0, pol);
-            }
-          } else {
-            if (lane == 0) mbar_arrive_expect_tx(fb, kChunkBytes);
+              if (sl[i] >= 0) e4 |= (uint32_t)exps[(int64_t)sl[i] * a.Hkv + t.hkv] << (8 * i);
+            *reinterpret_cast<uint32_t*>(smem + (exp_ring - base) + rs * 128 + 4 * lane) = e4;
             __syncwarp();
-            int r[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) r[i] = sl[i] >= 0 ? sl[i] : (int)a.num_slots;
-            tma_gather4(dst + 4 * lane * kD, mgather, fb, t.hkv * kD, r);
-          }
-          uint32_t e4 = 0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (sl[i] >= 0) e4 |= (uint32_t)exps[(int64_t)sl[i] * a.Hkv + t.hkv] << (8 * i);
-          *reinterpret_cast<uint32_t*>(smem + (exp_ring - base) + rs * 128 + 4 * lane) = e4;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(fb);
-          ++raw_done;
-        } else {
-        // ---- a bf16 stage
-        if (done >= (uint32_t)nst) ok = mbar_wait_warp(bar(bempty + st), (done / nst - 1) & 1, abort_flag);
-        if (!ok) break;
-        const uint32_t dst = ring + st * kTileBytes;
-        uint8_t* tile = smem + (dst - base);
-        const bool clear = !is_k && (kt.valid & 15) != 0;
-        const uint32_t fb = bar(clear ? S::BAR_VLAND : bfull + st);
-        if (lane == 0) mbar_arrive_expect_tx(fb, kTileBytes);
-        __syncwarp();
-        if (kt.fresh || contig) {
-          if (lane == 0) {
-            const CUtensorMap* mp = kt.fresh ? mfresh : mcache;
-            const int row = kt.fresh ? (int)kt.row : s0;
-            tma_load_3d(dst, mp, fb, 0, t.hkv, row, pol);
-            tma_load_3d(dst + kChunkBytes, mp, fb, 64, t.hkv, row, pol);
-          }
-        } else {
-          int r[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) r[i] = sl[i] >= 0 ? sl[i] : (int)a.num_slots;
-          tma_gather4(dst + 4 * lane * 128, mgather, fb, t.hkv * kD, r);
-          tma_gather4(dst + kChunkBytes + 4 * lane * 128, mgather, fb, t.hkv * kD + 64, r);
-        }
-        if (clear) {
-          ok = mbar_wait_warp(fb, land & 1, abort_flag);
-          if (!ok) break;
-          ++land;
-          clear_tail(tile, kt.valid, lane);
-          if (lane == 0) mbar_arrive(bar(bfull + st));
-        }
-        }
-      }
-    }
-    if (lane == 0 && *abort_flag) {
-      // Drain: wait (bounded) for the loads that may still be in flight.
-      if (!kQuant)
-        for (uint32_t n = (done > (uint32_t)nst ? done - nst : 0); n < done; ++n)
-          mbar_wait_drain(bar(bfull + n % nst), (n / nst) & 1, 100000000ull);
-      if (kQuant)
-        for (uint32_t n = (raw_done > (uint32_t)kRaw ? raw_done - kRaw : 0); n < raw_done; ++n)
-          mbar_wait_drain(bar(rfull + n % kRaw), (n / kRaw) & 1, 100000000ull);
-      if (!kQuant && !is_k) mbar_wait_drain(bar(S::BAR_VLAND), land & 1, 100000000ull);
-    }
-    __syncwarp();
-  } else if (warp == 9) {
-    // -------------------------------------------------------------------- MMA
-    if (lane == 0) {
-      const uint32_t idesc_pv = make_idesc_bf16(128, 128, true);
-      const uint32_t idesc_qk_full = make_idesc_bf16(128, 128, false);
-      const uint32_t dq = desc_lo(base + S::kOffQ, 16);
-      const uint32_t dk0 = desc_lo(base + S::kOffK, 16);
-      const uint32_t dv0 = desc_lo(base + S::kOffV, kChunkBytes);
-      constexpr uint32_t kStageStep = kTileBytes >> 4;  // (all offsets stay inside the address field)
-      // S(sb) = Q K(kst)^T over n_rows keys
-      auto qk = [&](int kst, int n_rows, uint32_t sb) {
-        const uint32_t idesc =
-            n_rows == kTileN ? idesc_qk_full : make_idesc_bf16(128, (n_rows + 15) & ~15, false);
-        const uint32_t b = dk0 + kst * kStageStep;
-        const uint32_t d = tmem + sb * 128;
-#pragma unroll
-        for (int s = 0; s < kD / 16; ++s) {
-          const uint32_t off = ((s >> 2) * kChunkBytes + (s & 3) * 32) >> 4;
-          mma_ss(d, dq + off, b + off, idesc, s > 0 ? 1u : 0u);
-        }
-      };
-      // O_h (+)= P_h V[64h .. 64h + 16 ksteps)
-      auto pv_half = [&](int vst, uint32_t sb, int h, int ksteps, bool acc) {
-        const uint32_t b = dv0 + vst * kStageStep;
-        const uint32_t d = tmem + 256 + h * 128;
-        const uint32_t p = tmem + sb * 128 + h * kHalfN;
-        if (ksteps == 4) {
-#pragma unroll
-          for (int s = 0; s < 4; ++s)
-            mma_ts(d, p + s * 8, b + (4 * h + s) * (2048 >> 4), idesc_pv, (acc || s > 0) ? 1u : 0u);
-        } else {
-          for (int s = 0; s < ksteps; ++s)
-            mma_ts(d, p + s * 8, b + (4 * h + s) * (2048 >> 4), idesc_pv, (acc || s > 0) ? 1u : 0u);
-        }
-      };
-      // pair: row tile i against KV tiles: S(i) = Q(i) K^T, O(i) (+)= P(i) V
-      auto qk_tile = [&](int i, int kst, int n_rows) {
-        const uint32_t idesc = n_rows == kTileN ? idesc_qk_full : make_idesc_bf16(128, (n_rows + 15) & ~15, false);
-        const uint32_t x = dq + i * kStageStep, b = dk0 + kst * kStageStep;
-#pragma unroll
-        for (int s = 0; s < kD / 16; ++s) {
-          const uint32_t off = ((s >> 2) * kChunkBytes + (s & 3) * 32) >> 4;
-          mma_ss(tmem + i * 128, x + off, b + off, idesc, s > 0 ? 1u : 0u);
-        }
-      };
-      auto pv_tile = [&](int i, int vst, int ksteps, bool acc) {
-        const uint32_t b = dv0 + vst * kStageStep;
-        const uint32_t d = tmem + 256 + i * 128, p = tmem + i * 128;
-        if (ksteps == 8) {
-#pragma unroll
-          for (int s = 0; s < 8; ++s) mma_ts(d, p + s * 8, b + s * (2048 >> 4), idesc_pv, (acc || s > 0) ? 1u : 0u);
-        } else {
-          for (int s = 0; s < ksteps; ++s) mma_ts(d, p + s * 8, b + s * (2048 >> 4), idesc_pv, (acc || s > 0) ? 1u : 0u);
-        }
-      };
-      uint32_t q_it = 0, k_it = 0, v_it = 0;
-      uint32_t p_it[2] = {0, 0};
-      bool ok = true;
-      for (int u = blockIdx.x; kPair && u < total_units && ok; u += gridDim.x) {
-        const Unit t = decode_unit(u, a, false);
-        if (!t.valid || t.nkv == 0) continue;
-        const int nt = t.rows > a.tile_rows ? 2 : 1;
-        ok = mbar_wait(bar(S::BAR_QFULL), q_it & 1, abort_flag);
-        if (!ok) break;
-        ++q_it;
-        {
-          const int kst = k_it % kStagesK;
-          ok = mbar_wait(bar(S::BAR_KFULL + kst), (k_it / kStagesK) & 1, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          const int valid = kv_tile(t, 0).valid;
-          for (int i = 0; i < nt; ++i) {
-            qk_tile(i, kst, valid);
-            umma_commit(bar(S::BAR_SFULL + i));
-          }
-          umma_commit(bar(S::BAR_KEMPTY + kst));
-          ++k_it;
-          if (t.nkv == 1) umma_commit(bar(S::BAR_QEMPTY));
-        }
-        for (int j = 0; j < t.nkv && ok; ++j) {
-          const int ks = (kv_tile(t, j).valid + 15) >> 4;  // 1..8 K-steps
-          const int vst = v_it % kStagesV, kst = k_it % kStagesK;
-          ok = mbar_wait(bar(S::BAR_VFULL + vst), (v_it / kStagesV) & 1, abort_flag);
-          if (!ok) break;
-          const bool more = j + 1 < t.nkv;
-          const int next = more ? kv_tile(t, j + 1).valid : 0;
-          for (int i = 0; i < nt && ok; ++i) {
-            ok = mbar_wait(bar(S::BAR_PFULL + i), p_it[i] & 1, abort_flag);
+            if (lane == 0) mbar_arrive(fb);
+            ++raw_done;
+          } else {
+            // ---- a bf16 stage
+            if (done >= (uint32_t)nst) ok = mbar_wait_warp(bar(bempty + st), (done / nst - 1) & 1, abort_flag);
             if (!ok) break;
-            ++p_it[i];
-            tc_fence_after();
-            pv_tile(i, vst, ks, j > 0);
-            if (more) {
-              if (i == 0) {
-                ok = mbar_wait(bar(S::BAR_KFULL + kst), (k_it / kStagesK) & 1, abort_flag);
-                if (!ok) break;
-                tc_fence_after();
+            const uint32_t dst = ring + st * kTileBytes;
+            uint8_t* tile = smem + (dst - base);
+            const bool clear = !is_k && (kt.valid & 15) != 0;
+            const uint32_t fb = bar(clear ? S::BAR_VLAND : bfull + st);
+            if (lane == 0) mbar_arrive_expect_tx(fb, kTileBytes);
+            __syncwarp();
+            if (kt.fresh || contig) {
+              if (lane == 0) {
+                const CUtensorMap* mp = kt.fresh ? mfresh : mcache;
+                const int row = kt.fresh ? (int)kt.row : s0;
+                tma_load_3d(dst, mp, fb, 0, t.hkv, row, pol);
+                tma_load_3d(dst + kChunkBytes, mp, fb, 64, t.hkv, row, pol);
               }
-              qk_tile(i, kst, next);
-              umma_commit(bar(S::BAR_SFULL + i));
             } else {
-              umma_commit(bar(S::BAR_OFULL + i));
+              int r[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) r[i] = sl[i] >= 0 ? sl[i] : (int)a.num_slots;
+              tma_gather4(dst + 4 * lane * 128, mgather, fb, t.hkv * kD, r);
+              tma_gather4(dst + kChunkBytes + 4 * lane * 128, mgather, fb, t.hkv * kD + 64, r);
+            }
+            if (clear) {
+              ok = mbar_wait_warp(fb, land & 1, abort_flag);
+              if (!ok) break;
+              ++land;
+              clear_tail(tile, kt.valid, lane);
+              if (lane == 0) mbar_arrive(bar(bfull + st));
             }
           }
-          if (!ok) break;
-          umma_commit(bar(S::BAR_VEMPTY + vst));
-          ++v_it;
-          if (more) {
-            umma_commit(bar(S::BAR_KEMPTY + kst));
-            ++k_it;
-            if (j + 2 == t.nkv) umma_commit(bar(S::BAR_QEMPTY));  // last QK issued
-          }
         }
       }
-      uint32_t g = 0;  // KV tiles whose PVs were issued (all units), = S tile index
-      for (int u = blockIdx.x; !kPair && u < total_units && ok; u += gridDim.x) {
-        const Unit t = decode_unit(u, a, false);
-        if (!t.valid || t.nkv == 0) continue;
-        ok = mbar_wait(bar(S::BAR_QFULL), q_it & 1, abort_flag);
-        if (!ok) break;
-        ++q_it;
-        const int npro = t.nkv < 2 ? t.nkv : 2;
-        for (int j = 0; j < npro && ok; ++j) {
-          const KvTile kt = kv_tile(t, j);
-          const int kst = k_it % kStagesK;
-          ok = mbar_wait(bar(S::BAR_KFULL + kst), (k_it / kStagesK) & 1, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          qk(kst, kt.valid, (g + j) & 1);
-          umma_commit(bar(S::BAR_SFULL + ((g + j) & 1)));
-          umma_commit(bar(S::BAR_KEMPTY + kst));
-          ++k_it;
-        }
-        if (!ok) break;
-        if (t.nkv <= 2) umma_commit(bar(S::BAR_QEMPTY));  // every QK of the unit issued
-        bool b_started = false;  // O_b written in this unit
-        for (int j = 0; j < t.nkv && ok; ++j, ++g) {
-          const KvTile kt = kv_tile(t, j);
-          const uint32_t sb = g & 1;
-          const int vst = v_it % kStagesV;
-          ok = mbar_wait(bar(S::BAR_VFULL + vst), (v_it / kStagesV) & 1, abort_flag);
-          if (!ok) break;
-          ok = mbar_wait(bar(S::BAR_PFULL + sb), (g >> 1) & 1, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          const int ks = (kt.valid + 15) >> 4;  // 1..8 K-steps
-          pv_half(vst, sb, 0, ks < 4 ? ks : 4, j > 0);
-          if (ks > 4) {
-            pv_half(vst, sb, 1, ks - 4, b_started);
-            b_started = true;
+      if (lane == 0 && *abort_flag) {
+        // Drain: wait (bounded) for the loads that may still be in flight.
+        if (!kQuant)
+          for (uint32_t n = (done > (uint32_t)nst ? done - nst : 0); n < done; ++n)
+            mbar_wait_drain(bar(bfull + n % nst), (n / nst) & 1, 100000000ull);
+        if (kQuant)
+          for (uint32_t n = (raw_done > (uint32_t)kRaw ? raw_done - kRaw : 0); n < raw_done; ++n)
+            mbar_wait_drain(bar(rfull + n % kRaw), (n / kRaw) & 1, 100000000ull);
+        if (!kQuant && !is_k) mbar_wait_drain(bar(S::BAR_VLAND), land & 1, 100000000ull);
+      }
+      __syncwarp();
+    } else if (warp == 9) {
+      // -------------------------------------------------------------------- MMA
+      if (lane == 0) {
+        const uint32_t idesc_pv = make_idesc_bf16(128, 128, true);
+        const uint32_t idesc_qk_full = make_idesc_bf16(128, 128, false);
+        const uint32_t dq = desc_lo(base + S::kOffQ, 16);
+        const uint32_t dk0 = desc_lo(base + S::kOffK, 16);
+        const uint32_t dv0 = desc_lo(base + S::kOffV, kChunkBytes);
+        constexpr uint32_t kStageStep = kTileBytes >> 4;  // (all offsets stay inside the address field)
+        // S(sb) = Q K(kst)^T over n_rows keys
+        auto qk = [&](int kst, int n_rows, uint32_t sb) {
+          const uint32_t idesc =
+              n_rows == kTileN ? idesc_qk_full : make_idesc_bf16(128, (n_rows + 15) & ~15, false);
+          const uint32_t b = dk0 + kst * kStageStep;
+          const uint32_t d = tmem + sb * 128;
+#pragma unroll
+          for (int s = 0; s < kD / 16; ++s) {
+            const uint32_t off = ((s >> 2) * kChunkBytes + (s & 3) * 32) >> 4;
+            mma_ss(d, dq + off, b + off, idesc, s > 0 ? 1u : 0u);
           }
-          umma_commit(bar(S::BAR_VEMPTY + vst));
-          umma_commit(bar(S::BAR_OREADY));
-          ++v_it;
-          if (j + 2 < t.nkv) {
-            const KvTile kn = kv_tile(t, j + 2);
+        };
+        // O_h (+)= P_h V[64h .. 64h + 16 ksteps)
+        auto pv_half = [&](int vst, uint32_t sb, int h, int ksteps, bool acc) {
+          const uint32_t b = dv0 + vst * kStageStep;
+          const uint32_t d = tmem + 256 + h * 128;
+          const uint32_t p = tmem + sb * 128 + h * kHalfN;
+          if (ksteps == 4) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+              mma_ts(d, p + s * 8, b + (4 * h + s) * (2048 >> 4), idesc_pv, (acc || s > 0) ? 1u : 0u);
+          } else {
+            for (int s = 0; s < ksteps; ++s)
+              mma_ts(d, p + s * 8, b + (4 * h + s) * (2048 >> 4), idesc_pv, (acc || s > 0) ? 1u : 0u);
+          }
+        };
+        // pair: row tile i against KV tiles: S(i) = Q(i) K^T, O(i) (+)= P(i) V
+        auto qk_tile = [&](int i, int kst, int n_rows) {
+          const uint32_t idesc = n_rows == kTileN ? idesc_qk_full : make_idesc_bf16(128, (n_rows + 15) & ~15, false);
+          const uint32_t x = dq + i * kStageStep, b = dk0 + kst * kStageStep;
+#pragma unroll
+          for (int s = 0; s < kD / 16; ++s) {
+            const uint32_t off = ((s >> 2) * kChunkBytes + (s & 3) * 32) >> 4;
+            mma_ss(tmem + i * 128, x + off, b + off, idesc, s > 0 ? 1u : 0u);
+          }
+        };
+        auto pv_tile = [&](int i, int vst, int ksteps, bool acc) {
+          const uint32_t b = dv0 + vst * kStageStep;
+          const uint32_t d = tmem + 256 + i * 128, p = tmem + i * 128;
+          if (ksteps == 8) {
+#pragma unroll
+            for (int s = 0; s < 8; ++s) mma_ts(d, p + s * 8, b + s * (2048 >> 4), idesc_pv, (acc || s > 0) ? 1u : 0u);
+          } else {
+            for (int s = 0; s < ksteps; ++s) mma_ts(d, p + s * 8, b + s * (2048 >> 4), idesc_pv, (acc || s > 0) ? 1u : 0u);
+          }
+        };
+        uint32_t q_it = 0, k_it = 0, v_it = 0;
+        uint32_t p_it[2] = {0, 0};
+        bool ok = true;
+        for (int u = blockIdx.x; kPair && u < total_units && ok; u += gridDim.x) {
+          const Unit t = decode_unit(u, a, false);
+          if (!t.valid || t.nkv == 0) continue;
+          const int nt = t.rows > a.tile_rows ? 2 : 1;
+          ok = mbar_wait(bar(S::BAR_QFULL), q_it & 1, abort_flag);
+          if (!ok) break;
+          ++q_it;
+          {
             const int kst = k_it % kStagesK;
             ok = mbar_wait(bar(S::BAR_KFULL + kst), (k_it / kStagesK) & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
-            qk(kst, kn.valid, sb);  // tile g + 2 uses the same S buffer
-            umma_commit(bar(S::BAR_SFULL + sb));
+            const int valid = kv_tile(t, 0).valid;
+            for (int i = 0; i < nt; ++i) {
+              qk_tile(i, kst, valid);
+              umma_commit(bar(S::BAR_SFULL + i));
+            }
             umma_commit(bar(S::BAR_KEMPTY + kst));
             ++k_it;
-            if (j + 3 == t.nkv) umma_commit(bar(S::BAR_QEMPTY));  // last QK issued
+            if (t.nkv == 1) umma_commit(bar(S::BAR_QEMPTY));
+          }
+          for (int j = 0; j < t.nkv && ok; ++j) {
+            const int ks = (kv_tile(t, j).valid + 15) >> 4;  // 1..8 K-steps
+            const int vst = v_it % kStagesV, kst = k_it % kStagesK;
+            ok = mbar_wait(bar(S::BAR_VFULL + vst), (v_it / kStagesV) & 1, abort_flag);
+            if (!ok) break;
+            const bool more = j + 1 < t.nkv;
+            const int next = more ? kv_tile(t, j + 1).valid : 0;
+            for (int i = 0; i < nt && ok; ++i) {
+              ok = mbar_wait(bar(S::BAR_PFULL + i), p_it[i] & 1, abort_flag);
+              if (!ok) break;
+              ++p_it[i];
+              tc_fence_after();
+              pv_tile(i, vst, ks, j > 0);
+              if (more) {
+                if (i == 0) {
+                  ok = mbar_wait(bar(S::BAR_KFULL + kst), (k_it / kStagesK) & 1, abort_flag);
+                  if (!ok) break;
+                  tc_fence_after();
+                }
+                qk_tile(i, kst, next);
+                umma_commit(bar(S::BAR_SFULL + i));
+              } else {
+                umma_commit(bar(S::BAR_OFULL + i));
+              }
+            }
+            if (!ok) break;
+            umma_commit(bar(S::BAR_VEMPTY + vst));
+            ++v_it;
+            if (more) {
+              umma_commit(bar(S::BAR_KEMPTY + kst));
+              ++k_it;
+              if (j + 2 == t.nkv) umma_commit(bar(S::BAR_QEMPTY));  // last QK issued
+            }
           }
         }
-        if (!ok) break;
-        umma_commit(bar(S::BAR_OFULL));
+        uint32_t g = 0;  // KV tiles whose PVs were issued (all units), = S tile index
+        for (int u = blockIdx.x; !kPair && u < total_units && ok; u += gridDim.x) {
+          const Unit t = decode_unit(u, a, false);
+          if (!t.valid || t.nkv == 0) continue;
+          ok = mbar_wait(bar(S::BAR_QFULL), q_it & 1, abort_flag);
+          if (!ok) break;
+          ++q_it;
+          const int npro = t.nkv < 2 ? t.nkv : 2;
+          for (int j = 0; j < npro && ok; ++j) {
+            const KvTile kt = kv_tile(t, j);
+            const int kst = k_it % kStagesK;
+            ok = mbar_wait(bar(S::BAR_KFULL + kst), (k_it / kStagesK) & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            qk(kst, kt.valid, (g + j) & 1);
+            umma_commit(bar(S::BAR_SFULL + ((g + j) & 1)));
+            umma_commit(bar(S::BAR_KEMPTY + kst));
+            ++k_it;
+          }
+          if (!ok) break;
+          if (t.nkv <= 2) umma_commit(bar(S::BAR_QEMPTY));  // every QK of the unit issued
+          bool b_started = false;  // O_b written in this unit
+          for (int j = 0; j < t.nkv && ok; ++j, ++g) {
+            const KvTile kt = kv_tile(t, j);
+            const uint32_t sb = g & 1;
+            const int vst = v_it % kStagesV;
+            ok = mbar_wait(bar(S::BAR_VFULL + vst), (v_it / kStagesV) & 1, abort_flag);
+            if (!ok) break;
+            ok = mbar_wait(bar(S::BAR_PFULL + sb), (g >> 1) & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            const int ks = (kt.valid + 15) >> 4;  // 1..8 K-steps
+            pv_half(vst, sb, 0, ks < 4 ? ks : 4, j > 0);
+            if (ks > 4) {
+              pv_half(vst, sb, 1, ks - 4, b_started);
+              b_started = true;
+            }
+            umma_commit(bar(S::BAR_VEMPTY + vst));
+            umma_commit(bar(S::BAR_OREADY));
+            ++v_it;
+            if (j + 2 < t.nkv) {
+              const KvTile kn = kv_tile(t, j + 2);
+              const int kst = k_it % kStagesK;
+              ok = mbar_wait(bar(S::BAR_KFULL + kst), (k_it / kStagesK) & 1, abort_flag);
+              if (!ok) break;
+              tc_fence_after();
+              qk(kst, kn.valid, sb);  // tile g + 2 uses the same S buffer
+              umma_commit(bar(S::BAR_SFULL + sb));
+              umma_commit(bar(S::BAR_KEMPTY + kst));
+              ++k_it;
+              if (j + 3 == t.nkv) umma_commit(bar(S::BAR_QEMPTY));  // last QK issued
+            }
+          }
+          if (!ok) break;
+          umma_commit(bar(S::BAR_OFULL));
+        }
+        // Make sure every issued MMA has finished before TMEM is released.
+        umma_commit(bar(S::BAR_DRAIN));
+        mbar_wait_drain(bar(S::BAR_DRAIN), 0, 100000000ull);
       }
-      // Make sure every issued MMA has finished before TMEM is released.
-      umma_commit(bar(S::BAR_DRAIN));
-      mbar_wait_drain(bar(S::BAR_DRAIN), 0, 100000000ull);
-    }
-    __syncwarp();
+      __syncwarp();
     } else {
       // ------------------------------------------------------------- loader of Q
       // The box brings all heads of the KV head's group for a tile's chunk rows: packed order.
@@ -933,166 +945,166 @@ __global__ void __launch_bounds__(Layout<kFmt, kPair>::kThreads, 1)
     if constexpr (kPair) {
       softmax_pair<S>(a, tmem, bar0, abort_flag);
     } else {
-    const int wg = warp >> 2;           // 0: keys 0-63 of a tile, 1: keys 64-127
-    const int wq = warp & 3;
-    const int row_in_tile = threadIdx.x & 127;
-    const uint32_t lane_base = (uint32_t)(wq * 32) << 16;
-    const uint32_t tOwn = tmem + lane_base + 256 + wg * 128;  // this warpgroup's accumulator
-    const uint32_t tOa = tmem + lane_base + 256;
-    const uint32_t tOb = tmem + lane_base + 384;
-    float2* xch = reinterpret_cast<float2*>(smem + S::kOffXch);
-    const float sl2 = a.scale_log2;
-    uint32_t g = 0, o_it = 0;
-    bool ok = true;
-    for (int u = blockIdx.x; u < total_units && ok; u += gridDim.x) {
-      const Unit t = decode_unit(u, a, false);
-      if (!t.valid) continue;
-      const int qr = (t.row0 + row_in_tile) / a.group;  // row of the chunk
-      const int seen = (int)(a.causal ? min(t.L, max((int64_t)0, t.L - t.sq.Lq + qr + 1)) : t.L);
-      // A warp whose 32 rows lie past the unit's last one only keeps the barriers going (its rows
-      // of P hold anything: rows of a product do not mix).
-      const bool idle = wq * 32 >= t.rows;
-      const bool row_ok = row_in_tile < t.rows;
-      float m = -INFINITY;  // running max (log2 units), -inf until a visible key
-      float l = 0.f;
-      for (int j = 0; j < t.nkv; ++j, ++g) {
-        const KvTile kt = kv_tile(t, j);
-        const uint32_t sb = g & 1;
-        ok = mbar_wait_warp(bar(S::BAR_SFULL + sb), (g >> 1) & 1, abort_flag);
+      const int wg = warp >> 2;           // 0: keys 0-63 of a tile, 1: keys 64-127
+      const int wq = warp & 3;
+      const int row_in_tile = threadIdx.x & 127;
+      const uint32_t lane_base = (uint32_t)(wq * 32) << 16;
+      const uint32_t tOwn = tmem + lane_base + 256 + wg * 128;  // this warpgroup's accumulator
+      const uint32_t tOa = tmem + lane_base + 256;
+      const uint32_t tOb = tmem + lane_base + 384;
+      float2* xch = reinterpret_cast<float2*>(smem + S::kOffXch);
+      const float sl2 = a.scale_log2;
+      uint32_t g = 0, o_it = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; u < total_units && ok; u += gridDim.x) {
+        const Unit t = decode_unit(u, a, false);
+        if (!t.valid) continue;
+        const int qr = (t.row0 + row_in_tile) / a.group;  // row of the chunk
+        const int seen = (int)(a.causal ? min(t.L, max((int64_t)0, t.L - t.sq.Lq + qr + 1)) : t.L);
+        // A warp whose 32 rows lie past the unit's last one only keeps the barriers going (its rows
+        // of P hold anything: rows of a product do not mix).
+        const bool idle = wq * 32 >= t.rows;
+        const bool row_ok = row_in_tile < t.rows;
+        float m = -INFINITY;  // running max (log2 units), -inf until a visible key
+        float l = 0.f;
+        for (int j = 0; j < t.nkv; ++j, ++g) {
+          const KvTile kt = kv_tile(t, j);
+          const uint32_t sb = g & 1;
+          ok = mbar_wait_warp(bar(S::BAR_SFULL + sb), (g >> 1) & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t tS = tmem + lane_base + sb * 128 + wg * kHalfN;
+          if (!idle && kt.valid > wg * kHalfN) {
+            uint32_t s[2][32];
+            tmem_ld32(tS, s[0]);
+            tmem_ld32(tS + 32, s[1]);
+            tmem_wait_ld();
+            const int nv = min(kt.valid, seen - kt.pos) - wg * kHalfN;  // this row's visible columns
+            if (__any_sync(0xffffffffu, nv < kHalfN)) {
+#pragma unroll
+              for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  if (c * 32 + e >= nv) s[c][e] = __float_as_uint(-INFINITY);
+            }
+            float mq[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float x = __uint_as_float(s[c][0]);
+#pragma unroll
+              for (int e = 1; e < 31; e += 2)
+                x = max3f(x, __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+              mq[c] = fmaxf(x, __uint_as_float(s[c][31]));
+            }
+            const float mxs = fmaxf(mq[0], mq[1]) * sl2;
+            // Lazy rescaling: a stale maximum stays while the new one exceeds it
+            // by at most 8 (log2 units), so P stays <= 256. A row's first visible
+            // key sets it (its accumulator holds zeros or is not written yet).
+            const bool first = m == -INFINITY;
+            const bool need = row_ok && !first && mxs > m + 8.f;  // (rows past the tile's last are another sequence's)
+            if (first) m = mxs;
+            if (__any_sync(0xffffffffu, need)) {
+              const float mn = first ? m : fmaxf(m, mxs);
+              const float alpha = first ? 1.f : ex2_approx(m - mn);
+              m = mn;
+              l *= alpha;
+              // The accumulator must hold every PV up to tile g-1: PV(g-2)
+              // completed before S(g) did, so one more completion of OREADY
+              // (parity of tile g-1) is all there is to wait for.
+              ok = mbar_wait_warp(bar(S::BAR_OREADY), (g - 1) & 1, abort_flag);
+              if (!ok) break;
+              tc_fence_after();
+#pragma unroll 1
+              for (int c = 0; c < 4; ++c) {
+                uint32_t o[32];
+                tmem_ld32(tOwn + c * 32, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                tmem_st32(tOwn + c * 32, o);
+              }
+            }
+            l += exp_store<2>(s, sl2, m == -INFINITY ? 0.f : m, tS);  // hidden columns give exact zeros
+            tmem_wait_st();
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(S::BAR_PFULL + sb));
+        }
         if (!ok) break;
-        tc_fence_after();
-        const uint32_t tS = tmem + lane_base + sb * 128 + wg * kHalfN;
-        if (!idle && kt.valid > wg * kHalfN) {
-          uint32_t s[2][32];
-          tmem_ld32(tS, s[0]);
-          tmem_ld32(tS + 32, s[1]);
-          tmem_wait_ld();
-          const int nv = min(kt.valid, seen - kt.pos) - wg * kHalfN;  // this row's visible columns
-          if (__any_sync(0xffffffffu, nv < kHalfN)) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (c * 32 + e >= nv) s[c][e] = __float_as_uint(-INFINITY);
-          }
-          float mq[2];
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float x = __uint_as_float(s[c][0]);
-#pragma unroll
-            for (int e = 1; e < 31; e += 2)
-              x = max3f(x, __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
-            mq[c] = fmaxf(x, __uint_as_float(s[c][31]));
-          }
-          const float mxs = fmaxf(mq[0], mq[1]) * sl2;
-          // Lazy rescaling: a stale maximum stays while the new one exceeds it
-          // by at most 8 (log2 units), so P stays <= 256. A row's first visible
-          // key sets it (its accumulator holds zeros or is not written yet).
-          const bool first = m == -INFINITY;
-          const bool need = row_ok && !first && mxs > m + 8.f;  // (rows past the tile's last are another sequence's)
-          if (first) m = mxs;
-          if (__any_sync(0xffffffffu, need)) {
-            const float mn = first ? m : fmaxf(m, mxs);
-            const float alpha = first ? 1.f : ex2_approx(m - mn);
-            m = mn;
-            l *= alpha;
-            // The accumulator must hold every PV up to tile g-1: PV(g-2)
-            // completed before S(g) did, so one more completion of OREADY
-            // (parity of tile g-1) is all there is to wait for.
-            ok = mbar_wait_warp(bar(S::BAR_OREADY), (g - 1) & 1, abort_flag);
+        // Epilogue: merge the two halves, then O / l -> bf16 (the row's only split)
+        // or O, (m, l) -> fp32 partials. Warpgroup w writes output columns [64w, 64w + 64).
+        const bool alone = t.sp.total <= a.split_chunks;
+        const int h = t.hkv * a.group + (t.row0 + row_in_tile) - qr * a.group;
+        __nv_bfloat16* orow = a.o + (t.sq.q_begin + qr) * a.o_stride + (int64_t)h * kD + wg * kHalfN;
+        const int64_t prow = ((int64_t)t.item * a.splits + t.split) * kTileM + row_in_tile;
+        if (t.nkv > 0) {
+          ok = mbar_wait_warp(bar(S::BAR_OFULL), o_it & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          // O = ca * O_a + cb * O_b; a half without a visible key (m = -inf) counts
+          // nothing, and O_b may not have been written at all.
+          float ca, cb;
+          if (wg == 1) {
+            xch[row_in_tile] = make_float2(m, l);
+            mbar_arrive(bar(S::BAR_XML));
+            ok = mbar_wait_warp(bar(S::BAR_XF), o_it & 1, abort_flag);
             if (!ok) break;
-            tc_fence_after();
+            const float2 f = xch[row_in_tile];
+            ca = f.x;
+            cb = f.y;
+          } else {
+            ok = mbar_wait_warp(bar(S::BAR_XML), o_it & 1, abort_flag);
+            if (!ok) break;
+            const float2 o1 = xch[row_in_tile];
+            const float mm = fmaxf(m, o1.x);
+            const float fa = m == -INFINITY ? 0.f : ex2_approx(m - mm);
+            const float fb = o1.x == -INFINITY ? 0.f : ex2_approx(o1.x - mm);
+            const float sum = l * fa + o1.y * fb;
+            const float inv = !alone ? 1.f : sum == 0.f ? 0.f : 1.f / sum;  // no visible key: zero row
+            ca = fa * inv;
+            cb = fb * inv;
+            xch[row_in_tile] = make_float2(ca, cb);
+            mbar_arrive(bar(S::BAR_XF));
+            if (!alone && row_ok) a.part_ml[prow] = make_float2(mm, sum);
+          }
+          ++o_it;
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              uint32_t o[32];
-              tmem_ld32(tOwn + c * 32, o);
-              tmem_wait_ld();
+          for (int c = 0; c < 2; ++c) {
+            if (idle) break;
+            uint32_t oa[32], ob[32];
+            tmem_ld32(tOa + wg * kHalfN + c * 32, oa);
+            tmem_ld32(tOb + wg * kHalfN + c * 32, ob);
+            tmem_wait_ld();
+            if (row_ok) {
+              float v[32];
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-              tmem_st32(tOwn + c * 32, o);
+              for (int e = 0; e < 32; ++e) {
+                v[e] = ca != 0.f ? __uint_as_float(oa[e]) * ca : 0.f;
+                if (cb != 0.f) v[e] = fmaf(__uint_as_float(ob[e]), cb, v[e]);
+              }
+              if (alone) {
+                uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                  dst[q] = make_uint4(pack_bf16x2(v[8 * q + 0], v[8 * q + 1]), pack_bf16x2(v[8 * q + 2], v[8 * q + 3]),
+                                      pack_bf16x2(v[8 * q + 4], v[8 * q + 5]), pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
+              } else {
+                float4* dst = reinterpret_cast<float4*>(a.part_o + prow * kD + wg * kHalfN + c * 32);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) dst[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+              }
             }
           }
-          l += exp_store<2>(s, sl2, m == -INFINITY ? 0.f : m, tS);  // hidden columns give exact zeros
-          tmem_wait_st();
+          // O is read out; the next unit's first PV may overwrite it once every
+          // softmax warp arrives on its first P barrier (program order + fence).
+          tc_fence_before();
+        } else if (row_ok) {
+          // No keys at all: the output row is zero.
+          uint4* dst = reinterpret_cast<uint4*>(orow);
+          for (int v = 0; v < kHalfN / 8; ++v) dst[v] = make_uint4(0, 0, 0, 0);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(S::BAR_PFULL + sb));
       }
-      if (!ok) break;
-      // Epilogue: merge the two halves, then O / l -> bf16 (the row's only split)
-      // or O, (m, l) -> fp32 partials. Warpgroup w writes output columns [64w, 64w + 64).
-      const bool alone = t.sp.total <= a.split_chunks;
-      const int h = t.hkv * a.group + (t.row0 + row_in_tile) - qr * a.group;
-      __nv_bfloat16* orow = a.o + (t.sq.q_begin + qr) * a.o_stride + (int64_t)h * kD + wg * kHalfN;
-      const int64_t prow = ((int64_t)t.item * a.splits + t.split) * kTileM + row_in_tile;
-      if (t.nkv > 0) {
-        ok = mbar_wait_warp(bar(S::BAR_OFULL), o_it & 1, abort_flag);
-        if (!ok) break;
-        tc_fence_after();
-        // O = ca * O_a + cb * O_b; a half without a visible key (m = -inf) counts
-        // nothing, and O_b may not have been written at all.
-        float ca, cb;
-        if (wg == 1) {
-          xch[row_in_tile] = make_float2(m, l);
-          mbar_arrive(bar(S::BAR_XML));
-          ok = mbar_wait_warp(bar(S::BAR_XF), o_it & 1, abort_flag);
-          if (!ok) break;
-          const float2 f = xch[row_in_tile];
-          ca = f.x;
-          cb = f.y;
-        } else {
-          ok = mbar_wait_warp(bar(S::BAR_XML), o_it & 1, abort_flag);
-          if (!ok) break;
-          const float2 o1 = xch[row_in_tile];
-          const float mm = fmaxf(m, o1.x);
-          const float fa = m == -INFINITY ? 0.f : ex2_approx(m - mm);
-          const float fb = o1.x == -INFINITY ? 0.f : ex2_approx(o1.x - mm);
-          const float sum = l * fa + o1.y * fb;
-          const float inv = !alone ? 1.f : sum == 0.f ? 0.f : 1.f / sum;  // no visible key: zero row
-          ca = fa * inv;
-          cb = fb * inv;
-          xch[row_in_tile] = make_float2(ca, cb);
-          mbar_arrive(bar(S::BAR_XF));
-          if (!alone && row_ok) a.part_ml[prow] = make_float2(mm, sum);
-        }
-        ++o_it;
-#pragma unroll 1
-        for (int c = 0; c < 2; ++c) {
-          if (idle) break;
-          uint32_t oa[32], ob[32];
-          tmem_ld32(tOa + wg * kHalfN + c * 32, oa);
-          tmem_ld32(tOb + wg * kHalfN + c * 32, ob);
-          tmem_wait_ld();
-          if (row_ok) {
-            float v[32];
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              v[e] = ca != 0.f ? __uint_as_float(oa[e]) * ca : 0.f;
-              if (cb != 0.f) v[e] = fmaf(__uint_as_float(ob[e]), cb, v[e]);
-            }
-            if (alone) {
-              uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);
-#pragma unroll
-              for (int q = 0; q < 4; ++q)
-                dst[q] = make_uint4(pack_bf16x2(v[8 * q + 0], v[8 * q + 1]), pack_bf16x2(v[8 * q + 2], v[8 * q + 3]),
-                                    pack_bf16x2(v[8 * q + 4], v[8 * q + 5]), pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
-            } else {
-              float4* dst = reinterpret_cast<float4*>(a.part_o + prow * kD + wg * kHalfN + c * 32);
-#pragma unroll
-              for (int q = 0; q < 8; ++q) dst[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-            }
-          }
-        }
-        // O is read out; the next unit's first PV may overwrite it once every
-        // softmax warp arrives on its first P barrier (program order + fence).
-        tc_fence_before();
-      } else if (row_ok) {
-        // No keys at all: the output row is zero.
-        uint4* dst = reinterpret_cast<uint4*>(orow);
-        for (int v = 0; v < kHalfN / 8; ++v) dst[v] = make_uint4(0, 0, 0, 0);
-      }
-    }
     }
   }
 

@@ -556,7 +556,7 @@ def test_refusals():
     kernels = lib.dllm_attn_chunk_launches
     assert kernels(1, 1, 4, 4, 1, 100000, 0) == 2                # splits and their merge
     assert kernels(1, 64, 32, 32, 1, 64, 0) == 1
-    assert kernels(1, 1, 4, 4, 512, 100000, 0) == 3              # the expanded copy, splits, merge
+    assert kernels(1, 1, 4, 4, 1024, 100000, 0) == 3             # the expanded copy, splits, merge
     assert kernels(9, 1, 4, 4, 1, 64, 0) == -1
     q = torch.zeros(1, 4, 128, dtype=torch.bfloat16)
     cu = torch.tensor([0, 1], dtype=torch.int32)
