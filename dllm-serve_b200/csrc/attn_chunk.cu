@@ -268,35 +268,39 @@ DLLM_DEVICE void chunk_step(uint32_t ks, uint32_t vs, uint32_t scales, uint32_t 
         }
       }
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+    for (int c = 0; c < 2; ++c) {
+      uint32_t q[kN][4];
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
-        uint32_t q[4];
         if constexpr (kQInRegs<kN>) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) q[i] = qf[n][8 * h + 4 * c + i];
+          for (int i = 0; i < 4; ++i) q[n][i] = qf[n][8 * h + 4 * c + i];
         } else {
           const int row = 8 * n + g;
           const uint4 x = lds128(qs + row * 256 + (((8 * h + 2 * t + c) ^ (row & 1)) << 4));
-          q[0] = x.x, q[1] = x.y, q[2] = x.z, q[3] = x.w;
+          q[n][0] = x.x, q[n][1] = x.y, q[n][2] = x.z, q[n][3] = x.w;
         }
         if constexpr (kQuant && !kCodes) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) q[i] = f16_to_bf16(q[i], back[n]);
+          for (int i = 0; i < 4; ++i) q[n][i] = f16_to_bf16(q[n][i], back[n]);
         }
+      }
+      // (a product waits for the one before it into the same scores: kN * KT products apart)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
 #pragma unroll
           for (int kt = 0; kt < KT; ++kt) {
             const uint32_t(&k0)[8] = ka[kt][0];
             const uint32_t(&k1)[8] = ka[kt][1];
             const int x = 4 * c + 2 * i;
             if constexpr (kCodes)
-              mma16816_f16(s[kt][n], k0[x], k1[x], k0[x + 1], k1[x + 1], q[2 * i], q[2 * i + 1]);
+              mma16816_f16(s[kt][n], k0[x], k1[x], k0[x + 1], k1[x + 1], q[n][2 * i], q[n][2 * i + 1]);
             else
-              mma16816(s[kt][n], k0[x], k1[x], k0[x + 1], k1[x + 1], q[2 * i], q[2 * i + 1]);
+              mma16816(s[kt][n], k0[x], k1[x], k0[x + 1], k1[x + 1], q[n][2 * i], q[n][2 * i + 1]);
           }
-      }
+    }
   }
   // the value exponents of the chunk against the unit of O
   float ufac = 1.f, grow = 1.f;  // P times this; O times this
