@@ -677,22 +677,22 @@ __global__ void __launch_bounds__(kThreads, Cfg<kFmt, kN>::kCtas) attn_chunk_ker
     float mm = -INFINITY;
 #pragma unroll
     for (int x = 0; x < kWarps; ++x) mm = fmaxf(mm, ml[x * kRows + row].x);
+    const float least = mm == -INFINITY ? 0.f : mm;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float sum = 0.f;
-    if (mm != -INFINITY) {
 #pragma unroll
-      for (int x = 0; x < kWarps; ++x) {
-        const float2 s = ml[x * kRows + row];
-        const float f = ex2_approx(s.x - mm);
-        const float4 y = *reinterpret_cast<const float4*>(mo + ((size_t)x * kRows + row) * kD + d);
-        sum = fmaf(s.y, f, sum);
-        acc.x = fmaf(y.x, f, acc.x), acc.y = fmaf(y.y, f, acc.y);
-        acc.z = fmaf(y.z, f, acc.z), acc.w = fmaf(y.w, f, acc.w);
-      }
+    for (int x = 0; x < kWarps; ++x) {
+      const float2 s = ml[x * kRows + row];
+      const float f = ex2_approx(s.x - least);
+      const float4 y = *reinterpret_cast<const float4*>(mo + ((size_t)x * kRows + row) * kD + d);
+      sum = fmaf(s.y, f, sum);  // (a NaN sum stays, whatever its maximum)
+      acc.x = fmaf(y.x, f, acc.x), acc.y = fmaf(y.y, f, acc.y);
+      acc.z = fmaf(y.z, f, acc.z), acc.w = fmaf(y.w, f, acc.w);
     }
+    if (mm == -INFINITY) acc = make_float4(0.f, 0.f, 0.f, 0.f);  // no visible key here, or scores that leave no maximum
     if (alone) {
-      const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;  // a row without keys is zero
       const int r = (row0 + row) / a.group, h = hkv * a.group + (row0 + row) - r * a.group;
+      const float inv = sees_key(a, sq, r) ? 1.f / sum : 0.f;
       uint2 x;
       x.x = pack_bf16x2(acc.x * inv, acc.y * inv);
       x.y = pack_bf16x2(acc.z * inv, acc.w * inv);
@@ -733,8 +733,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<kFmt, kN>::kCtas) attn_chunk_ker
       acc.x = fmaf(y.x, f, acc.x), acc.y = fmaf(y.y, f, acc.y);
       acc.z = fmaf(y.z, f, acc.z), acc.w = fmaf(y.w, f, acc.w);
     }
-    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
     const int r = (row0 + row) / a.group, h = hkv * a.group + (row0 + row) - r * a.group;
+    const float inv = sees_key(a, sq, r) ? 1.f / sum : 0.f;
     uint2 out;
     out.x = pack_bf16x2(acc.x * inv, acc.y * inv);
     out.y = pack_bf16x2(acc.z * inv, acc.w * inv);
@@ -798,8 +798,8 @@ __global__ void __launch_bounds__(256) attn_chunk_merge_kernel(const __grid_cons
       }
     }
   }
-  const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
   const int r = (row0 + row) / a.group, h = hkv * a.group + (row0 + row) - r * a.group;
+  const float inv = sees_key(a, sq, r) ? 1.f / sum : 0.f;
   uint2 out;
   out.x = pack_bf16x2(acc.x * inv, acc.y * inv);
   out.y = pack_bf16x2(acc.z * inv, acc.w * inv);

@@ -44,6 +44,14 @@ DLLM_DEVICE Seq load_seq(const ChunkArgs& a, int b, bool report) {
   return s;
 }
 
+// Whether row i of the chunk sees a key; a row that sees none is zero. (A running
+// maximum of -infinity does not tell: the maxima drop NaN scores, so a row that
+// has met nothing else has it too, and must come out as NaN.)
+DLLM_DEVICE bool sees_key(const ChunkArgs& a, const Seq& s, int i) {
+  const int64_t L = (int64_t)s.nc + s.nk;
+  return (a.causal ? L - s.Lq + i + 1 : L) > 0;
+}
+
 // Key chunks of a row tile: the cached rows in chunks of KB keys, then the
 // fresh rows in chunks of FB, both cut at the last key any row of the tile
 // sees.

@@ -367,8 +367,8 @@ DLLM_DEVICE void softmax_pair(const ChunkArgs& a, uint32_t tmem, uint32_t bar0, 
       if (!mbar_wait_warp(bar(S::BAR_OFULL + wg), o_it & 1, abort_flag)) return;
       ++o_it;
       tc_fence_after();
-      const float inv = l == 0.f ? 0.f : 1.f / l;  // no visible key: zero row
-      const bool none = m == -INFINITY;
+      const float inv = 1.f / l;
+      const bool none = seen <= 0;  // no visible key: zero row
       const int qj = lane & 3;
       __nv_bfloat16* quad[4];
       bool live[4];
@@ -1061,7 +1061,7 @@ __global__ void __launch_bounds__(Layout<kFmt, kPair>::kThreads, 1)
             const float fa = m == -INFINITY ? 0.f : ex2_approx(m - mm);
             const float fb = o1.x == -INFINITY ? 0.f : ex2_approx(o1.x - mm);
             const float sum = l * fa + o1.y * fb;
-            const float inv = !alone ? 1.f : sum == 0.f ? 0.f : 1.f / sum;  // no visible key: zero row
+            const float inv = !alone ? 1.f : seen <= 0 ? 0.f : 1.f / sum;  // no visible key: zero row
             ca = fa * inv;
             cb = fb * inv;
             xch[row_in_tile] = make_float2(ca, cb);

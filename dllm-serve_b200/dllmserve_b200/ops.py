@@ -651,7 +651,9 @@ def chunk_attention(
 
     ``causal``: the chunk's rows are the last positions of the keys, and row i
     of Lq sees the first L - Lq + i + 1 of L keys; else every row sees all. A
-    row that sees no key is zero. Returns ``out`` (new by default)."""
+    row that sees no key is zero, one with a NaN among its scores is NaN. Values
+    at positions that a row does not see must be finite within the sequence's own
+    keys. Returns ``out`` (new by default)."""
     Hq, D, q_str = _chunk_rows("q", q)
     if (k is None) != (v is None) or (k is None) != (cu_seqlens_k is None):
         raise ValueError("k, v and cu_seqlens_k go together")

@@ -187,7 +187,8 @@ DLLM_API int dllm_load_kvcache_quant(void* key, int64_t key_stride, void* value,
  *     128], at most max_fresh per sequence), or none (k, v, cu_seqlens_k null).
  * With causal != 0 query row i of the chunk's Lq rows sees the first C_b + F_b - Lq + i + 1
  * keys (the chunk's rows are the last Lq positions), else all of them. A row that sees no
- * key is zero. Values at positions that a row does not see must be finite within the
+ * key is zero; a row with a NaN among the scores that it sees, or none above -inf, is NaN.
+ * Values at positions that a row does not see must be finite within the
  * sequence's own keys; what other slots hold does not matter.
  *
  * format: DLLM_KV_*; k_exp / v_exp as in dllm_store_kvcache_quant (null for bf16). Cache

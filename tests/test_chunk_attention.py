@@ -694,3 +694,100 @@ def test_sizes_at_the_ends_of_the_range(dev, fmt, nq):
         args, kw = c.args(dev)
         for causal in (True, False):
             c.check(_ops().chunk_attention(*args, causal=causal, **kw), causal)
+
+
+# hq, hkv, query rows, cached rows, fresh rows, kernels of a launch over bf16 and over quantised caches
+FORMS = [
+    (4, 4, [1, 3], [40, 9], [1, 3], 1, 1),                  # few rows, one split
+    (28, 4, [2, 1], [1100, 40], None, 1, 1),                # splits merged by their cluster
+    (4, 2, [8, 3], [9000, 70], [8, 3], 2, 2),               # splits merged by a second kernel
+    (4, 4, [32, 20], [60, 5], [32, 20], 1, 1),              # 32 rows
+    (3, 1, [50, 4], [30, 2], None, 1, 1),                   # one row tile per unit; more rows than keys
+    (4, 2, [40, 70], [1500, 20], [40, 70], 2, 2),           # its splits
+    (16, 16, [1000, 1100], [130, 20], [1000, 1100], 1, 2),  # two row tiles per unit; rows expanded once
+]
+
+
+def _form(seed, fmt, shape):
+    hq, hkv, nq, nc, nf, *kernels = FORMS[shape]
+    c = Case(seed + shape, fmt, hq, hkv, nq, nc, nf, shape % 2 == 0, page=32, spread=False)
+    args, kw = c.args("cuda:0")
+    kw["max_context"] = max(nc)
+    ops = _ops()
+    before = ops.LAUNCHES[0]
+    out = ops.chunk_attention(*args, causal=True, **kw)
+    assert ops.LAUNCHES[0] - before == kernels[fmt != "bf16"]
+    return c, args, kw, out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3", "int8"])
+@pytest.mark.parametrize("shape", range(len(FORMS)))
+def test_nan_queries(dev, fmt, shape):
+    """A query row with a NaN is NaN, unless it sees no key; the others do not change."""
+    c, args, kw, want = _form(600, fmt, shape)
+    n = sum(c.nq)
+    want = want[:n].clone()
+    bad = torch.zeros(n, c.hq, dtype=torch.bool)
+    bad[torch.arange(0, n, 3), torch.arange(0, n, 3) % c.hq] = True
+    bad[n - 1] = True
+    q = args[0].clone()
+    q[:n, :, 5][bad.to(dev)] = math.nan
+    got = _ops().chunk_attention(q, *args[1:], causal=True, **kw)[:n]
+    length = [a + (0 if c.nf is None else b) for a, b in zip(c.nc, c.nf or c.nc)]
+    sees = torch.cat([torch.arange(m) + (k - m + 1) > 0 for m, k in zip(c.nq, length)])
+    hit = (bad & sees[:, None]).to(dev)
+    assert hit.any() and torch.isnan(got[hit]).all()
+    got, want = got.float().masked_fill(hit[..., None], 0), want.float().masked_fill(hit[..., None], 0)
+    if max(c.nq) * (c.hq // c.hkv) <= (16 if fmt == "bf16" else 32):  # the kernel for few rows
+        assert torch.equal(got, want)
+    else:
+        # (the 128-row kernel rescales the rows of a warp together, so the bits may differ: both results
+        # are within (2^-8 + e) sum p |v| + 2^-8 |o|, e <= 2^-11, of the definition)
+        big = max([float(c.values[1][x.long()].abs().max()) for x in c.lists] + ([] if c.v is None else [float(c.v.abs().max())]))
+        assert (got - want).abs().max() <= 4.3 * 2.0 ** -8 * big
+    assert (got[~sees.to(dev)] == 0).all()
+    assert _ops().read_device_status(dev) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3", "int8"])
+@pytest.mark.parametrize("shape", range(len(FORMS)))
+def test_nan_keys(dev, fmt, shape):
+    """Every key of a KV head is NaN: so is every row that sees one, in that head alone."""
+    c, args, kw, want = _form(600, fmt, shape)
+    n, group = sum(c.nq), c.hq // c.hkv
+    want = want[:n].clone()
+    kc = args[1].clone()
+    if fmt == "bf16":
+        kc[:, :, 0] = math.nan
+    else:
+        kw["k_exp"][:, :, 0] = 255
+    if c.k is not None:
+        kw["k"][:, 0] = math.nan
+    got = _ops().chunk_attention(args[0], kc, *args[2:], causal=True, **kw)[:n]
+    length = [a + (0 if c.nf is None else b) for a, b in zip(c.nc, c.nf or c.nc)]
+    sees = torch.cat([torch.arange(m) + (k - m + 1) > 0 for m, k in zip(c.nq, length)]).to(dev)
+    assert torch.isnan(got[sees][:, :group]).all()
+    assert torch.equal(got[:, group:], want[:, group:])
+    assert (got[~sees] == 0).all()
+    assert _ops().read_device_status(dev) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", range(len(FORMS)))
+def test_scores_of_minus_infinity(dev, shape):
+    """Rows whose scores are all -inf have no softmax: NaN, as the definition gives."""
+    c, args, kw, want = _form(600, "bf16", shape)
+    n, group = sum(c.nq), c.hq // c.hkv
+    want = want[:n].clone()
+    args[0][:, :group] = args[0][:, :group].abs() + 1
+    args[1][:, :, 0] = -math.inf
+    if c.k is not None:
+        kw["k"][:, 0] = -math.inf
+    got = _ops().chunk_attention(*args, causal=True, **kw)[:n]
+    length = [a + (0 if c.nf is None else b) for a, b in zip(c.nc, c.nf or c.nc)]
+    sees = torch.cat([torch.arange(m) + (k - m + 1) > 0 for m, k in zip(c.nq, length)]).to(dev)
+    assert torch.isnan(got[sees][:, :group]).all()
+    assert torch.equal(got[:, group:], want[:, group:])
+    assert (got[~sees] == 0).all()
