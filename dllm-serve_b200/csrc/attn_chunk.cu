@@ -95,7 +95,8 @@ struct Cfg {
   static constexpr uint32_t kOffStages = 0;
   static constexpr uint32_t kOffScales = kOffStages + kWarps * kStages * kStageBytes;
   static constexpr uint32_t kOffRowFactor = kOffScales + kWarps * kStages * kScaleBytes;  // float per packed row
-  static constexpr uint32_t kOffQ = kOffRowFactor + kN * 8 * 4;
+  static constexpr uint32_t kOffBlind = kOffRowFactor + kN * 8 * 4;  // how many rows of the chunk see no key
+  static constexpr uint32_t kOffQ = kOffBlind + 16;
   static constexpr uint32_t kSmemBytes = kOffQ + kN * 8 * kD * 2;
   static_assert(kCtas * (kSmemBytes + 1024) <= 233472, "the CTAs do not fit an SM");
   // the merge buffers (per warp: rows x 128 floats, then rows float2) reuse the stages
@@ -567,6 +568,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<kFmt, kN>::kCtas) attn_chunk_ker
     if (i + 1 < kStages - 1) put_scales(i);
   }
 
+  // (kept in shared memory: a register less in the main loop)
+  if (threadIdx.x == 0) asm volatile("st.shared.s32 [%0], %1;" ::"r"(base + C::kOffBlind), "r"(blind_rows(a, sq)) : "memory");
   // Q rows, packed and swizzled (zero past the tile's rows); f16 with a row factor if the cache is quantised
   for (int i = threadIdx.x; i < kRows * 16; i += kThreads) {
     const int p = i >> 4, u = i & 15;
@@ -671,6 +674,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<kFmt, kN>::kCtas) attn_chunk_ker
     }
   __syncthreads();
   const bool alone = sp.total <= a.split_chunks;  // no other split has keys of this tile
+  int blind;
+  asm volatile("ld.shared.s32 %0, [%1];" : "=r"(blind) : "r"(base + C::kOffBlind));
   for (int i = threadIdx.x; i < kRows * (kD / 4); i += kThreads) {
     const int row = i / (kD / 4), d = (i % (kD / 4)) * 4;
     if (row >= rows) break;
@@ -692,7 +697,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kFmt, kN>::kCtas) attn_chunk_ker
     if (mm == -INFINITY) acc = make_float4(0.f, 0.f, 0.f, 0.f);  // no visible key here, or scores that leave no maximum
     if (alone) {
       const int r = (row0 + row) / a.group, h = hkv * a.group + (row0 + row) - r * a.group;
-      const float inv = sees_key(a, sq, r) ? 1.f / sum : 0.f;
+      const float inv = r >= blind ? 1.f / sum : 0.f;
       uint2 x;
       x.x = pack_bf16x2(acc.x * inv, acc.y * inv);
       x.y = pack_bf16x2(acc.z * inv, acc.w * inv);
@@ -734,7 +739,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kFmt, kN>::kCtas) attn_chunk_ker
       acc.z = fmaf(y.z, f, acc.z), acc.w = fmaf(y.w, f, acc.w);
     }
     const int r = (row0 + row) / a.group, h = hkv * a.group + (row0 + row) - r * a.group;
-    const float inv = sees_key(a, sq, r) ? 1.f / sum : 0.f;
+    const float inv = r >= blind ? 1.f / sum : 0.f;
     uint2 out;
     out.x = pack_bf16x2(acc.x * inv, acc.y * inv);
     out.y = pack_bf16x2(acc.z * inv, acc.w * inv);
@@ -799,7 +804,7 @@ __global__ void __launch_bounds__(256) attn_chunk_merge_kernel(const __grid_cons
     }
   }
   const int r = (row0 + row) / a.group, h = hkv * a.group + (row0 + row) - r * a.group;
-  const float inv = sees_key(a, sq, r) ? 1.f / sum : 0.f;
+  const float inv = r >= blind_rows(a, sq) ? 1.f / sum : 0.f;
   uint2 out;
   out.x = pack_bf16x2(acc.x * inv, acc.y * inv);
   out.y = pack_bf16x2(acc.z * inv, acc.w * inv);

@@ -44,12 +44,12 @@ DLLM_DEVICE Seq load_seq(const ChunkArgs& a, int b, bool report) {
   return s;
 }
 
-// Whether row i of the chunk sees a key; a row that sees none is zero. (A running
-// maximum of -infinity does not tell: the maxima drop NaN scores, so a row that
-// has met nothing else has it too, and must come out as NaN.)
-DLLM_DEVICE bool sees_key(const ChunkArgs& a, const Seq& s, int i) {
-  const int64_t L = (int64_t)s.nc + s.nk;
-  return (a.causal ? L - s.Lq + i + 1 : L) > 0;
+// How many of the chunk's first rows see no key; those are zero. (A maximum of
+// -infinity does not tell: the maxima drop NaN scores, and a row that has met
+// nothing else is NaN.)
+DLLM_DEVICE int blind_rows(const ChunkArgs& a, const Seq& s) {
+  const int L = s.nc + s.nk;  // at most 2^30
+  return a.causal ? s.Lq - L : L > 0 ? 0 : s.Lq;
 }
 
 // Key chunks of a row tile: the cached rows in chunks of KB keys, then the
