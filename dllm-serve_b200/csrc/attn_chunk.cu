@@ -12,8 +12,8 @@
 // conversion per pair (to bf16 it takes four), so both products use f16
 // operands, and powers of two keep that as exact as bf16:
 //   Q: each row is scaled so that its largest element lies in [2^14, 2^15).
-//      bf16 values fit f16's 11 bits; only elements 2^-38 times smaller than
-//      the row's largest lose bits.
+//      bf16 values fit f16's 11 bits; elements below 2^-31 of the row's largest
+//      lose some, an error of at most 2^-39 of that largest.
 //   P: p * 2^(e_v - E + 15), E the largest value exponent this warp has met
 //      (O is in units of 2^(E - 15) and is rescaled when E grows). p <= 1, so
 //      nothing overflows; down to 2^-14 these keep 11 bits, and below that the
@@ -77,8 +77,9 @@ constexpr uint32_t kScaleBytes = 34 * 8;  // of a stage: 32 (K, V) scales, the l
 constexpr int kNoExp = -(1 << 30);        // no value exponent met
 constexpr int kClusterSplits = 8;         // splits that merge within a cluster
 // A scaled Q (below 2^15) times codes (at most 448) over 128 dimensions is below 2^31; with keys'
-// 2^e (e <= 121) lowered by this the scores stay finite, whatever the cache holds.
-constexpr float kKeyDown = 0x1p-24f;
+// 2^e (e <= 121) lowered by 2^-kKeyDown the products stay finite, whatever the cache holds. The row's
+// factor makes up for it (fit_row_factors() where that is no float).
+constexpr int kKeyDown = 24;
 
 template <int kFmt>
 constexpr int chunk_keys() { return kFmt == kFmtBf16 ? 16 : 32; }
@@ -96,6 +97,7 @@ struct Cfg {
   static constexpr uint32_t kOffScales = kOffStages + kWarps * kStages * kStageBytes;
   static constexpr uint32_t kOffRowFactor = kOffScales + kWarps * kStages * kScaleBytes;  // float per packed row
   static constexpr uint32_t kOffBlind = kOffRowFactor + kN * 8 * 4;  // how many rows of the chunk see no key
+  static constexpr uint32_t kOffDown = kOffBlind + 4;                 // float: what the keys' 2^e are lowered by
   static constexpr uint32_t kOffQ = kOffBlind + 16;
   static constexpr uint32_t kSmemBytes = kOffQ + kN * 8 * kD * 2;
   static_assert(kCtas * (kSmemBytes + 1024) <= 233472, "the CTAs do not fit an SM");
@@ -158,6 +160,9 @@ DLLM_DEVICE float4 cluster_ld4(uint32_t a, int rank) {
   return v;
 }
 
+// 2^e, 0 below the normal range.
+DLLM_DEVICE float pow2(int e) { return __int_as_float(max(e + 127, 0) << 23); }
+
 // Four codes -> two words of f16 pairs, unscaled (exact).
 template <int kFmt>
 DLLM_DEVICE void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
@@ -185,8 +190,6 @@ DLLM_DEVICE uint32_t f16_to_bf16(uint32_t w, float f) {
   const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w));
   return pack_bf16x2(x.x * f, x.y * f);
 }
-// 2^e, 0 below the normal range.
-DLLM_DEVICE float pow2(int e) { return __int_as_float(max(e + 127, 0) << 23); }
 
 // Shared-memory swizzles (16-byte units of a row) that make the reads of the
 // header comment free of bank conflicts: eight lanes read two K rows x four
@@ -444,6 +447,37 @@ DLLM_DEVICE void chunk_step(uint32_t ks, uint32_t vs, uint32_t scales, uint32_t 
   }
 }
 
+// A row's scores are its products (2^kKeyDown too small) times scale_log2 2^kKeyDown 2^-up, Q having been
+// scaled by 2^up. For |q| from 2^121 on, at a scale of 128^-0.5, that factor is no float. The tile's keys are
+// then lowered by x powers of two less, x what its largest factor needs: that row's products can only
+// overflow where its scores do. The other rows' Q is lowered by 2^-x instead, so their products and
+// factors stay as they are (bits are lost from 2^-(31 - x) of the largest element on). Every thread of the
+// CTA calls this, with row factors and Q in shared memory; returns x. (Two factors per score in the main
+// loop instead took 184 us for 178: eight int8 contexts of 16,384 rows, 32 heads; this form 179.)
+template <int kRows>
+DLLM_DEVICE int fit_row_factors(float* factor, uint32_t qs, float scale_log2, int lane) {
+  const float all = scale_log2 * pow2(kKeyDown);
+  float top = 0.f;
+  for (int p = lane; p < kRows; p += 32) top = fmaxf(top, factor[p]);
+  if (!__any_sync(0xffffffffu, all * top == INFINITY)) return 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const int x = min((__float_as_int(all) >> 23) + (__float_as_int(top) >> 23) - 2 * 127 - 126, kKeyDown);
+  __half2 f = __float2half2_rn(pow2(-x));
+  for (int i = threadIdx.x; i < kRows * 64; i += kThreads) {
+    if (all * factor[i >> 6] == INFINITY) continue;
+    uint32_t w;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(qs + i * 4));
+    const __half2 y = __hmul2(*reinterpret_cast<__half2*>(&w), f);
+    asm volatile("st.shared.u32 [%0], %1;" ::"r"(qs + i * 4), "r"(*reinterpret_cast<const uint32_t*>(&y)) : "memory");
+  }
+  __syncthreads();  // every thread has read the factors
+  for (int p = threadIdx.x; p < kRows; p += kThreads)
+    if (all * factor[p] != INFINITY) factor[p] *= pow2(x);
+  __syncthreads();
+  return x;
+}
+
 template <int kFmt, int kN>
 __global__ void __launch_bounds__(kThreads, Cfg<kFmt, kN>::kCtas) attn_chunk_kernel(const __grid_constant__ ChunkArgs a) {
   constexpr int KB = chunk_keys<kFmt>();
@@ -543,16 +577,16 @@ __global__ void __launch_bounds__(kThreads, Cfg<kFmt, kN>::kCtas) attn_chunk_ker
     }
     cp_async_commit();
   };
-  // Scales of chunk i, issued by the last issue(): 2^(e - 24) of each key, 2^(e - e_max + 15) of
+  // Scales of chunk i, issued by the last issue(): 2^e of each key times `down`, 2^(e - e_max + 15) of
   // each value, then the values' largest exponent.
-  auto put_scales = [&](int i) {
+  auto put_scales = [&](int i, float down) {
     if constexpr (kQuant) {
       if (i < n_mine && c_begin + warp + i * kWarps < sp.cached) {
         const uint32_t at = scale0 + (i % kStages) * kScaleBytes;
         const int ev = (int)pend_v - 127;
         const bool live = pend_v != 0 && pend_v != kNanByte;
         const int hi = __reduce_max_sync(0xffffffffu, live ? ev : kNoExp);
-        const float2 x = make_float2(exp_scale(pend_k) * kKeyDown, live ? pow2(ev - hi + 15) : exp_scale(pend_v));
+        const float2 x = make_float2(exp_scale(pend_k) * down, live ? pow2(ev - hi + 15) : exp_scale(pend_v));
         asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at + lane * 8), "f"(x.x), "f"(x.y) : "memory");
         if (lane == 0) asm volatile("st.shared.s32 [%0], %1;" ::"r"(at + 32 * 8), "r"(hi) : "memory");
       }
@@ -565,11 +599,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<kFmt, kN>::kCtas) attn_chunk_ker
   for (int i = 0; i < kStages - 1; ++i) {
     issue(i, raw);
     raw = lookup(i + 1);
-    if (i + 1 < kStages - 1) put_scales(i);
+    if (i + 1 < kStages - 1) put_scales(i, pow2(-kKeyDown));
   }
 
-  // (kept in shared memory: a register less in the main loop)
-  if (threadIdx.x == 0) asm volatile("st.shared.s32 [%0], %1;" ::"r"(base + C::kOffBlind), "r"(blind_rows(a, sq)) : "memory");
+  if (threadIdx.x == 0) {  // (in shared memory: fewer registers in the main loop)
+    asm volatile("st.shared.s32 [%0], %1;" ::"r"(base + C::kOffBlind), "r"(blind_rows(a, sq)) : "memory");
+    if constexpr (kQuant) asm volatile("st.shared.f32 [%0], %1;" ::"r"(base + C::kOffDown), "f"(pow2(-kKeyDown)) : "memory");
+  }
   // Q rows, packed and swizzled (zero past the tile's rows); f16 with a row factor if the cache is quantised
   for (int i = threadIdx.x; i < kRows * 16; i += kThreads) {
     const int p = i >> 4, u = i & 15;
@@ -599,6 +635,18 @@ __global__ void __launch_bounds__(kThreads, Cfg<kFmt, kN>::kCtas) attn_chunk_ker
                  : "memory");
   }
   __syncthreads();
+  float* factor = reinterpret_cast<float*>(smem + C::kOffRowFactor);
+  int less = 0;
+  if constexpr (kQuant) {
+    less = fit_row_factors<kRows>(factor, base + C::kOffQ, a.scale_log2, lane);
+    if (less > 0) {
+      if (threadIdx.x == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(base + C::kOffDown), "f"(pow2(less - kKeyDown)) : "memory");
+#pragma unroll
+      for (int i = 0; i + 1 < kStages - 1; ++i)  // scales that are there already
+        *reinterpret_cast<float*>(smem + (scale0 - base) + i * kScaleBytes + lane * 8) *= pow2(less);
+      __syncthreads();
+    }
+  }
   uint32_t qf[kN][16] = {};
   float back[kN];
   const int64_t L = (int64_t)sq.nc + sq.nk;
@@ -611,7 +659,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<kFmt, kN>::kCtas) attn_chunk_ker
       const uint4 x = lds128(base + C::kOffQ + row * 256 + (((8 * (hc >> 1) + 2 * t + (hc & 1)) ^ (row & 1)) << 4));
       qf[n][4 * hc] = x.x, qf[n][4 * hc + 1] = x.y, qf[n][4 * hc + 2] = x.z, qf[n][4 * hc + 3] = x.w;
     }
-    const float* factor = reinterpret_cast<const float*>(smem + C::kOffRowFactor);
     back[n] = kQuant ? factor[row] : 1.f;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -620,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kFmt, kN>::kCtas) attn_chunk_ker
       w.m[n][r] = -INFINITY;
       w.l[n][r] = 0.f;
       w.seen[n][r] = (int)(a.causal ? min(L, max((int64_t)0, L - sq.Lq + i + 1)) : L);
-      w.rf[n][r] = kQuant ? a.scale_log2 / kKeyDown * factor[p] : a.scale_log2;
+      w.rf[n][r] = kQuant ? a.scale_log2 * pow2(kKeyDown - less) * factor[p] : a.scale_log2;
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -631,7 +678,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<kFmt, kN>::kCtas) attn_chunk_ker
   const int seen_by_all = (int)(a.causal ? min(L, max((int64_t)0, L - sq.Lq + row0 / a.group + 1)) : L);
 
   for (int i = 0; i < n_mine; ++i) {
-    put_scales(i + kStages - 2);
+    float down = 0.f;
+    if constexpr (kQuant) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(down) : "r"(base + C::kOffDown));
+    put_scales(i + kStages - 2, down);
     cp_async_wait<kStages - 2>();
     __syncwarp();  // chunk i has arrived for every lane, and no lane still reads chunk i - 1
     issue(i + kStages - 1, raw);

@@ -791,3 +791,37 @@ def test_scores_of_minus_infinity(dev, shape):
     assert torch.isnan(got[sees][:, :group]).all()
     assert torch.equal(got[:, group:], want[:, group:])
     assert (got[~sees] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3", "int8"])
+@pytest.mark.parametrize("nq", [1, 8, 16, 40])
+@pytest.mark.parametrize("dk", [-90, 100])
+def test_queries_at_the_end_of_the_range(dev, fmt, nq, dk):
+    """Every other row has an element of 2^108 where its head's keys are zero,
+    with a scale of 2^10: the scores are ordinary (keys of 2^-90), or those of
+    the rows between are and the large rows' are zero (keys of 2^100)."""
+    c = Case(86, fmt, 4, 2, [nq, 2], [200, 33], [nq, 2], False, spread=False)
+    up = lambda t, e: (t.double() * 2.0 ** e).to(torch.bfloat16)  # noqa: E731
+    used = c.slots.long()
+    if fmt == "bf16":
+        rows = c.caches[0].view(-1, 2, D)
+        rows[used] = up(rows[used], dk)
+        c.values[0][used] = rows[used].double()
+    else:
+        byte = c.exps[0].view(-1, 2)[used].int() + dk
+        assert byte.min() >= 27 and byte.max() <= 246
+        c.exps[0].view(-1, 2)[used] = byte.to(torch.uint8)
+        c.values[0][used] *= 2.0 ** dk
+    c.caches[0].view(-1, 2, D).view(torch.int8 if fmt != "bf16" else torch.bfloat16)[used, :, :1] = 0
+    c.values[0][used, :, 0] = 0
+    c.k = up(c.k, dk)
+    c.k[:, :, 0] = 0
+    c.q = up(torch.round(c.q.float() * 4) / 4, -dk - 13)  # (multiples of 2^-33 of the largest: exact in f16)
+    if dk > 0:
+        c.q[::2] = 0
+    c.q[::2, :, 0] = 2.0 ** 108
+    args, kw = c.args(dev)
+    for causal in (True, False):
+        c.check(_ops().chunk_attention(*args, 1024.0, causal=causal, **kw), causal, scale=1024.0)
+    assert _ops().read_device_status(dev) == 0
