@@ -825,3 +825,38 @@ def test_queries_at_the_end_of_the_range(dev, fmt, nq, dk):
     for causal in (True, False):
         c.check(_ops().chunk_attention(*args, 1024.0, causal=causal, **kw), causal, scale=1024.0)
     assert _ops().read_device_status(dev) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("tables", [True, False])
+def test_expanded_rows_and_splits(dev, fmt, tables):
+    """Rows of a quantised cache expanded once, with keys split between units:
+    the partial results lie behind the expanded copy in one workspace."""
+    nq, nc = [130, 160], [1500, 1300]
+    c = Case(87, fmt, 14, 2, nq, nc, None if tables else nq, tables, page=64, spread=False)
+    args, kw = c.args(dev)
+    from dllmserve_b200 import _native
+
+    sizes = (_native.KV_E4M3 if fmt == "e4m3" else _native.KV_INT8, 2, 14, 2, max(nq), max(nc), 0 if tables else max(nq))
+    assert _native.lib().dllm_attn_chunk_launches(*sizes) == 3  # the expansion, the units, the merge
+    for causal in (True, False):
+        out = torch.full(c.q.shape, 5.0, dtype=torch.bfloat16, device=dev)
+        _ops().chunk_attention(*args, causal=causal, max_context=max(nc), out=out, **kw)
+        c.check(out, causal)
+        assert (out[sum(nq):] == 5).all()
+        again = _ops().chunk_attention(*args, causal=causal, max_context=max(nc), **kw)
+        assert torch.equal(again[:sum(nq)], out[:sum(nq)])
+    assert _ops().read_device_status(dev) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("nq", [[1, 3], [8, 5], [32, 20], [33, 1, 140]])
+def test_fresh_rows_over_an_empty_quantised_cache(dev, fmt, nq):
+    """Contexts of length zero in every kernel that reads codes: the fresh rows alone."""
+    c = Case(88, fmt, 6, 6, nq, [0] * len(nq), nq, True)
+    args, kw = c.args(dev)
+    for causal in (True, False):
+        c.check(_ops().chunk_attention(*args, causal=causal, **kw), causal)
+    assert _ops().read_device_status(dev) == 0
