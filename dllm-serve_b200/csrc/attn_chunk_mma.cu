@@ -1042,8 +1042,9 @@ __global__ void __launch_bounds__(Layout<kFmt, kPair>::kThreads, 1)
           ok = mbar_wait_warp(bar(S::BAR_OFULL), o_it & 1, abort_flag);
           if (!ok) break;
           tc_fence_after();
-          // O = ca * O_a + cb * O_b; a half without a visible key (m = -inf) counts
-          // nothing, and O_b may not have been written at all.
+          // O = ca * O_a + cb * O_b. A half without a visible key (m = -inf) counts nothing: factor
+          // -1, its accumulator is not read (O_b may not have been written at all). Where both
+          // have none above -inf, but the row sees keys, the factors come out as NaN.
           float ca, cb;
           if (wg == 1) {
             xch[row_in_tile] = make_float2(m, l);
@@ -1062,8 +1063,9 @@ __global__ void __launch_bounds__(Layout<kFmt, kPair>::kThreads, 1)
             const float fb = o1.x == -INFINITY ? 0.f : ex2_approx(o1.x - mm);
             const float sum = l * fa + o1.y * fb;
             const float inv = !alone ? 1.f : seen <= 0 ? 0.f : 1.f / sum;  // no visible key: zero row
-            ca = fa * inv;
-            cb = fb * inv;
+            const bool none = !alone || seen <= 0 || mm > -INFINITY;
+            ca = none && m == -INFINITY ? -1.f : fa * inv;
+            cb = none && o1.x == -INFINITY ? -1.f : fb * inv;
             xch[row_in_tile] = make_float2(ca, cb);
             mbar_arrive(bar(S::BAR_XF));
             if (!alone && row_ok) a.part_ml[prow] = make_float2(mm, sum);
@@ -1080,8 +1082,8 @@ __global__ void __launch_bounds__(Layout<kFmt, kPair>::kThreads, 1)
               float v[32];
 #pragma unroll
               for (int e = 0; e < 32; ++e) {
-                v[e] = ca != 0.f ? __uint_as_float(oa[e]) * ca : 0.f;
-                if (cb != 0.f) v[e] = fmaf(__uint_as_float(ob[e]), cb, v[e]);
+                v[e] = ca == -1.f ? 0.f : __uint_as_float(oa[e]) * ca;
+                if (cb != -1.f) v[e] = fmaf(__uint_as_float(ob[e]), cb, v[e]);
               }
               if (alone) {
                 uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);

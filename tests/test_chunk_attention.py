@@ -860,3 +860,29 @@ def test_fresh_rows_over_an_empty_quantised_cache(dev, fmt, nq):
     for causal in (True, False):
         c.check(_ops().chunk_attention(*args, causal=causal, **kw), causal)
     assert _ops().read_device_status(dev) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3", "int8"])
+@pytest.mark.parametrize("nq", [[1], [8], [32], [100], [600, 600]])
+def test_nan_value_of_small_weight(dev, fmt, nq):
+    """A visible value that is NaN makes the row NaN, however far its score lies below the largest."""
+    c = Case(89, fmt, 16, 16, nq, [128] * len(nq), None, True, page=128, spread=False)
+    c.q = c.q.abs() + 1
+    at = c.slots.long()
+    if fmt == "bf16":
+        keys = c.caches[0].view(-1, 16, D)
+        keys[at] = keys[at].abs()
+        keys[at[::128][:, None] + torch.arange(64)] = -32.0  # scores of -360 and less against at least 0
+        c.caches[1].view(-1, 16, D)[at[3::128], 5] = math.nan
+    else:
+        codes = c.caches[0].view(-1, 16, D)
+        codes[at] = codes[at].float().abs().to(codes.dtype)
+        low = at[::128][:, None] + torch.arange(64)
+        codes[low] = torch.tensor(-1.0).to(codes.dtype)
+        c.exps[0].view(-1, 16)[low] = 127 + 5
+        c.exps[1].view(-1, 16)[at[3::128], 5] = 255
+    args, kw = c.args(dev)
+    out = _ops().chunk_attention(*args, causal=False, **kw)[:sum(nq)]
+    assert torch.isnan(out[:, 5]).all()
+    assert torch.isfinite(out[:, :5]).all() and torch.isfinite(out[:, 6:]).all()
