@@ -35,9 +35,9 @@
 // tcgen05 kernel writes them to shared memory first.
 //
 // Measured, decode (one row, 32 heads): 8 contexts of 4,096-32,768 rows bf16 350
-// us, 6.6 TB/s, e4m3 199 us, 5.9 TB/s (of 16,384 rows each 170 us, 6.4 TB/s):
+// us, 6.6 TB/s, e4m3 202 us, 5.8 TB/s (of 16,384 rows each 170 us, 6.4 TB/s):
 // the cache's bytes, where lengths are even. 32 contexts of 128-1,024 bf16 rows,
-// 28/4 heads: 13.5 us, 2.8 TB/s: a launch, one split's chunks and the merge one
+// 28/4 heads: 14.7 us, 2.6 TB/s: a launch, one split's chunks and the merge one
 // after another. 8 x 32 rows over 1,144 e4m3 rows: 42.5 us: with eight warps an SM
 // the latencies of conversions and products, one launch not filling the last
 // seventh of the SMs' places.

@@ -40,9 +40,8 @@ struct ChunkArgs {
   int max_q;
   int max_fresh;           // no sequence has more fresh rows
   int B;
-  int Hq;
   int Hkv;
-  int group;               // Hq / Hkv
+  int group;               // Hq / Hkv (Hq query heads)
   float scale_log2;        // softmax_scale * log2(e)
   int causal;
   __nv_bfloat16* o;

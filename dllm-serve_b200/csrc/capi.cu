@@ -610,7 +610,6 @@ int dllm_attn_chunk_fwd(const dllm_chunk_args* args) {
   a.max_q = max_seqlen_q;
   a.max_fresh = max_fresh;
   a.B = batch;
-  a.Hq = num_heads;
   a.Hkv = num_kv_heads;
   a.group = num_heads / num_kv_heads;
   a.scale_log2 = p.softmax_scale * 1.4426950408889634f;

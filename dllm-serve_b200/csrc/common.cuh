@@ -24,7 +24,7 @@ enum DeviceError : int32_t {
   kDevWaitTimeout = 2,        // an mbarrier wait exceeded its time limit
   kDevBadSequence = 3,        // inconsistent per-sequence metadata
   kDevPositionOutOfRange = 4, // a rotary position outside the cos/sin cache (row zeroed)
-  kDevNonFinite = 5,          // a NaN or infinity was quantised (stored saturated)
+  kDevNonFinite = 5,          // an infinity (stored saturated) or a NaN (its row marked) was quantised
 };
 
 DLLM_DEVICE void set_error(int32_t* err, int32_t code) {

@@ -141,9 +141,6 @@ DLLM_DEVICE int cand_token(int c, int blk_start, int blk_len) {
   return c < blk_start ? c : c + blk_len;
 }
 
-// kGroup (head_select only): more than one query head per KV head. The two
-// cases are separate instantiations so that the grouped scoring's registers
-// do not cost the single-head scoring loop.
 // Writes a selected head row (16 lanes x 8 bf16 each of K and V) into a slot of
 // a quantised cache. Every lane of `mask`, the row's 16 lanes, takes part;
 // dst < 0: nothing is written.
@@ -164,6 +161,9 @@ DLLM_DEVICE void put_quantised(const SelectArgs& a, uint4 k, uint4 v, int64_t ds
   }
 }
 
+// kGroup (head_select only): more than one query head per KV head. The two
+// cases are separate instantiations so that the grouped scoring's registers
+// do not cost the single-head scoring loop. kFmt: the cache's format.
 template <bool kHeadSelect, bool kGroup, int kFmt>
 __global__ void __launch_bounds__(kThreads, 2) select_kv_kernel(SelectArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
